@@ -425,6 +425,91 @@ int32_t riallm_cuda_attention(riallm_ctx* ctx, const void* q, const void* k_cach
 int32_t riallm_cuda_linear_bf16(riallm_ctx* ctx, const void* x, const void* w, void* y, int32_t M,
                                 int32_t N, int32_t K, void* stream);
 
+/* ---------------------------------------------- paged key-value cache
+ * The contiguous cache above holds S_max positions per sequence, used or
+ * not. A paged cache holds, per layer, pools k_pages and v_pages
+ * [num_pages, nkv, page_size, d] (bf16, 16-byte aligned), and the sequences'
+ * pages are named by page_table: entry b * table_stride + i is the page of
+ * positions [i * page_size, (i + 1) * page_size) of sequence b, i <
+ * max_pages (int32, on the device). An entry outside [0, num_pages) is a
+ * page that the sequence does not hold: its positions are neither written
+ * nor read. One page may stand in several sequences' tables (a shared
+ * prefix) as long as no call appends to it. page_size is 16, 32, 64 or 128;
+ * d is 64 or 128; nh / nkv at most 16. No riallm counterpart: its KVCACHE
+ * (src/model.rs:15-38) is one contiguous tensor per layer. These functions
+ * leave the calling thread's current device as it was. */
+
+/* Host-only helper (no device work; page_table is host memory here): the
+ * row of a pool, viewed as [num_pages * nkv * page_size, d], that holds
+ * `position` of sequence b for kv_head; -1 where the sequence holds none. */
+int64_t riallm_paged_row(const int32_t* page_table, int64_t table_stride, int32_t max_pages, int32_t num_pages,
+                         int32_t nkv, int32_t page_size, int32_t b, int32_t kv_head, int64_t position);
+
+/* riallm_cuda_rope_kv_append into pages: rotary embedding
+ * (src/model.rs:1002-1071) of the q and k heads of qkv
+ * [B*T, (nh + 2*nkv) * d] at position pos[b] + t; q to q_out [B*T, nh*d],
+ * rotated k and the v heads into the pages. The angle position * inv_freq[i]
+ * is not rounded to float32 (riallm's float32 product is 6e-3 off at position
+ * 100000). A position outside [0, max_pages * page_size), or in a page that
+ * the sequence does not hold, writes nothing to the pools. Two rows that are
+ * given the same place of a page leave either's values there. */
+int32_t riallm_cuda_rope_paged_append(riallm_ctx* ctx, const void* qkv, const int32_t* pos,
+                                      const int32_t* page_table, int64_t table_stride, int32_t max_pages,
+                                      int32_t B, int32_t T, int32_t nh, int32_t nkv, int32_t d,
+                                      const float* inv_freq, void* q_out, void* k_pages, void* v_pages,
+                                      int32_t num_pages, int32_t page_size, void* stream);
+
+/* Bytes of workspace that riallm_cuda_paged_attention needs for a call of
+ * this shape on the context's device (0: none). */
+uint64_t riallm_cuda_paged_attention_workspace(const riallm_ctx* ctx, int32_t B, int32_t T, int32_t nh,
+                                               int32_t nkv, int32_t d, int32_t max_pages, int32_t page_size);
+
+/* riallm_cuda_attention over pages: row b*T + t, at position
+ * p = pos[b] + t, attends the held positions j <= p (and below max_pages *
+ * page_size); with window > 0 only those with j > p - window or j < sinks.
+ * Scores q.k / sqrt(d), softmax and the weighted sum of v in float32; q and
+ * out are [B*T, nh*d] bf16, 16-byte aligned. A row that sees nothing
+ * (p < 0, no page held) is zero. What the pools hold at positions that a row
+ * does not see, infinities and NaN among it, does not change that row.
+ * The workspace is the caller's (256-byte aligned), needs no initial values,
+ * and is free again when the call's work is done on `stream`; calls that may
+ * overlap need one each. Nothing else is shared between calls. */
+int32_t riallm_cuda_paged_attention(riallm_ctx* ctx, const void* q, const void* k_pages, const void* v_pages,
+                                    const int32_t* pos, const int32_t* page_table, int64_t table_stride,
+                                    int32_t max_pages, int32_t B, int32_t T, int32_t nh, int32_t nkv, int32_t d,
+                                    int32_t num_pages, int32_t page_size, int32_t window, int32_t sinks, void* out,
+                                    void* workspace, uint64_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------ drafted tokens
+ * Bytes of workspace that riallm_cuda_verify_draft needs (0: none). */
+uint64_t riallm_cuda_verify_draft_workspace(const riallm_ctx* ctx, int32_t B, int32_t n, int32_t V);
+
+/* Verifies up to n drafted tokens per sequence and takes one more, from
+ * given uniform numbers in [0, 1). No riallm counterpart (its generate,
+ * src/model.rs:1223-1270, takes the argmax one token at a time).
+ * logits [B, n + 1, V] (float32 or bf16): row i gives p_i =
+ * softmax(logits / temperature[b]), the distribution of the token at draft
+ * position i; draft_tokens [B, n]; draft_probs [B, n, V] float32: the
+ * distributions q_i that the drafts were drawn from, or NULL where each was
+ * chosen outright (q_i = 1 at the draft). Draft x_i is accepted when
+ * accept_u[b, i] * q_i(x_i) < p_i(x_i), until the first that is not. A draft
+ * outside [0, V) ends its sequence's drafts. Then one token is sampled with
+ * sample_u[b] by inverse CDF, the lowest token whose cumulative weight
+ * exceeds sample_u * total: from max(0, p_i - q_i) after a rejection (from
+ * p_i if that is zero throughout), from p_i otherwise. temperature 0 or less,
+ * and a row that holds a NaN, +inf or -inf throughout, puts all of p_i on
+ * the lowest token of the maximum (NaN left out).
+ * tokens [B, n + 1] receives the accepted drafts, the sampled token, then
+ * -1; accepted [B] the number of accepted drafts. p, its sums and the
+ * comparisons are 64-bit, and results do not depend on the order in which
+ * blocks run. n <= 255; with n == 0 (one sampled token per sequence)
+ * draft_tokens and accept_u may be NULL. Workspace as above. */
+int32_t riallm_cuda_verify_draft(riallm_ctx* ctx, const void* logits, int32_t logits_dtype,
+                                 const int32_t* draft_tokens, const float* draft_probs, const float* temperature,
+                                 const float* accept_u, const float* sample_u, int32_t B, int32_t n, int32_t V,
+                                 int32_t* tokens, int32_t* accepted, void* workspace, uint64_t workspace_bytes,
+                                 void* stream);
+
 int32_t riallm_cuda_profile_enable(riallm_ctx* ctx, int32_t enable);
 int32_t riallm_cuda_profile_read(riallm_ctx* ctx, float* ms_per_phase,
                                  uint64_t* calls);

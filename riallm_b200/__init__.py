@@ -31,6 +31,7 @@ __all__ = [
     "compress_layer_state_dict", "dequantize_layer_state_dict", "apply_moe", "route", "Context",
     "RiallmError", "ModelLoadingError", "MemoryError_", "ConfigError", "QuantizationError",
     "CudaError", "TimeoutError_", "lib", "AutoModel", "ModelConfig",
+    "PagedKVCache", "paged_attention", "rope_paged_append", "verify_draft",
 ]
 
 
@@ -86,6 +87,7 @@ class CMoeWeights(ctypes.Structure):
 
 # Every symbol include/riallm_cuda.h declares: name -> (restype, argtypes).
 _i32, _u32, _u64, _vp = ctypes.c_int32, ctypes.c_uint32, ctypes.c_uint64, ctypes.c_void_p
+_i64 = ctypes.c_int64
 _pp = ctypes.POINTER(ctypes.c_void_p)
 SIGNATURES = {
     "riallm_cuda_abi_version": (_i32, []),
@@ -147,6 +149,15 @@ SIGNATURES = {
                                           _i32, _vp]),
     "riallm_cuda_attention": (_i32, [_vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _vp, _vp]),
     "riallm_cuda_linear_bf16": (_i32, [_vp, _vp, _vp, _vp, _i32, _i32, _i32, _vp]),
+    "riallm_paged_row": (_i64, [_vp, _i64, _i32, _i32, _i32, _i32, _i32, _i32, _i64]),
+    "riallm_cuda_rope_paged_append": (_i32, [_vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _i32, _i32, _vp, _vp,
+                                             _vp, _vp, _i32, _i32, _vp]),
+    "riallm_cuda_paged_attention_workspace": (_u64, [_vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32]),
+    "riallm_cuda_paged_attention": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _i32, _i32,
+                                           _i32, _i32, _i32, _i32, _vp, _vp, _u64, _vp]),
+    "riallm_cuda_verify_draft_workspace": (_u64, [_vp, _i32, _i32, _i32]),
+    "riallm_cuda_verify_draft": (_i32, [_vp, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _vp, _vp, _vp,
+                                        _u64, _vp]),
 }
 
 PHASES = ("route", "gather", "gate_up", "down", "shared", "combine", "dispatch", "return")
@@ -544,8 +555,15 @@ def route(gate: TensorLike, hidden: torch.Tensor, num_experts_per_tok: int, num_
 
 def __getattr__(name: str):
     """AutoModel / ModelConfig (src/auto_model.rs, src/config.rs) live in
-    riallm_b200.auto_model and are loaded on first use."""
+    riallm_b200.auto_model, the paged cache's functions in riallm_b200.paged
+    and verify_draft in riallm_b200.sampling; they are loaded on first use."""
     if name in ("AutoModel", "ModelConfig"):
         from . import auto_model
         return getattr(auto_model, name)
+    if name in ("PagedKVCache", "paged_attention", "rope_paged_append"):
+        from . import paged
+        return getattr(paged, name)
+    if name == "verify_draft":
+        from . import sampling
+        return sampling.verify_draft
     raise AttributeError(f"module 'riallm_b200' has no attribute {name!r}")

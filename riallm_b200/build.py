@@ -19,7 +19,8 @@ BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libriallm_cuda.so")
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 
-SOURCES = ["api.cu", "quant.cu", "route.cu", "expert_tc.cu", "noalloc.cu", "stream.cu", "decoder.cu", "ep.cu"]
+SOURCES = ["api.cu", "quant.cu", "route.cu", "expert_tc.cu", "noalloc.cu", "stream.cu", "decoder.cu", "ep.cu",
+           "paged.cu", "verify.cu"]
 HEADERS = ["common.cuh", "internal.h"]
 
 NVCC_FLAGS = [

@@ -66,6 +66,39 @@ struct riallm_ctx {
 
 namespace rl {
 
+// Runs an entry point's body on the context's device and gives the calling
+// thread its device back; no C++ exception leaves it.
+template <typename F>
+inline int32_t guarded(riallm_ctx* ctx, F&& body) noexcept {
+  int before = -1, status;
+  if (cudaGetDevice(&before) != cudaSuccess) before = -1;
+  if (before != ctx->device && cudaSetDevice(ctx->device) != cudaSuccess) return RIALLM_ERR_CUDA;
+  try {
+    status = body();
+  } catch (...) {
+    status = RIALLM_ERR_MEMORY;  // a message that could not be stored
+  }
+  if (before >= 0 && before != ctx->device) cudaSetDevice(before);
+  return status;
+}
+// Records why a call is refused (if there is a context to record it in).
+inline int32_t refuse(riallm_ctx* ctx, int32_t code, const char* what, const char* why) noexcept {
+  try {
+    if (ctx) ctx->last_error = std::string(what) + ": " + why;
+  } catch (...) {
+  }
+  return code;
+}
+// Status of one kernel launch, counted when it succeeded.
+inline int32_t launched(riallm_ctx* ctx, const char* what, cudaError_t e) {
+  if (e == cudaSuccess) {
+    ctx->launches += 1;
+    return RIALLM_OK;
+  }
+  ctx->last_error = std::string(what) + " launch: " + cudaGetErrorString(e);
+  return RIALLM_ERR_CUDA;
+}
+
 // Phase profiling (riallm_cuda_profile_enable): an event pair around a
 // phase on the call's stream, recorded only while profiling is on.
 inline cudaEvent_t take_event(riallm_ctx* ctx) {
