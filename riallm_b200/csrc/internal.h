@@ -30,6 +30,9 @@ struct riallm_ctx {
   void* attn_ws = nullptr;
   // Kernel launches issued by this context.
   uint64_t launches = 0;
+  // Kernels whose shared-memory limit has been raised on this context's
+  // device, a bit each (rl::allow_smem).
+  uint32_t smem_allowed = 0;
   // Phase profiling: event pairs recorded per call, summed on read.
   bool profiling = false;
   struct PhaseEvents {
@@ -97,6 +100,20 @@ inline int32_t launched(riallm_ctx* ctx, const char* what, cudaError_t e) {
   }
   ctx->last_error = std::string(what) + " launch: " + cudaGetErrorString(e);
   return RIALLM_ERR_CUDA;
+}
+
+// Raises a kernel's dynamic shared-memory limit, once per context; `bit`
+// names the kernel.
+template <typename K>
+inline int32_t allow_smem(riallm_ctx* ctx, const char* what, K kernel, int bytes, int bit) {
+  if (ctx->smem_allowed >> bit & 1) return RIALLM_OK;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) {
+    ctx->last_error = std::string(what) + ": cudaFuncSetAttribute: " + cudaGetErrorString(e);
+    return RIALLM_ERR_CUDA;
+  }
+  ctx->smem_allowed |= 1u << bit;
+  return RIALLM_OK;
 }
 
 // Phase profiling (riallm_cuda_profile_enable): an event pair around a

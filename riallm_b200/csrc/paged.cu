@@ -8,7 +8,8 @@
 // neither written nor read. riallm keeps one contiguous cache per layer
 // (KVCACHE, src/model.rs:15-38); rotary embedding and attention follow
 // src/model.rs:912-1071 as the contiguous kernels in decoder.cu do.
-#include <cfloat>
+#include <algorithm>
+#include <cmath>
 
 #include "common.cuh"
 #include "internal.h"
@@ -85,61 +86,567 @@ __global__ void __launch_bounds__(64)
   }
 }
 
-// Which keys the row at position p sees: [0, min(p + 1, cap)), and with a
-// window only the last `window` of [0, p] and the first `sinks`.
-struct Window {
+// Which keys a row sees: j <= hi, and j >= lo or j < sinks.
+struct Span {
+  int lo, hi;
+};
+// What the attention kernels share. Row r of a (sequence, kv head) pair is
+// token r / rep under query head kh * rep + r % rep: the heads of one kv head
+// are rows of one matrix product with its keys.
+struct AttnArgs {
+  const uint16_t* q;
+  const uint16_t* k;
+  const uint16_t* v;
+  const int* pos;
+  Pages pg;
+  int B, T, nh, rep;
   int window, sinks;
-  __device__ __forceinline__ int64_t first(int64_t p) const {  // first key inside the window
-    return window > 0 ? max((int64_t)0, p - window + 1) : 0;
+  float scale_log2;  // log2(e) / sqrt(d): weights are powers of two
+  uint16_t* out;
+
+  __device__ __forceinline__ Span span(int64_t p) const {  // of the row at position p
+    const int64_t cap = pg.cap();
+    Span s;
+    s.hi = (int)max((int64_t)-1, min(p, cap - 1));
+    s.lo = window > 0 ? (int)max((int64_t)0, min(p - window + 1, (int64_t)INT32_MAX)) : 0;
+    return s;
+  }
+};
+__device__ __forceinline__ bool sees(Span s, int sinks, int j) { return j <= s.hi && (j >= s.lo || j < sinks); }
+
+// The blocks of kBlock keys that some row of a sequence sees, in order: the
+// first `ns` hold sinks, the others start at block `w0`.
+struct Blocks {
+  int ns, w0, n;
+  Span all;  // what the sequence's rows see together
+  __device__ __forceinline__ int index(int i) const { return i < ns ? i : w0 + i - ns; }
+};
+template <int kBlock>
+__device__ __forceinline__ Blocks blocks_of(const AttnArgs& a, int64_t first, int64_t last) {
+  Blocks r;
+  r.all.hi = a.span(last).hi;
+  r.all.lo = a.span(first).lo;
+  r.w0 = r.all.lo / kBlock;
+  const int nw = r.all.hi >= r.all.lo ? r.all.hi / kBlock - r.w0 + 1 : 0;
+  const int sink_end = min(a.sinks, r.all.hi + 1);  // sinks that exist
+  r.ns = a.window > 0 && sink_end > 0 ? (sink_end - 1) / kBlock + 1 : 0;
+  if (nw > 0) r.ns = min(r.ns, r.w0);
+  r.n = max(1, r.ns + nw);  // one block, seen by nobody, where nothing is seen
+  return r;
+}
+
+__device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], const void* p) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(rl::smem_u32(p))
+               : "memory");
+}
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], const void* p) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(rl::smem_u32(p))
+               : "memory");
+}
+// d[16 x 8] += a[16 x 16] b[16 x 8], bf16 with float32 sums.
+__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// 16 bytes, or 16 zero bytes where `bytes` is 0 (src is not read then).
+__device__ __forceinline__ void cp_async_16z(void* dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(rl::smem_u32(dst)), "l"(src), "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ bool odd16(uint32_t x) {  // either bf16 of x is infinite or NaN
+  return (x & 0x7f80u) == 0x7f80u || (x & 0x7f800000u) == 0x7f800000u;
+}
+
+// ---------------------------------------------------------------- few rows
+//
+// Attention of few rows per sequence (single new tokens, drafted ones): a
+// pass over the keys and values, bound by reading them. The work of a call,
+// 64 keys of one (sequence, kv head, row tile) group a unit, is cut into as
+// many equal contiguous shares as there are CTAs, whatever the sequences'
+// lengths; a group that a share boundary cuts leaves partial results, which
+// join_kernel adds up. The lengths are the device's, so a captured call
+// follows them.
+//
+// In a CTA each of 4 warps takes 16 keys of every unit and is its own
+// pipeline: cp.async into its own ring of kStages x (16 keys, 16 values),
+// scores and weighted sums on m16n8k16 matrix instructions (the up to
+// 16 * MT rows against 16 keys), running maximum and sum in registers, no
+// barrier with other warps until a group's end. The products are 1/40 of
+// what even these instructions can do at the rate the bytes arrive, so
+// nothing is gained by a 128-row tcgen05 tile of which 4 to 32 rows are
+// used.
+constexpr int kUnitKeys = 64, kFewWarps = 4;
+
+template <int D>
+constexpr int kFewStages = D == 128 ? 3 : 6;
+template <int D, int MT>
+constexpr int kFewSmem = kFewWarps * kFewStages<D> * 2 * 16 * D * 2 + 16 * MT * D * 4;
+
+// Share of CTA c of G: units [W c / G, W (c+1) / G). The CTA of unit u.
+__device__ __forceinline__ int64_t share_begin(int64_t W, int G, int c) { return W * c / G; }
+__device__ __forceinline__ int share_of(int64_t W, int G, int64_t u) { return (int)(((u + 1) * G - 1) / W); }
+
+// Finds where a unit lies: every thread of a block of N threads sums the
+// units of its slab of sequences.
+struct UnitAt {
+  int64_t W;      // all units of the call
+  int64_t start;  // first unit of sequence b
+  int b;
+  Blocks bl;
+};
+template <int N>
+__device__ __forceinline__ void find_unit(const AttnArgs& a, int groups, int c, int G, int ahead, UnitAt& at) {
+  __shared__ int64_t sums[N];
+  __shared__ int64_t sh_start;
+  __shared__ int sh_b;
+  const int per = (a.B + N - 1) / N;
+  const int b0 = min(a.B, (int)threadIdx.x * per), b1 = min(a.B, b0 + per);
+  int64_t mine = 0;
+  for (int b = b0; b < b1; ++b)
+    mine += (int64_t)blocks_of<kUnitKeys>(a, a.pos[b], (int64_t)a.pos[b] + a.T - 1).n * groups;
+  sums[threadIdx.x] = mine;
+  __syncthreads();
+#pragma unroll
+  for (int o = 1; o < N; o <<= 1) {  // inclusive scan
+    const int64_t x = (int)threadIdx.x >= o ? sums[threadIdx.x - o] : 0;
+    __syncthreads();
+    sums[threadIdx.x] += x;
+    __syncthreads();
+  }
+  at.W = sums[N - 1];
+  const int64_t u = min(share_begin(at.W, G, c + ahead), at.W - 1);
+  int64_t s = sums[threadIdx.x] - mine;
+  if (u >= s && u < s + mine) {
+    for (int b = b0; b < b1; ++b) {
+      const int64_t n = (int64_t)blocks_of<kUnitKeys>(a, a.pos[b], (int64_t)a.pos[b] + a.T - 1).n * groups;
+      if (u < s + n) {
+        sh_b = b;
+        sh_start = s;
+        break;
+      }
+      s += n;
+    }
+  }
+  __syncthreads();
+  at.b = sh_b;
+  at.start = sh_start;
+  at.bl = blocks_of<kUnitKeys>(a, a.pos[at.b], (int64_t)a.pos[at.b] + a.T - 1);
+}
+
+// Walks the units of a share.
+struct Cursor {
+  int b, g, i;
+  int64_t p0;
+  Blocks bl;
+  __device__ __forceinline__ void load(const AttnArgs& a) {
+    p0 = a.pos[b];
+    bl = blocks_of<kUnitKeys>(a, p0, p0 + a.T - 1);
+  }
+  __device__ __forceinline__ void next(const AttnArgs& a, int groups) {
+    if (++i < bl.n) return;
+    i = 0;
+    if (++g < groups) return;
+    g = 0;
+    if (++b < a.B) load(a);
   }
 };
 
-// Warp per (row, head): keys one at a time, a lane per d / 32 dimensions,
-// running maximum and sum in float32.
-template <int D>
-__global__ void __launch_bounds__(128)
-    paged_attention_kernel(const uint16_t* __restrict__ q, const uint16_t* __restrict__ kp,
-                           const uint16_t* __restrict__ vp, const int* __restrict__ pos, Pages pg, Window win,
-                           int64_t pairs, int T, int nh, float scale, uint16_t* __restrict__ out) {
-  constexpr int E = D / 32;
+// A partial result: maxima, sums and accumulators of the rows of one tile.
+template <int D, int MT>
+constexpr int kSlotFloats = 16 * MT * (D + 2);
+
+template <int D, int MT>
+__global__ void __launch_bounds__(kFewWarps * 32, 2)
+    few_rows_kernel(const AttnArgs a, int tiles, float* __restrict__ ws) {
+  constexpr int S = kFewStages<D>, C = D / 8, kRows = 16 * MT;
+  extern __shared__ __align__(128) uint16_t smem[];
+  __shared__ float sm_m[kFewWarps][kRows], sm_l[kFewWarps][kRows];
   rl::pdl_wait();
   rl::pdl_launch_dependents();
-  const int lane = threadIdx.x & 31;
-  const int64_t pair = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (pair >= pairs) return;
-  const int64_t row = pair / nh;
-  const int h = (int)(pair - row * nh), kh = h / (nh / pg.nkv);
-  const int b = (int)(row / T);
-  const int64_t p = (int64_t)pos[b] + (row - (int64_t)b * T);
-  const int64_t L = max((int64_t)0, min(p + 1, pg.cap()));
-  const int64_t lo = win.first(p);
-  float qr[E], acc[E], m = -FLT_MAX, l = 0.f;
-  bool any = false;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, G = gridDim.x;
+  const int groups = a.pg.nkv * tiles;
+  UnitAt at;
+  find_unit<kFewWarps * 32>(a, groups, blockIdx.x, G, 0, at);
+  const int64_t u0 = share_begin(at.W, G, blockIdx.x), u1 = share_begin(at.W, G, blockIdx.x + 1);
+  if (u0 >= u1) return;
+  const int count = (int)(u1 - u0);
+  Cursor now;
+  now.b = at.b;
+  now.load(a);
+  now.g = (int)((u0 - at.start) / now.bl.n);
+  now.i = (int)((u0 - at.start) - (int64_t)now.g * now.bl.n);
+  Cursor ahead = now;
+
+  uint16_t* ring = smem + warp * (S * 2 * 16 * D);
+  float* merged = reinterpret_cast<float*>(smem + kFewWarps * S * 2 * 16 * D);  // [kRows][D]
+
+  // Loads of unit n (counted from u0) go to stage n % S. Bit n % 32 of
+  // `held` says whether this warp has anything to do in unit n.
+  uint32_t held = 0;
+  int issued = 0;
+  int page = -1;
+  auto key0 = [&](const Cursor& c) { return c.bl.index(c.i) * kUnitKeys + warp * 16; };
+  auto fetch_page = [&]() {  // the page of the unit that is loaded next
+    page = -1;
+    if (issued < count) {
+      const int j = key0(ahead);
+      const bool any = j <= ahead.bl.all.hi && (j + 15 >= ahead.bl.all.lo || j < a.sinks);
+      if (any) page = a.pg.table[ahead.b * a.pg.stride + (j >> a.pg.lg)];
+    }
+  };
+  auto issue = [&]() {
+    if (issued < count) {
+      const bool ok = (unsigned)page < (unsigned)a.pg.num_pages;
+      held = (held & ~(1u << (issued & 31))) | ((ok ? 1u : 0u) << (issued & 31));
+      if (ok) {
+        const int j = key0(ahead), kh = ahead.g / tiles;
+        const int64_t row = (((int64_t)page * a.pg.nkv + kh) << a.pg.lg) + (j & ((1 << a.pg.lg) - 1));
+        uint16_t* ks = ring + (issued % S) * (2 * 16 * D);
+        uint16_t* vs = ks + 16 * D;
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    qr[e] = bf2f(q[pair * D + lane * E + e]);
-    acc[e] = 0.f;
+        for (int x = 0; x < 16 * C / 32; ++x) {
+          const int idx = x * 32 + lane, key = idx / C, c = idx % C;
+          const bool in = sees(ahead.bl.all, a.sinks, j + key);
+          const int64_t off = (row + (in ? key : 0)) * D + c * 8;
+          const int to = key * D + ((c ^ (key & 7)) * 8);
+          cp_async_16z(ks + to, a.k + off, in ? 16 : 0);
+          cp_async_16z(vs + to, a.v + off, in ? 16 : 0);
+        }
+      }
+      ++issued;
+      if (issued < count) ahead.next(a, groups);
+      fetch_page();
+    }
+    rl::cp_async_commit();
+  };
+  fetch_page();
+#pragma unroll
+  for (int s = 0; s < S - 1; ++s) issue();
+
+  uint32_t qf[MT][D / 16][4];
+  float o[MT][D / 8][4], m[MT][2], l[MT][2];
+  Span sp[MT][2];
+  int tile = 0, kh = 0, first = 0;
+  const int all_rows = a.T * a.rep;
+  for (int n = 0; n < count; ++n) {
+    if (n == 0 || now.i == 0) {  // a group begins
+      kh = now.g / tiles;
+      tile = now.g - kh * tiles;
+      first = n;
+#pragma unroll
+      for (int t = 0; t < MT; ++t) {
+#pragma unroll
+        for (int x = 0; x < D / 8; ++x)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[t][x][e] = 0.f;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int r = tile * kRows + t * 16 + h * 8 + (lane >> 2);
+          m[t][h] = -INFINITY;
+          l[t][h] = 0.f;
+          const bool in = r < all_rows;
+          const int tok = in ? r / a.rep : 0, hd = in ? r - tok * a.rep : 0;
+          sp[t][h] = in ? a.span(now.p0 + tok) : Span{0, -1};
+          const uint32_t* qr = reinterpret_cast<const uint32_t*>(
+              a.q + (((int64_t)now.b * a.T + tok) * a.nh + kh * a.rep + hd) * D);
+#pragma unroll
+          for (int x = 0; x < D / 16; ++x) {
+            qf[t][x][h] = in ? __ldg(qr + x * 8 + (lane & 3)) : 0u;
+            qf[t][x][2 + h] = in ? __ldg(qr + x * 8 + 4 + (lane & 3)) : 0u;
+          }
+        }
+      }
+    }
+    rl::cp_async_wait<S - 2>();
+    __syncwarp();
+    if (held >> (n & 31) & 1) {
+      const int j0 = key0(now);
+      uint16_t* ks = ring + (n % S) * (2 * 16 * D);
+      uint16_t* vs = ks + 16 * D;
+      float sc[MT][2][4];
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int y = 0; y < 2; ++y)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sc[t][y][e] = 0.f;
+#pragma unroll
+      for (int x = 0; x < D / 16; ++x) {
+        uint32_t kf[4];
+        const int key = (lane & 7) + ((lane >> 4) << 3), c = 2 * x + ((lane >> 3) & 1);
+        ldmatrix_x4(kf, ks + key * D + ((c ^ (key & 7)) * 8));
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+          mma_16816(sc[t][0], qf[t][x], kf[0], kf[1]);
+          mma_16816(sc[t][1], qf[t][x], kf[2], kf[3]);
+        }
+      }
+      // Does any row of the sequence not see one of these keys?
+      const int64_t pl = now.p0 + a.T - 1;
+      const bool edge = j0 + 15 > min(now.p0, a.pg.cap() - 1) ||
+                        (a.window > 0 && j0 < pl - a.window + 1 && j0 + 15 >= a.sinks);
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float top = -INFINITY;
+#pragma unroll
+          for (int y = 0; y < 2; ++y)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float& x = sc[t][y][2 * h + e];
+              x *= a.scale_log2;
+              if (edge && !sees(sp[t][h], a.sinks, j0 + y * 8 + (lane & 3) * 2 + e)) x = -INFINITY;
+              top = fmaxf(top, x);
+            }
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+          const float mn = fmaxf(m[t][h], top);
+          const float base = mn == -INFINITY ? 0.f : mn;
+          const float corr = ex2(m[t][h] - base);
+          m[t][h] = mn;
+          float sum = 0.f;
+#pragma unroll
+          for (int y = 0; y < 2; ++y)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float& x = sc[t][y][2 * h + e];
+              x = ex2(x - base);
+              sum += x;
+            }
+          l[t][h] = fmaf(l[t][h], corr, sum);
+          if (__any_sync(0xffffffffu, corr != 1.f)) {
+#pragma unroll
+            for (int x = 0; x < D / 8; ++x) {
+              o[t][x][2 * h] *= corr;
+              o[t][x][2 * h + 1] *= corr;
+            }
+          }
+        }
+      if (edge && a.T > 1) {
+        // A value that is not finite, of a key that some rows see and some
+        // do not: 0 times it would reach the latter through the product.
+        // It is added to the rows that see it and zeroed for the product.
+        bool odd = false;
+#pragma unroll
+        for (int x = 0; x < 16 * C / 32; ++x) {
+          const uint4 w = *reinterpret_cast<const uint4*>(vs + (x * 32 + lane) * 8);
+          odd |= odd16(w.x) | odd16(w.y) | odd16(w.z) | odd16(w.w);
+        }
+        if (__any_sync(0xffffffffu, odd)) {
+          for (int key = 0; key < 16; ++key)
+#pragma unroll
+            for (int x = 0; x < D / 8; ++x) {
+              const uint32_t w =
+                  *reinterpret_cast<const uint32_t*>(vs + key * D + ((x ^ (key & 7)) * 8) + (lane & 3) * 2);
+              if (!odd16(w)) continue;
+              const float lo = bf2f((uint16_t)w), hi = bf2f((uint16_t)(w >> 16));
+#pragma unroll
+              for (int t = 0; t < MT; ++t)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                  if (sees(sp[t][h], a.sinks, j0 + key)) {
+                    if (!isfinite(lo)) o[t][x][2 * h] += lo;
+                    if (!isfinite(hi)) o[t][x][2 * h + 1] += hi;
+                  }
+            }
+          __syncwarp();
+          for (int x = lane; x < 16 * D; x += 32)
+            if ((vs[x] & 0x7f80u) == 0x7f80u) vs[x] = 0;
+          __syncwarp();
+        }
+      }
+      // The weights as bf16 and what that leaves, also as bf16: two products
+      // keep 16 bits of each weight (one alone costs as much accuracy again
+      // as the rounding of the output), and the matrix pipe is idle anyway.
+      uint32_t ph[MT][4], pr[MT][4];
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int y = 0; y < 2; ++y)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float x0 = sc[t][y][2 * h], x1 = sc[t][y][2 * h + 1];
+            const uint32_t hi = rl::pack_bf16x2(x0, x1);
+            ph[t][2 * y + h] = hi;
+            pr[t][2 * y + h] = rl::pack_bf16x2(x0 - __uint_as_float(hi << 16), x1 - __uint_as_float(hi & 0xffff0000u));
+          }
+#pragma unroll
+      for (int x = 0; x < D / 16; ++x) {
+        uint32_t vf[4];
+        const int key = (lane & 7) + (((lane >> 3) & 1) << 3), c = 2 * x + (lane >> 4);
+        ldmatrix_x4_trans(vf, vs + key * D + ((c ^ (key & 7)) * 8));
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+          mma_16816(o[t][2 * x], ph[t], vf[0], vf[1]);
+          mma_16816(o[t][2 * x + 1], ph[t], vf[2], vf[3]);
+          mma_16816(o[t][2 * x], pr[t], vf[0], vf[1]);
+          mma_16816(o[t][2 * x + 1], pr[t], vf[2], vf[3]);
+        }
+      }
+    }
+    __syncwarp();
+    issue();  // into the stage that was read before this one
+
+    const bool whole_end = now.i + 1 == now.bl.n;
+    if (whole_end || n + 1 == count) {  // the group ends, or this CTA's share of it
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          l[t][h] += __shfl_xor_sync(0xffffffffu, l[t][h], 1);
+          l[t][h] += __shfl_xor_sync(0xffffffffu, l[t][h], 2);
+          if ((lane & 3) == 0) {
+            sm_m[warp][t * 16 + h * 8 + (lane >> 2)] = m[t][h];
+            sm_l[warp][t * 16 + h * 8 + (lane >> 2)] = l[t][h];
+          }
+        }
+      __syncthreads();
+      float f[MT][2];
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int r = t * 16 + h * 8 + (lane >> 2);
+          float M = sm_m[0][r];
+          for (int w = 1; w < kFewWarps; ++w) M = fmaxf(M, sm_m[w][r]);
+          f[t][h] = M == -INFINITY ? 0.f : ex2(m[t][h] - M);
+        }
+      for (int w = 0; w < kFewWarps; ++w) {  // in warp order: the same sum every time
+        if (warp == w)
+#pragma unroll
+          for (int t = 0; t < MT; ++t)
+#pragma unroll
+            for (int x = 0; x < D / 8; ++x)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                float2* to = reinterpret_cast<float2*>(merged + (t * 16 + h * 8 + (lane >> 2)) * D + x * 8 +
+                                                       (lane & 3) * 2);
+                float2 y = w ? *to : make_float2(0.f, 0.f);
+                // A warp that has seen nothing adds nothing (0 * its NaN-free zeros).
+                y.x += o[t][x][2 * h] * f[t][h];
+                y.y += o[t][x][2 * h + 1] * f[t][h];
+                *to = y;
+              }
+        __syncthreads();
+      }
+      // Whole group here: the output. Otherwise the CTA's slot of partial
+      // results, 2 per CTA: one for a group that began in an earlier share
+      // or with this share, one for a group that began inside it.
+      const bool whole = whole_end && now.i == n - first;
+      const int rows = min(kRows, all_rows - tile * kRows);
+      float* slot = ws + (2 * (int64_t)blockIdx.x + (first == 0 ? 0 : 1)) * kSlotFloats<D, MT>;
+      for (int x = threadIdx.x; x < rows * (D / 2); x += kFewWarps * 32) {
+        const int r = x / (D / 2), c = (x - r * (D / 2)) * 2;
+        const float2 y = *reinterpret_cast<const float2*>(merged + r * D + c);
+        float M = sm_m[0][r], L = 0.f;
+        for (int w = 1; w < kFewWarps; ++w) M = fmaxf(M, sm_m[w][r]);
+        for (int w = 0; w < kFewWarps; ++w) L += M == -INFINITY ? 0.f : sm_l[w][r] * ex2(sm_m[w][r] - M);
+        if (whole) {
+          const float inv = L == 0.f ? 0.f : __fdiv_rn(1.f, L);
+          const int rr = tile * kRows + r, tok = rr / a.rep, hd = rr - tok * a.rep;
+          *reinterpret_cast<uint32_t*>(a.out + (((int64_t)now.b * a.T + tok) * a.nh + kh * a.rep + hd) * D + c) =
+              rl::pack_bf16x2(y.x * inv, y.y * inv);
+        } else {
+          *reinterpret_cast<float2*>(slot + 2 * kRows + r * D + c) = y;
+          if (c == 0) {
+            slot[r] = M;
+            slot[kRows + r] = L;
+          }
+        }
+      }
+      __syncthreads();
+    }
+    if (n + 1 < count) now.next(a, groups);
   }
-  for (int64_t j = 0; j < L; ++j) {
-    if (j < lo && j >= win.sinks) j = lo;
-    if (j >= L) break;
-    const int64_t at = pg.row(b, kh, j);
-    if (at < 0) continue;
-    any = true;
-    float s = 0.f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) s = fmaf(qr[e], bf2f(kp[at * D + lane * E + e]), s);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    s *= scale;
-    const float mn = fmaxf(m, s), corr = expf(m - mn), w = expf(s - mn);
-    m = mn;
-    l = fmaf(l, corr, w);
-#pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = fmaf(acc[e], corr, w * bf2f(vp[at * D + lane * E + e]));
+}
+
+// CTA c adds up the partial results of the group that the boundary between
+// the shares of CTAs c and c + 1 cuts, if c is the first that holds part of
+// it. Threads (dimension, row).
+template <int D, int MT>
+__global__ void __launch_bounds__(D * 4) join_kernel(const AttnArgs a, int tiles, int G, const float* __restrict__ ws) {
+  constexpr int kRows = 16 * MT;
+  rl::pdl_wait();
+  rl::pdl_launch_dependents();
+  const int groups = a.pg.nkv * tiles, c0 = blockIdx.x;
+  UnitAt at;
+  find_unit<D * 4>(a, groups, c0, G, 1, at);
+  const int64_t u = share_begin(at.W, G, c0 + 1);  // first unit of the next share
+  const int64_t g = (u - at.start) / at.bl.n, g0 = at.start + g * at.bl.n, g1 = g0 + at.bl.n;
+  if (u == g0 || u >= at.W || share_begin(at.W, G, c0) == u) return;  // not cut here, or c0 holds nothing
+  if (share_of(at.W, G, g0) != c0) return;
+  const int c1 = share_of(at.W, G, g1 - 1);
+  const int kh = (int)(g / tiles), tile = (int)(g - (int64_t)kh * tiles);
+  const int rows = min(kRows, a.T * a.rep - tile * kRows);
+  const int d = threadIdx.x % D;
+  auto slot = [&](int c) {
+    // In c0 the group may have begun inside the share.
+    return ws + (2 * (int64_t)c + (c == c0 && share_begin(at.W, G, c) < g0 ? 1 : 0)) * kSlotFloats<D, MT>;
+  };
+  for (int r = threadIdx.x / D; r < rows; r += 4) {
+    float M = -INFINITY;
+    for (int c = c0; c <= c1; ++c)
+      if (share_begin(at.W, G, c) < share_begin(at.W, G, c + 1)) M = fmaxf(M, __ldcg(slot(c) + r));
+    float num = 0.f, den = 0.f;
+    if (M != -INFINITY)
+      for (int c = c0; c <= c1; ++c) {
+        if (share_begin(at.W, G, c) == share_begin(at.W, G, c + 1)) continue;
+        const float* s = slot(c);
+        const float w = ex2(__ldcg(s + r) - M);
+        den = fmaf(w, __ldcg(s + kRows + r), den);
+        num = fmaf(w, __ldcg(s + 2 * kRows + r * D + d), num);
+      }
+    const int rr = tile * kRows + r, tok = rr / a.rep, hd = rr - tok * a.rep;
+    a.out[(((int64_t)at.b * a.T + tok) * a.nh + kh * a.rep + hd) * D + d] = f2bf(den == 0.f ? 0.f : num / den);
   }
-#pragma unroll
-  for (int e = 0; e < E; ++e) out[pair * D + lane * E + e] = f2bf(any ? __fdiv_rn(acc[e], l) : 0.f);
+}
+
+// The launch of a call with few rows: CTAs, row tiles and whether a group
+// can be cut at all.
+struct FewPlan {
+  int MT, tiles, G;
+  bool join;
+  uint64_t ws_bytes;
+};
+FewPlan few_plan(int num_sms, int B, int T, int nh, int nkv, int d, int64_t cap) {
+  FewPlan p;
+  const int64_t rows = (int64_t)T * (nh / nkv);
+  p.MT = rows <= 16 ? 1 : 2;
+  p.tiles = (int)((rows + 16 * p.MT - 1) / (16 * p.MT));
+  const int64_t blocks = (cap + kUnitKeys - 1) / kUnitKeys;
+  const int64_t most = (int64_t)B * nkv * p.tiles * blocks;
+  p.G = (int)std::min<int64_t>(2 * num_sms, most);
+  p.join = blocks > 1 && p.G > 1;
+  p.ws_bytes = p.join ? (uint64_t)2 * p.G * 16 * p.MT * (d + 2) * sizeof(float) : 0;
+  return p;
+}
+
+template <int D, int MT>
+int32_t launch_few(riallm_ctx* ctx, const AttnArgs& a, const FewPlan& p, float* ws, cudaStream_t st) {
+  if (int s = rl::allow_smem(ctx, "paged_attention", few_rows_kernel<D, MT>, kFewSmem<D, MT>,
+                             D / 64 * 2 + MT - 3))
+    return s;
+  if (int s = rl::launched(ctx, "paged_attention",
+                           rl::launch_pdl(few_rows_kernel<D, MT>, dim3(p.G), dim3(kFewWarps * 32), kFewSmem<D, MT>, st,
+                                          a, p.tiles, ws)))
+    return s;
+  if (!p.join) return RIALLM_OK;
+  return rl::launched(ctx, "paged_attention join",
+                      rl::launch_pdl(join_kernel<D, MT>, dim3(p.G - 1), dim3(D * 4), 0, st, a, p.tiles, p.G,
+                                     static_cast<const float*>(ws)));
 }
 
 bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -202,8 +709,8 @@ int32_t riallm_cuda_rope_paged_append(riallm_ctx* ctx, const void* qkv, const in
 
 uint64_t riallm_cuda_paged_attention_workspace(const riallm_ctx* ctx, int32_t B, int32_t T, int32_t nh, int32_t nkv,
                                                int32_t d, int32_t max_pages, int32_t page_size) {
-  (void)ctx, (void)B, (void)T, (void)nh, (void)nkv, (void)d, (void)max_pages, (void)page_size;
-  return 0;
+  if (!ctx || B <= 0 || T <= 0 || nkv <= 0 || nh < nkv || max_pages <= 0 || page_size <= 0) return 0;
+  return few_plan(ctx->num_sms, B, T, nh, nkv, d, (int64_t)max_pages * page_size).ws_bytes;
 }
 
 int32_t riallm_cuda_paged_attention(riallm_ctx* ctx, const void* q, const void* k_pages, const void* v_pages,
@@ -215,23 +722,29 @@ int32_t riallm_cuda_paged_attention(riallm_ctx* ctx, const void* q, const void* 
   if (int s = check_pages(ctx, what, B, T, nh, nkv, d, num_pages, page_size, max_pages, table_stride)) return s;
   if (window < 0 || sinks < 0)
     return rl::refuse(ctx, RIALLM_ERR_CONFIG, what, "window and sinks must not be negative");
-  const int64_t pairs = (int64_t)B * T * nh;
-  if (ctx && pairs == 0) return RIALLM_OK;
+  if (ctx && (int64_t)B * T == 0) return RIALLM_OK;
   if (!ctx || !q || !k_pages || !v_pages || !pos || !page_table || !out)
     return rl::refuse(ctx, RIALLM_ERR_INVALID, what, "NULL argument");
   if (!al16(q) || !al16(out) || !al16(k_pages) || !al16(v_pages))
     return rl::refuse(ctx, RIALLM_ERR_INVALID, what, "buffers must be 16-byte aligned");
-  if ((pairs + 3) / 4 > INT32_MAX) return rl::refuse(ctx, RIALLM_ERR_CONFIG, what, "too many rows");
-  (void)workspace, (void)workspace_bytes;
+  const FewPlan p = few_plan(ctx->num_sms, B, T, nh, nkv, d, (int64_t)max_pages * page_size);
+  if (p.ws_bytes && (!workspace || workspace_bytes < p.ws_bytes || (reinterpret_cast<uintptr_t>(workspace) & 255)))
+    return rl::refuse(ctx, RIALLM_ERR_MEMORY, what, "workspace missing, too small or not 256-byte aligned");
   return rl::guarded(ctx, [&]() -> int32_t {
-    const Pages pg = make_pages(page_table, table_stride, max_pages, num_pages, nkv, page_size);
-    const float scale = (float)(1.0 / sqrt((double)d));
-    return rl::launched(ctx, what,
-                        rl::launch_pdl(d == 128 ? paged_attention_kernel<128> : paged_attention_kernel<64>,
-                                       dim3((unsigned)((pairs + 3) / 4)), dim3(128), 0, (cudaStream_t)stream,
-                                       static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(k_pages),
-                                       static_cast<const uint16_t*>(v_pages), pos, pg, Window{window, sinks}, pairs, T,
-                                       nh, scale, static_cast<uint16_t*>(out)));
+    AttnArgs a;
+    a.q = static_cast<const uint16_t*>(q);
+    a.k = static_cast<const uint16_t*>(k_pages);
+    a.v = static_cast<const uint16_t*>(v_pages);
+    a.pos = pos;
+    a.pg = make_pages(page_table, table_stride, max_pages, num_pages, nkv, page_size);
+    a.B = B, a.T = T, a.nh = nh, a.rep = nh / nkv;
+    a.window = window, a.sinks = sinks;
+    a.scale_log2 = (float)(1.4426950408889634 / sqrt((double)d));
+    a.out = static_cast<uint16_t*>(out);
+    float* ws = static_cast<float*>(workspace);
+    cudaStream_t st = (cudaStream_t)stream;
+    if (d == 128) return p.MT == 1 ? launch_few<128, 1>(ctx, a, p, ws, st) : launch_few<128, 2>(ctx, a, p, ws, st);
+    return p.MT == 1 ? launch_few<64, 1>(ctx, a, p, ws, st) : launch_few<64, 2>(ctx, a, p, ws, st);
   });
 }
 
