@@ -198,40 +198,52 @@ constexpr int kFewSmem = kFewWarps * kFewStages<D> * 2 * 16 * D * 2 + 16 * MT * 
 __device__ __forceinline__ int64_t share_begin(int64_t W, int G, int c) { return W * c / G; }
 __device__ __forceinline__ int share_of(int64_t W, int G, int64_t u) { return (int)(((u + 1) * G - 1) / W); }
 
-// Finds where a unit lies: every thread of a block of N threads sums the
-// units of its slab of sequences.
+// Finds where the first unit of share c (of the call's G shares, fewer where
+// there are fewer units) lies: every thread of a block of N threads sums the
+// units of its slab of sequences, and the thread whose slab holds the unit
+// walks it.
 struct UnitAt {
   int64_t W;      // all units of the call
-  int64_t start;  // first unit of sequence b
+  int G;          // shares, none of them empty
+  int64_t u;      // the share's first unit (W where there is no such share)
+  int64_t start;  // first unit of sequence b, which holds u
   int b;
   Blocks bl;
 };
 template <int N>
-__device__ __forceinline__ void find_unit(const AttnArgs& a, int groups, int c, int G, int ahead, UnitAt& at) {
-  __shared__ int64_t sums[N];
+__device__ __forceinline__ UnitAt find_unit(const AttnArgs& a, int groups, int G, int c) {
+  __shared__ int64_t sums[N / 32];
   __shared__ int64_t sh_start;
   __shared__ int sh_b;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int per = (a.B + N - 1) / N;
   const int b0 = min(a.B, (int)threadIdx.x * per), b1 = min(a.B, b0 + per);
   int64_t mine = 0;
   for (int b = b0; b < b1; ++b)
     mine += (int64_t)blocks_of<kUnitKeys>(a, a.pos[b], (int64_t)a.pos[b] + a.T - 1).n * groups;
-  sums[threadIdx.x] = mine;
-  __syncthreads();
+  int64_t upto = mine;  // inclusive scan
 #pragma unroll
-  for (int o = 1; o < N; o <<= 1) {  // inclusive scan
-    const int64_t x = (int)threadIdx.x >= o ? sums[threadIdx.x - o] : 0;
-    __syncthreads();
-    sums[threadIdx.x] += x;
-    __syncthreads();
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t x = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += x;
   }
-  at.W = sums[N - 1];
-  const int64_t u = min(share_begin(at.W, G, c + ahead), at.W - 1);
-  int64_t s = sums[threadIdx.x] - mine;
-  if (u >= s && u < s + mine) {
+  if (lane == 31) sums[warp] = upto;
+  __syncthreads();
+  UnitAt at;
+  at.W = 0;
+  int64_t before = 0;
+#pragma unroll
+  for (int w = 0; w < N / 32; ++w) {
+    before += w < warp ? sums[w] : 0;
+    at.W += sums[w];
+  }
+  at.G = (int)min((int64_t)G, at.W);
+  at.u = c < at.G ? share_begin(at.W, at.G, c) : at.W;
+  int64_t s = before + upto - mine;
+  if (at.u >= s && at.u < s + mine) {
     for (int b = b0; b < b1; ++b) {
       const int64_t n = (int64_t)blocks_of<kUnitKeys>(a, a.pos[b], (int64_t)a.pos[b] + a.T - 1).n * groups;
-      if (u < s + n) {
+      if (at.u < s + n) {
         sh_b = b;
         sh_start = s;
         break;
@@ -239,10 +251,12 @@ __device__ __forceinline__ void find_unit(const AttnArgs& a, int groups, int c, 
       s += n;
     }
   }
+  if (at.u >= at.W) return at;
   __syncthreads();
   at.b = sh_b;
   at.start = sh_start;
   at.bl = blocks_of<kUnitKeys>(a, a.pos[at.b], (int64_t)a.pos[at.b] + a.T - 1);
+  return at;
 }
 
 // Walks the units of a share.
@@ -275,13 +289,12 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
   __shared__ float sm_m[kFewWarps][kRows], sm_l[kFewWarps][kRows];
   rl::pdl_wait();
   rl::pdl_launch_dependents();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, G = gridDim.x;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int groups = a.pg.nkv * tiles;
-  UnitAt at;
-  find_unit<kFewWarps * 32>(a, groups, blockIdx.x, G, 0, at);
-  const int64_t u0 = share_begin(at.W, G, blockIdx.x), u1 = share_begin(at.W, G, blockIdx.x + 1);
-  if (u0 >= u1) return;
-  const int count = (int)(u1 - u0);
+  const UnitAt at = find_unit<kFewWarps * 32>(a, groups, gridDim.x, blockIdx.x);
+  const int64_t u0 = at.u;
+  if (u0 >= at.W) return;
+  const int count = (int)(share_begin(at.W, at.G, blockIdx.x + 1) - u0);
   Cursor now;
   now.b = at.b;
   now.load(a);
@@ -574,43 +587,65 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
 }
 
 // CTA c adds up the partial results of the group that the boundary between
-// the shares of CTAs c and c + 1 cuts, if c is the first that holds part of
-// it. Threads (dimension, row).
+// the shares c and c + 1 cuts, if c is the first that holds part of it.
+// Threads (dimension, row); the weights of the parts are worked out once a
+// row, a part a thread.
+constexpr int kMaxShares = 512;
 template <int D, int MT>
 __global__ void __launch_bounds__(D * 4) join_kernel(const AttnArgs a, int tiles, int G, const float* __restrict__ ws) {
-  constexpr int kRows = 16 * MT;
+  constexpr int kRows = 16 * MT, kSlot = kSlotFloats<D, MT>, kW = D / 32;
+  __shared__ float weight[4][kMaxShares], red[2][4][kW];
   rl::pdl_wait();
   rl::pdl_launch_dependents();
   const int groups = a.pg.nkv * tiles, c0 = blockIdx.x;
-  UnitAt at;
-  find_unit<D * 4>(a, groups, c0, G, 1, at);
-  const int64_t u = share_begin(at.W, G, c0 + 1);  // first unit of the next share
-  const int64_t g = (u - at.start) / at.bl.n, g0 = at.start + g * at.bl.n, g1 = g0 + at.bl.n;
-  if (u == g0 || u >= at.W || share_begin(at.W, G, c0) == u) return;  // not cut here, or c0 holds nothing
-  if (share_of(at.W, G, g0) != c0) return;
-  const int c1 = share_of(at.W, G, g1 - 1);
+  const UnitAt at = find_unit<D * 4>(a, groups, G, c0 + 1);
+  if (at.u >= at.W) return;
+  const int64_t g = (at.u - at.start) / at.bl.n, g0 = at.start + g * at.bl.n, g1 = g0 + at.bl.n;
+  if (at.u == g0 || share_of(at.W, at.G, g0) != c0) return;  // not cut here, or cut before as well
+  const int parts = share_of(at.W, at.G, g1 - 1) - c0 + 1;
+  // The first part is in its CTA's second slot where the group began inside
+  // that CTA's share.
+  const float* first = ws + (2 * (int64_t)c0 + (share_begin(at.W, at.G, c0) < g0 ? 1 : 0)) * kSlot;
+  const float* rest = ws + 2 * (int64_t)c0 * kSlot;
   const int kh = (int)(g / tiles), tile = (int)(g - (int64_t)kh * tiles);
   const int rows = min(kRows, a.T * a.rep - tile * kRows);
-  const int d = threadIdx.x % D;
-  auto slot = [&](int c) {
-    // In c0 the group may have begun inside the share.
-    return ws + (2 * (int64_t)c + (c == c0 && share_begin(at.W, G, c) < g0 ? 1 : 0)) * kSlotFloats<D, MT>;
-  };
-  for (int r = threadIdx.x / D; r < rows; r += 4) {
+  const int d = threadIdx.x % D, rs = threadIdx.x / D, lane = d & 31, w = d >> 5;
+  for (int r0 = 0; r0 < rows; r0 += 4) {
+    const int r = r0 + rs;
+    const bool in = r < rows;
     float M = -INFINITY;
-    for (int c = c0; c <= c1; ++c)
-      if (share_begin(at.W, G, c) < share_begin(at.W, G, c + 1)) M = fmaxf(M, __ldcg(slot(c) + r));
-    float num = 0.f, den = 0.f;
-    if (M != -INFINITY)
-      for (int c = c0; c <= c1; ++c) {
-        if (share_begin(at.W, G, c) == share_begin(at.W, G, c + 1)) continue;
-        const float* s = slot(c);
-        const float w = ex2(__ldcg(s + r) - M);
-        den = fmaf(w, __ldcg(s + kRows + r), den);
-        num = fmaf(w, __ldcg(s + 2 * kRows + r * D + d), num);
+    if (in)
+      for (int i = d; i < parts; i += D) M = fmaxf(M, __ldcg((i ? rest + (int64_t)i * 2 * kSlot : first) + r));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    if (lane == 0) red[0][rs][w] = M;
+    __syncthreads();
+#pragma unroll
+    for (int x = 0; x < kW; ++x) M = fmaxf(M, red[0][rs][x]);
+    float den = 0.f;
+    if (in)
+      for (int i = d; i < parts; i += D) {
+        const float* s = i ? rest + (int64_t)i * 2 * kSlot : first;
+        const float f = M == -INFINITY ? 0.f : ex2(__ldcg(s + r) - M);
+        weight[rs][i] = f;
+        den = fmaf(f, __ldcg(s + kRows + r), den);
       }
-    const int rr = tile * kRows + r, tok = rr / a.rep, hd = rr - tok * a.rep;
-    a.out[(((int64_t)at.b * a.T + tok) * a.nh + kh * a.rep + hd) * D + d] = f2bf(den == 0.f ? 0.f : num / den);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) den += __shfl_xor_sync(0xffffffffu, den, o);
+    if (lane == 0) red[1][rs][w] = den;
+    __syncthreads();
+    den = 0.f;
+#pragma unroll
+    for (int x = 0; x < kW; ++x) den += red[1][rs][x];
+    if (in) {
+      const int64_t at_d = 2 * kRows + r * D + d;
+      float num = weight[rs][0] * __ldcg(first + at_d);
+#pragma unroll 8
+      for (int i = 1; i < parts; ++i) num = fmaf(weight[rs][i], __ldcg(rest + (int64_t)i * 2 * kSlot + at_d), num);
+      const int rr = tile * kRows + r, tok = rr / a.rep, hd = rr - tok * a.rep;
+      a.out[(((int64_t)at.b * a.T + tok) * a.nh + kh * a.rep + hd) * D + d] = f2bf(den == 0.f ? 0.f : num / den);
+    }
+    __syncthreads();  // weight and red are written again
   }
 }
 
@@ -628,7 +663,7 @@ FewPlan few_plan(int num_sms, int B, int T, int nh, int nkv, int d, int64_t cap)
   p.tiles = (int)((rows + 16 * p.MT - 1) / (16 * p.MT));
   const int64_t blocks = (cap + kUnitKeys - 1) / kUnitKeys;
   const int64_t most = (int64_t)B * nkv * p.tiles * blocks;
-  p.G = (int)std::min<int64_t>(2 * num_sms, most);
+  p.G = (int)std::min<int64_t>(std::min(2 * num_sms, kMaxShares), most);
   p.join = blocks > 1 && p.G > 1;
   p.ws_bytes = p.join ? (uint64_t)2 * p.G * 16 * p.MT * (d + 2) * sizeof(float) : 0;
   return p;
