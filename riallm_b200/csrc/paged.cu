@@ -182,7 +182,7 @@ __device__ __forceinline__ bool odd16(uint32_t x) {  // either bf16 of x is infi
 // In a CTA each of 4 warps takes 16 keys of every unit and is its own
 // pipeline: cp.async into its own ring of kStages x (16 keys, 16 values),
 // scores and weighted sums on m16n8k16 matrix instructions (the up to
-// 16 * MT rows against 16 keys), running maximum and sum in registers, no
+// 16 rows against 16 keys), running maximum and sum in registers, no
 // barrier with other warps until a group's end. The products are 1/40 of
 // what even these instructions can do at the rate the bytes arrive, so
 // nothing is gained by a 128-row tcgen05 tile of which 4 to 32 rows are
@@ -191,8 +191,8 @@ constexpr int kUnitKeys = 64, kFewWarps = 4;
 
 template <int D>
 constexpr int kFewStages = D == 128 ? 3 : 6;
-template <int D, int MT>
-constexpr int kFewSmem = kFewWarps * kFewStages<D> * 2 * 16 * D * 2 + 16 * MT * D * 4;
+template <int D>
+constexpr int kFewSmem = kFewStages<D> * (kFewWarps * 2 + 1) * 16 * D * 2;
 
 // Share of CTA c of G: units [W c / G, W (c+1) / G). The CTA of unit u.
 __device__ __forceinline__ int64_t share_begin(int64_t W, int G, int c) { return W * c / G; }
@@ -278,19 +278,19 @@ struct Cursor {
 };
 
 // A partial result: maxima, sums and accumulators of the rows of one tile.
-template <int D, int MT>
-constexpr int kSlotFloats = 16 * MT * (D + 2);
+template <int D>
+constexpr int kSlotFloats = 16 * (D + 2);
 
-template <int D, int MT>
+template <int D>
 __global__ void __launch_bounds__(kFewWarps * 32, 2)
     few_rows_kernel(const AttnArgs a, int tiles, float* __restrict__ ws) {
-  constexpr int S = kFewStages<D>, C = D / 8, kRows = 16 * MT;
+  constexpr int S = kFewStages<D>, C = D / 8;
   extern __shared__ __align__(128) uint16_t smem[];
-  __shared__ float sm_m[kFewWarps][kRows], sm_l[kFewWarps][kRows];
+  __shared__ float sm_m[kFewWarps][16], sm_l[kFewWarps][16];
   rl::pdl_wait();
   rl::pdl_launch_dependents();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int groups = a.pg.nkv * tiles;
+  const int groups = a.pg.nkv * tiles, all_rows = a.T * a.rep;
   const UnitAt at = find_unit<kFewWarps * 32>(a, groups, gridDim.x, blockIdx.x);
   const int64_t u0 = at.u;
   if (u0 >= at.W) return;
@@ -303,13 +303,13 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
   Cursor ahead = now;
 
   uint16_t* ring = smem + warp * (S * 2 * 16 * D);
-  float* merged = reinterpret_cast<float*>(smem + kFewWarps * S * 2 * 16 * D);  // [kRows][D]
+  uint16_t* queries = smem + kFewWarps * S * 2 * 16 * D;  // S tiles of 16 query rows, for all warps
 
-  // Loads of unit n (counted from u0) go to stage n % S. Bit n % 32 of
-  // `held` says whether this warp has anything to do in unit n.
+  // Loads of unit n (counted from u0) go to stage n % S, and with a group's
+  // first unit its query rows, a quarter by each warp. Bit n % 32 of `held`
+  // says whether this warp has anything to do in unit n.
   uint32_t held = 0;
-  int issued = 0;
-  int page = -1;
+  int issued = 0, begun = 0, page = -1;
   auto key0 = [&](const Cursor& c) { return c.bl.index(c.i) * kUnitKeys + warp * 16; };
   auto fetch_page = [&]() {  // the page of the unit that is loaded next
     page = -1;
@@ -321,10 +321,24 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
   };
   auto issue = [&]() {
     if (issued < count) {
+      const int kh = ahead.g / tiles;
+      if (issued == 0 || ahead.i == 0) {
+        const int tile = ahead.g - kh * tiles;
+        uint16_t* to = queries + (begun % S) * 16 * D;
+#pragma unroll
+        for (int x = 0; x < 4 * C / 32; ++x) {
+          const int idx = x * 32 + lane, r = warp * 4 + idx / C, c = idx % C, rr = tile * 16 + r;
+          const bool in = rr < all_rows;
+          const int tok = in ? rr / a.rep : 0, hd = in ? rr - tok * a.rep : 0;
+          cp_async_16z(to + r * D + ((c ^ (r & 7)) * 8),
+                       a.q + (((int64_t)ahead.b * a.T + tok) * a.nh + kh * a.rep + hd) * D + c * 8, in ? 16 : 0);
+        }
+        ++begun;
+      }
       const bool ok = (unsigned)page < (unsigned)a.pg.num_pages;
       held = (held & ~(1u << (issued & 31))) | ((ok ? 1u : 0u) << (issued & 31));
       if (ok) {
-        const int j = key0(ahead), kh = ahead.g / tiles;
+        const int j = key0(ahead);
         const int64_t row = (((int64_t)page * a.pg.nkv + kh) << a.pg.lg) + (j & ((1 << a.pg.lg) - 1));
         uint16_t* ks = ring + (issued % S) * (2 * 16 * D);
         uint16_t* vs = ks + 16 * D;
@@ -348,106 +362,95 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
 #pragma unroll
   for (int s = 0; s < S - 1; ++s) issue();
 
-  uint32_t qf[MT][D / 16][4];
-  float o[MT][D / 8][4], m[MT][2], l[MT][2];
-  Span sp[MT][2];
-  int tile = 0, kh = 0, first = 0;
-  const int all_rows = a.T * a.rep;
+  uint32_t qf[D / 16][4];
+  float o[D / 8][4], m[2], l[2];
+  Span sp[2];
+  int tile = 0, kh = 0, first = 0, group = 0;
   for (int n = 0; n < count; ++n) {
+    rl::cp_async_wait<S - 2>();
     if (n == 0 || now.i == 0) {  // a group begins
+      __syncthreads();           // every warp's quarter of its query rows has arrived
       kh = now.g / tiles;
       tile = now.g - kh * tiles;
       first = n;
+      const uint16_t* qs = queries + (group % S) * 16 * D;
+      ++group;
 #pragma unroll
-      for (int t = 0; t < MT; ++t) {
-#pragma unroll
-        for (int x = 0; x < D / 8; ++x)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[t][x][e] = 0.f;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int r = tile * kRows + t * 16 + h * 8 + (lane >> 2);
-          m[t][h] = -INFINITY;
-          l[t][h] = 0.f;
-          const bool in = r < all_rows;
-          const int tok = in ? r / a.rep : 0, hd = in ? r - tok * a.rep : 0;
-          sp[t][h] = in ? a.span(now.p0 + tok) : Span{0, -1};
-          const uint32_t* qr = reinterpret_cast<const uint32_t*>(
-              a.q + (((int64_t)now.b * a.T + tok) * a.nh + kh * a.rep + hd) * D);
-#pragma unroll
-          for (int x = 0; x < D / 16; ++x) {
-            qf[t][x][h] = in ? __ldg(qr + x * 8 + (lane & 3)) : 0u;
-            qf[t][x][2 + h] = in ? __ldg(qr + x * 8 + 4 + (lane & 3)) : 0u;
-          }
-        }
+      for (int x = 0; x < D / 16; ++x) {
+        const int r = lane & 15, c = 2 * x + (lane >> 4);
+        ldmatrix_x4(qf[x], qs + r * D + ((c ^ (r & 7)) * 8));
       }
+#pragma unroll
+      for (int x = 0; x < D / 8; ++x)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[x][e] = 0.f;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int r = tile * 16 + h * 8 + (lane >> 2);
+        m[h] = -INFINITY;
+        l[h] = 0.f;
+        sp[h] = r < all_rows ? a.span(now.p0 + r / a.rep) : Span{0, -1};
+      }
+    } else {
+      __syncwarp();
     }
-    rl::cp_async_wait<S - 2>();
-    __syncwarp();
+    uint16_t* ks = ring + (n % S) * (2 * 16 * D);
+    uint16_t* vs = ks + 16 * D;
     if (held >> (n & 31) & 1) {
       const int j0 = key0(now);
-      uint16_t* ks = ring + (n % S) * (2 * 16 * D);
-      uint16_t* vs = ks + 16 * D;
-      float sc[MT][2][4];
+      float sc[2][4];
 #pragma unroll
-      for (int t = 0; t < MT; ++t)
+      for (int y = 0; y < 2; ++y)
 #pragma unroll
-        for (int y = 0; y < 2; ++y)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) sc[t][y][e] = 0.f;
+        for (int e = 0; e < 4; ++e) sc[y][e] = 0.f;
 #pragma unroll
       for (int x = 0; x < D / 16; ++x) {
         uint32_t kf[4];
         const int key = (lane & 7) + ((lane >> 4) << 3), c = 2 * x + ((lane >> 3) & 1);
         ldmatrix_x4(kf, ks + key * D + ((c ^ (key & 7)) * 8));
-#pragma unroll
-        for (int t = 0; t < MT; ++t) {
-          mma_16816(sc[t][0], qf[t][x], kf[0], kf[1]);
-          mma_16816(sc[t][1], qf[t][x], kf[2], kf[3]);
-        }
+        mma_16816(sc[0], qf[x], kf[0], kf[1]);
+        mma_16816(sc[1], qf[x], kf[2], kf[3]);
       }
       // Does any row of the sequence not see one of these keys?
       const int64_t pl = now.p0 + a.T - 1;
       const bool edge = j0 + 15 > min(now.p0, a.pg.cap() - 1) ||
                         (a.window > 0 && j0 < pl - a.window + 1 && j0 + 15 >= a.sinks);
 #pragma unroll
-      for (int t = 0; t < MT; ++t)
+      for (int h = 0; h < 2; ++h) {
+        float top = -INFINITY;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float top = -INFINITY;
+        for (int y = 0; y < 2; ++y)
 #pragma unroll
-          for (int y = 0; y < 2; ++y)
+          for (int e = 0; e < 2; ++e) {
+            float& x = sc[y][2 * h + e];
+            x *= a.scale_log2;
+            if (edge && !sees(sp[h], a.sinks, j0 + y * 8 + (lane & 3) * 2 + e)) x = -INFINITY;
+            top = fmaxf(top, x);
+          }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const float mn = fmaxf(m[h], top);
+        const float base = mn == -INFINITY ? 0.f : mn;
+        const float corr = ex2(m[h] - base);
+        m[h] = mn;
+        float sum = 0.f;
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              float& x = sc[t][y][2 * h + e];
-              x *= a.scale_log2;
-              if (edge && !sees(sp[t][h], a.sinks, j0 + y * 8 + (lane & 3) * 2 + e)) x = -INFINITY;
-              top = fmaxf(top, x);
-            }
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-          const float mn = fmaxf(m[t][h], top);
-          const float base = mn == -INFINITY ? 0.f : mn;
-          const float corr = ex2(m[t][h] - base);
-          m[t][h] = mn;
-          float sum = 0.f;
+        for (int y = 0; y < 2; ++y)
 #pragma unroll
-          for (int y = 0; y < 2; ++y)
+          for (int e = 0; e < 2; ++e) {
+            float& x = sc[y][2 * h + e];
+            x = ex2(x - base);
+            sum += x;
+          }
+        l[h] = fmaf(l[h], corr, sum);
+        if (__any_sync(0xffffffffu, corr != 1.f)) {
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              float& x = sc[t][y][2 * h + e];
-              x = ex2(x - base);
-              sum += x;
-            }
-          l[t][h] = fmaf(l[t][h], corr, sum);
-          if (__any_sync(0xffffffffu, corr != 1.f)) {
-#pragma unroll
-            for (int x = 0; x < D / 8; ++x) {
-              o[t][x][2 * h] *= corr;
-              o[t][x][2 * h + 1] *= corr;
-            }
+          for (int x = 0; x < D / 8; ++x) {
+            o[x][2 * h] *= corr;
+            o[x][2 * h + 1] *= corr;
           }
         }
+      }
       if (edge && a.T > 1) {
         // A value that is not finite, of a key that some rows see and some
         // do not: 0 times it would reach the latter through the product.
@@ -467,13 +470,11 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
               if (!odd16(w)) continue;
               const float lo = bf2f((uint16_t)w), hi = bf2f((uint16_t)(w >> 16));
 #pragma unroll
-              for (int t = 0; t < MT; ++t)
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-                  if (sees(sp[t][h], a.sinks, j0 + key)) {
-                    if (!isfinite(lo)) o[t][x][2 * h] += lo;
-                    if (!isfinite(hi)) o[t][x][2 * h + 1] += hi;
-                  }
+              for (int h = 0; h < 2; ++h)
+                if (sees(sp[h], a.sinks, j0 + key)) {
+                  if (!isfinite(lo)) o[x][2 * h] += lo;
+                  if (!isfinite(hi)) o[x][2 * h + 1] += hi;
+                }
             }
           __syncwarp();
           for (int x = lane; x < 16 * D; x += 32)
@@ -484,103 +485,92 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
       // The weights as bf16 and what that leaves, also as bf16: two products
       // keep 16 bits of each weight (one alone costs as much accuracy again
       // as the rounding of the output), and the matrix pipe is idle anyway.
-      uint32_t ph[MT][4], pr[MT][4];
+      uint32_t ph[4], pr[4];
 #pragma unroll
-      for (int t = 0; t < MT; ++t)
+      for (int y = 0; y < 2; ++y)
 #pragma unroll
-        for (int y = 0; y < 2; ++y)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float x0 = sc[t][y][2 * h], x1 = sc[t][y][2 * h + 1];
-            const uint32_t hi = rl::pack_bf16x2(x0, x1);
-            ph[t][2 * y + h] = hi;
-            pr[t][2 * y + h] = rl::pack_bf16x2(x0 - __uint_as_float(hi << 16), x1 - __uint_as_float(hi & 0xffff0000u));
-          }
+        for (int h = 0; h < 2; ++h) {
+          const float x0 = sc[y][2 * h], x1 = sc[y][2 * h + 1];
+          const uint32_t hi = rl::pack_bf16x2(x0, x1);
+          ph[2 * y + h] = hi;
+          pr[2 * y + h] = rl::pack_bf16x2(x0 - __uint_as_float(hi << 16), x1 - __uint_as_float(hi & 0xffff0000u));
+        }
 #pragma unroll
       for (int x = 0; x < D / 16; ++x) {
         uint32_t vf[4];
-        const int key = (lane & 7) + (((lane >> 3) & 1) << 3), c = 2 * x + (lane >> 4);
+        const int key = lane & 15, c = 2 * x + (lane >> 4);
         ldmatrix_x4_trans(vf, vs + key * D + ((c ^ (key & 7)) * 8));
-#pragma unroll
-        for (int t = 0; t < MT; ++t) {
-          mma_16816(o[t][2 * x], ph[t], vf[0], vf[1]);
-          mma_16816(o[t][2 * x + 1], ph[t], vf[2], vf[3]);
-          mma_16816(o[t][2 * x], pr[t], vf[0], vf[1]);
-          mma_16816(o[t][2 * x + 1], pr[t], vf[2], vf[3]);
-        }
+        mma_16816(o[2 * x], ph, vf[0], vf[1]);
+        mma_16816(o[2 * x + 1], ph, vf[2], vf[3]);
+        mma_16816(o[2 * x], pr, vf[0], vf[1]);
+        mma_16816(o[2 * x + 1], pr, vf[2], vf[3]);
       }
     }
     __syncwarp();
     issue();  // into the stage that was read before this one
 
     const bool whole_end = now.i + 1 == now.bl.n;
-    if (whole_end || n + 1 == count) {  // the group ends, or this CTA's share of it
+    if (whole_end || n + 1 == count) {
+      // The group ends, or this CTA's share of it. Each warp leaves its
+      // result in the stage it has just read (2 * 16 * D bf16 hold 16 * D
+      // floats), columns swizzled by the row; then all add up the four.
 #pragma unroll
-      for (int t = 0; t < MT; ++t)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          l[t][h] += __shfl_xor_sync(0xffffffffu, l[t][h], 1);
-          l[t][h] += __shfl_xor_sync(0xffffffffu, l[t][h], 2);
-          if ((lane & 3) == 0) {
-            sm_m[warp][t * 16 + h * 8 + (lane >> 2)] = m[t][h];
-            sm_l[warp][t * 16 + h * 8 + (lane >> 2)] = l[t][h];
-          }
+      for (int h = 0; h < 2; ++h) {
+        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+        const int r = h * 8 + (lane >> 2);
+        if ((lane & 3) == 0) {
+          sm_m[warp][r] = m[h];
+          sm_l[warp][r] = l[h];
         }
-      __syncthreads();
-      float f[MT][2];
 #pragma unroll
-      for (int t = 0; t < MT; ++t)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int r = t * 16 + h * 8 + (lane >> 2);
-          float M = sm_m[0][r];
-          for (int w = 1; w < kFewWarps; ++w) M = fmaxf(M, sm_m[w][r]);
-          f[t][h] = M == -INFINITY ? 0.f : ex2(m[t][h] - M);
-        }
-      for (int w = 0; w < kFewWarps; ++w) {  // in warp order: the same sum every time
-        if (warp == w)
-#pragma unroll
-          for (int t = 0; t < MT; ++t)
-#pragma unroll
-            for (int x = 0; x < D / 8; ++x)
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                float2* to = reinterpret_cast<float2*>(merged + (t * 16 + h * 8 + (lane >> 2)) * D + x * 8 +
-                                                       (lane & 3) * 2);
-                float2 y = w ? *to : make_float2(0.f, 0.f);
-                // A warp that has seen nothing adds nothing (0 * its NaN-free zeros).
-                y.x += o[t][x][2 * h] * f[t][h];
-                y.y += o[t][x][2 * h + 1] * f[t][h];
-                *to = y;
-              }
-        __syncthreads();
+        for (int x = 0; x < D / 8; ++x)
+          *reinterpret_cast<float2*>(reinterpret_cast<float*>(ks) + r * D + ((x * 8 + (lane & 3) * 2) ^ ((r & 3) * 8))) =
+              make_float2(o[x][2 * h], o[x][2 * h + 1]);
       }
+      __syncthreads();
       // Whole group here: the output. Otherwise the CTA's slot of partial
       // results, 2 per CTA: one for a group that began in an earlier share
       // or with this share, one for a group that began inside it.
       const bool whole = whole_end && now.i == n - first;
-      const int rows = min(kRows, all_rows - tile * kRows);
-      float* slot = ws + (2 * (int64_t)blockIdx.x + (first == 0 ? 0 : 1)) * kSlotFloats<D, MT>;
-      for (int x = threadIdx.x; x < rows * (D / 2); x += kFewWarps * 32) {
-        const int r = x / (D / 2), c = (x - r * (D / 2)) * 2;
-        const float2 y = *reinterpret_cast<const float2*>(merged + r * D + c);
-        float M = sm_m[0][r], L = 0.f;
+      const int rows = min(16, all_rows - tile * 16);
+      float* slot = ws + (2 * (int64_t)blockIdx.x + (first == 0 ? 0 : 1)) * kSlotFloats<D>;
+      const float* part = reinterpret_cast<const float*>(smem) + (n % S) * (16 * D);
+      for (int x = threadIdx.x; x < rows * (D / 4); x += kFewWarps * 32) {
+        const int r = x / (D / 4), c = (x - r * (D / 4)) * 4;
+        float M = sm_m[0][r];
+#pragma unroll
         for (int w = 1; w < kFewWarps; ++w) M = fmaxf(M, sm_m[w][r]);
-        for (int w = 0; w < kFewWarps; ++w) L += M == -INFINITY ? 0.f : sm_l[w][r] * ex2(sm_m[w][r] - M);
+        float L = 0.f;
+        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (M != -INFINITY)
+#pragma unroll
+          for (int w = 0; w < kFewWarps; ++w) {
+            const float f = ex2(sm_m[w][r] - M);
+            const float4 z = *reinterpret_cast<const float4*>(part + w * (S * 16 * D) + r * D + (c ^ ((r & 3) * 8)));
+            L = fmaf(sm_l[w][r], f, L);
+            y.x = fmaf(z.x, f, y.x);
+            y.y = fmaf(z.y, f, y.y);
+            y.z = fmaf(z.z, f, y.z);
+            y.w = fmaf(z.w, f, y.w);
+          }
         if (whole) {
           const float inv = L == 0.f ? 0.f : __fdiv_rn(1.f, L);
-          const int rr = tile * kRows + r, tok = rr / a.rep, hd = rr - tok * a.rep;
-          *reinterpret_cast<uint32_t*>(a.out + (((int64_t)now.b * a.T + tok) * a.nh + kh * a.rep + hd) * D + c) =
-              rl::pack_bf16x2(y.x * inv, y.y * inv);
+          const int rr = tile * 16 + r, tok = rr / a.rep, hd = rr - tok * a.rep;
+          *reinterpret_cast<uint2*>(a.out + (((int64_t)now.b * a.T + tok) * a.nh + kh * a.rep + hd) * D + c) =
+              make_uint2(rl::pack_bf16x2(y.x * inv, y.y * inv), rl::pack_bf16x2(y.z * inv, y.w * inv));
         } else {
-          *reinterpret_cast<float2*>(slot + 2 * kRows + r * D + c) = y;
+          // Two floats at a time: D + 2 floats a row keep 8-byte alignment only.
+          float2* to = reinterpret_cast<float2*>(slot + 32 + r * D + c);
+          to[0] = make_float2(y.x, y.y);
+          to[1] = make_float2(y.z, y.w);
           if (c == 0) {
             slot[r] = M;
-            slot[kRows + r] = L;
+            slot[16 + r] = L;
           }
         }
       }
-      __syncthreads();
+      __syncthreads();  // before the stages, sm_m and sm_l are written again
     }
     if (n + 1 < count) now.next(a, groups);
   }
@@ -591,9 +581,9 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
 // Threads (dimension, row); the weights of the parts are worked out once a
 // row, a part a thread.
 constexpr int kMaxShares = 512;
-template <int D, int MT>
+template <int D>
 __global__ void __launch_bounds__(D * 4) join_kernel(const AttnArgs a, int tiles, int G, const float* __restrict__ ws) {
-  constexpr int kRows = 16 * MT, kSlot = kSlotFloats<D, MT>, kW = D / 32;
+  constexpr int kRows = 16, kSlot = kSlotFloats<D>, kW = D / 32;
   __shared__ float weight[4][kMaxShares], red[2][4][kW];
   rl::pdl_wait();
   rl::pdl_launch_dependents();
@@ -649,38 +639,36 @@ __global__ void __launch_bounds__(D * 4) join_kernel(const AttnArgs a, int tiles
   }
 }
 
-// The launch of a call with few rows: CTAs, row tiles and whether a group
-// can be cut at all.
+// The launch of a call with few rows: row tiles of 16, CTAs, and whether a
+// group can be cut at all.
 struct FewPlan {
-  int MT, tiles, G;
+  int tiles, G;
   bool join;
   uint64_t ws_bytes;
 };
 FewPlan few_plan(int num_sms, int B, int T, int nh, int nkv, int d, int64_t cap) {
   FewPlan p;
   const int64_t rows = (int64_t)T * (nh / nkv);
-  p.MT = rows <= 16 ? 1 : 2;
-  p.tiles = (int)((rows + 16 * p.MT - 1) / (16 * p.MT));
+  p.tiles = (int)((rows + 15) / 16);
   const int64_t blocks = (cap + kUnitKeys - 1) / kUnitKeys;
   const int64_t most = (int64_t)B * nkv * p.tiles * blocks;
   p.G = (int)std::min<int64_t>(std::min(2 * num_sms, kMaxShares), most);
   p.join = blocks > 1 && p.G > 1;
-  p.ws_bytes = p.join ? (uint64_t)2 * p.G * 16 * p.MT * (d + 2) * sizeof(float) : 0;
+  p.ws_bytes = p.join ? (uint64_t)2 * p.G * 16 * (d + 2) * sizeof(float) : 0;
   return p;
 }
 
-template <int D, int MT>
+template <int D>
 int32_t launch_few(riallm_ctx* ctx, const AttnArgs& a, const FewPlan& p, float* ws, cudaStream_t st) {
-  if (int s = rl::allow_smem(ctx, "paged_attention", few_rows_kernel<D, MT>, kFewSmem<D, MT>,
-                             D / 64 * 2 + MT - 3))
-    return s;
-  if (int s = rl::launched(ctx, "paged_attention",
-                           rl::launch_pdl(few_rows_kernel<D, MT>, dim3(p.G), dim3(kFewWarps * 32), kFewSmem<D, MT>, st,
-                                          a, p.tiles, ws)))
+  const char* what = "paged_attention";
+  if (int s = rl::allow_smem(ctx, what, few_rows_kernel<D>, kFewSmem<D>, D / 64 - 1)) return s;
+  if (int s = rl::launched(ctx, what,
+                           rl::launch_pdl(few_rows_kernel<D>, dim3(p.G), dim3(kFewWarps * 32), kFewSmem<D>, st, a,
+                                          p.tiles, ws)))
     return s;
   if (!p.join) return RIALLM_OK;
-  return rl::launched(ctx, "paged_attention join",
-                      rl::launch_pdl(join_kernel<D, MT>, dim3(p.G - 1), dim3(D * 4), 0, st, a, p.tiles, p.G,
+  return rl::launched(ctx, what,
+                      rl::launch_pdl(join_kernel<D>, dim3(p.G - 1), dim3(D * 4), 0, st, a, p.tiles, p.G,
                                      static_cast<const float*>(ws)));
 }
 
@@ -778,8 +766,7 @@ int32_t riallm_cuda_paged_attention(riallm_ctx* ctx, const void* q, const void* 
     a.out = static_cast<uint16_t*>(out);
     float* ws = static_cast<float*>(workspace);
     cudaStream_t st = (cudaStream_t)stream;
-    if (d == 128) return p.MT == 1 ? launch_few<128, 1>(ctx, a, p, ws, st) : launch_few<128, 2>(ctx, a, p, ws, st);
-    return p.MT == 1 ? launch_few<64, 1>(ctx, a, p, ws, st) : launch_few<64, 2>(ctx, a, p, ws, st);
+    return d == 128 ? launch_few<128>(ctx, a, p, ws, st) : launch_few<64>(ctx, a, p, ws, st);
   });
 }
 
