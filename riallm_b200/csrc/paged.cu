@@ -113,12 +113,16 @@ struct AttnArgs {
   }
 };
 __device__ __forceinline__ bool sees(Span s, int sinks, int j) { return j <= s.hi && (j >= s.lo || j < sinks); }
+// Does some row between positions p0 and p1 not see some key of [j0, j1]?
+__device__ __forceinline__ bool is_edge(const AttnArgs& a, int64_t p0, int64_t p1, int j0, int j1) {
+  return j1 > min(p0, a.pg.cap() - 1) || (a.window > 0 && j0 < p1 - a.window + 1 && j1 >= a.sinks);
+}
 
-// The blocks of kBlock keys that some row of a sequence sees, in order: the
-// first `ns` hold sinks, the others start at block `w0`.
+// The blocks of kBlock keys that some row between two positions sees, in
+// order: the first `ns` hold sinks, the others start at block `w0`.
 struct Blocks {
   int ns, w0, n;
-  Span all;  // what the sequence's rows see together
+  Span all;  // what these rows see together
   __device__ __forceinline__ int index(int i) const { return i < ns ? i : w0 + i - ns; }
 };
 template <int kBlock>
@@ -134,6 +138,128 @@ __device__ __forceinline__ Blocks blocks_of(const AttnArgs& a, int64_t first, in
   r.n = max(1, r.ns + nw);  // one block, seen by nobody, where nothing is seen
   return r;
 }
+
+// The work of a call: the rows of every sequence in tiles of R; a group is
+// one (sequence, tile, kv head), a unit one of its blocks of kBlock keys.
+// Units are ordered by sequence, tile, kv head, block, and cut into as many
+// equal contiguous shares as there are CTAs, whatever the sequences' lengths
+// and the tiles' place under the causal diagonal; a group that a share
+// boundary cuts leaves partial results, which join_kernel adds up. The
+// lengths are the device's, so a captured call follows them.
+template <int R_, int kBlock_>
+struct Shape {
+  static constexpr int R = R_, kBlock = kBlock_;
+};
+struct Tile {
+  int b, row0, rows;    // sequence; first row and rows, of its T * rep
+  int64_t p0, p1;       // positions of the first and last row
+  Blocks bl;
+};
+template <typename Sh>
+__device__ __forceinline__ Tile tile_of(const AttnArgs& a, int tiles, int x) {
+  Tile t;
+  t.b = x / tiles;
+  t.row0 = (x - t.b * tiles) * Sh::R;
+  t.rows = min(Sh::R, a.T * a.rep - t.row0);
+  const int64_t p = a.pos[t.b];
+  t.p0 = p + t.row0 / a.rep;
+  t.p1 = p + (t.row0 + t.rows - 1) / a.rep;
+  t.bl = blocks_of<Sh::kBlock>(a, t.p0, t.p1);
+  return t;
+}
+// Where row r of a tile lies in q and out, in heads.
+__device__ __forceinline__ int64_t head_of(const AttnArgs& a, const Tile& t, int kh, int r) {
+  const int rr = t.row0 + r, tok = rr / a.rep;
+  return ((int64_t)t.b * a.T + tok) * a.nh + kh * a.rep + (rr - tok * a.rep);
+}
+
+// Share c of G: units [W c / G, W (c+1) / G). The share that unit u is in.
+__device__ __forceinline__ int64_t share_begin(int64_t W, int G, int c) { return W * c / G; }
+__device__ __forceinline__ int share_of(int64_t W, int G, int64_t u) { return (int)(((u + 1) * G - 1) / W); }
+
+// Finds where the first unit of share c (of the call's G shares, fewer where
+// there are fewer units) lies: every thread of a block of N threads sums the
+// units of its slab of tiles, and the thread whose slab holds the unit walks
+// it.
+struct UnitAt {
+  int64_t W;      // all units of the call
+  int G;          // shares, none of them empty
+  int64_t u;      // the share's first unit (W where there is no such share)
+  int64_t start;  // first unit of tile x, which holds u
+  int x;
+};
+template <typename Sh, int N>
+__device__ __forceinline__ UnitAt find_unit(const AttnArgs& a, int tiles, int G, int c) {
+  __shared__ int64_t sums[N / 32];
+  __shared__ int64_t sh_start;
+  __shared__ int sh_x;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int all = a.B * tiles, per = (all + N - 1) / N;
+  const int x0 = min(all, (int)threadIdx.x * per), x1 = min(all, x0 + per);
+  auto units = [&](int x) { return (int64_t)tile_of<Sh>(a, tiles, x).bl.n * a.pg.nkv; };
+  int64_t mine = 0;
+  for (int x = x0; x < x1; ++x) mine += units(x);
+  int64_t upto = mine;  // inclusive scan
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t y = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += y;
+  }
+  if (lane == 31) sums[warp] = upto;
+  __syncthreads();
+  UnitAt at;
+  at.W = 0;
+  int64_t before = 0;
+#pragma unroll
+  for (int w = 0; w < N / 32; ++w) {
+    before += w < warp ? sums[w] : 0;
+    at.W += sums[w];
+  }
+  at.G = (int)min((int64_t)G, at.W);
+  at.u = c < at.G ? share_begin(at.W, at.G, c) : at.W;
+  int64_t s = before + upto - mine;
+  if (at.u >= s && at.u < s + mine) {
+    for (int x = x0; x < x1; ++x) {
+      const int64_t n = units(x);
+      if (at.u < s + n) {
+        sh_x = x;
+        sh_start = s;
+        break;
+      }
+      s += n;
+    }
+  }
+  if (at.u >= at.W) return at;
+  __syncthreads();
+  at.x = sh_x;
+  at.start = sh_start;
+  return at;
+}
+
+// Walks the units from a place on.
+template <typename Sh>
+struct Cursor {
+  int x, kh, i;
+  Tile t;
+  __device__ __forceinline__ void init(const AttnArgs& a, int tiles, const UnitAt& at) {
+    x = at.x;
+    t = tile_of<Sh>(a, tiles, x);
+    kh = (int)((at.u - at.start) / t.bl.n);
+    i = (int)((at.u - at.start) - (int64_t)kh * t.bl.n);
+  }
+  __device__ __forceinline__ void next_group(const AttnArgs& a, int tiles) {
+    i = 0;
+    if (++kh < a.pg.nkv) return;
+    kh = 0;
+    if (++x < a.B * tiles) t = tile_of<Sh>(a, tiles, x);
+  }
+};
+
+// A share leaves at most two partial results, in slots 2c and 2c + 1: of the
+// group it begins with, and of one that begins inside it. A slot holds the
+// maxima, the sums and the accumulators of a tile's rows.
+template <typename Sh, int D>
+constexpr int kSlotFloats = Sh::R * (D + 2);
 
 __device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], const void* p) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
@@ -172,12 +298,7 @@ __device__ __forceinline__ bool odd16(uint32_t x) {  // either bf16 of x is infi
 // ---------------------------------------------------------------- few rows
 //
 // Attention of few rows per sequence (single new tokens, drafted ones): a
-// pass over the keys and values, bound by reading them. The work of a call,
-// 64 keys of one (sequence, kv head, row tile) group a unit, is cut into as
-// many equal contiguous shares as there are CTAs, whatever the sequences'
-// lengths; a group that a share boundary cuts leaves partial results, which
-// join_kernel adds up. The lengths are the device's, so a captured call
-// follows them.
+// pass over the keys and values, bound by reading them.
 //
 // In a CTA each of 4 warps takes 16 keys of every unit and is its own
 // pipeline: cp.async into its own ring of kStages x (16 keys, 16 values),
@@ -185,101 +306,15 @@ __device__ __forceinline__ bool odd16(uint32_t x) {  // either bf16 of x is infi
 // 16 rows against 16 keys), running maximum and sum in registers, no
 // barrier with other warps until a group's end. The products are 1/40 of
 // what even these instructions can do at the rate the bytes arrive, so
-// nothing is gained by a 128-row tcgen05 tile of which 4 to 32 rows are
+// nothing is gained by a 128-row tcgen05 tile of which 4 to 16 rows are
 // used.
-constexpr int kUnitKeys = 64, kFewWarps = 4;
+constexpr int kFewWarps = 4;
+using Few = Shape<16, 64>;
 
 template <int D>
 constexpr int kFewStages = D == 128 ? 3 : 6;
 template <int D>
 constexpr int kFewSmem = kFewStages<D> * (kFewWarps * 2 + 1) * 16 * D * 2;
-
-// Share of CTA c of G: units [W c / G, W (c+1) / G). The CTA of unit u.
-__device__ __forceinline__ int64_t share_begin(int64_t W, int G, int c) { return W * c / G; }
-__device__ __forceinline__ int share_of(int64_t W, int G, int64_t u) { return (int)(((u + 1) * G - 1) / W); }
-
-// Finds where the first unit of share c (of the call's G shares, fewer where
-// there are fewer units) lies: every thread of a block of N threads sums the
-// units of its slab of sequences, and the thread whose slab holds the unit
-// walks it.
-struct UnitAt {
-  int64_t W;      // all units of the call
-  int G;          // shares, none of them empty
-  int64_t u;      // the share's first unit (W where there is no such share)
-  int64_t start;  // first unit of sequence b, which holds u
-  int b;
-  Blocks bl;
-};
-template <int N>
-__device__ __forceinline__ UnitAt find_unit(const AttnArgs& a, int groups, int G, int c) {
-  __shared__ int64_t sums[N / 32];
-  __shared__ int64_t sh_start;
-  __shared__ int sh_b;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int per = (a.B + N - 1) / N;
-  const int b0 = min(a.B, (int)threadIdx.x * per), b1 = min(a.B, b0 + per);
-  int64_t mine = 0;
-  for (int b = b0; b < b1; ++b)
-    mine += (int64_t)blocks_of<kUnitKeys>(a, a.pos[b], (int64_t)a.pos[b] + a.T - 1).n * groups;
-  int64_t upto = mine;  // inclusive scan
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int64_t x = __shfl_up_sync(0xffffffffu, upto, o);
-    if (lane >= o) upto += x;
-  }
-  if (lane == 31) sums[warp] = upto;
-  __syncthreads();
-  UnitAt at;
-  at.W = 0;
-  int64_t before = 0;
-#pragma unroll
-  for (int w = 0; w < N / 32; ++w) {
-    before += w < warp ? sums[w] : 0;
-    at.W += sums[w];
-  }
-  at.G = (int)min((int64_t)G, at.W);
-  at.u = c < at.G ? share_begin(at.W, at.G, c) : at.W;
-  int64_t s = before + upto - mine;
-  if (at.u >= s && at.u < s + mine) {
-    for (int b = b0; b < b1; ++b) {
-      const int64_t n = (int64_t)blocks_of<kUnitKeys>(a, a.pos[b], (int64_t)a.pos[b] + a.T - 1).n * groups;
-      if (at.u < s + n) {
-        sh_b = b;
-        sh_start = s;
-        break;
-      }
-      s += n;
-    }
-  }
-  if (at.u >= at.W) return at;
-  __syncthreads();
-  at.b = sh_b;
-  at.start = sh_start;
-  at.bl = blocks_of<kUnitKeys>(a, a.pos[at.b], (int64_t)a.pos[at.b] + a.T - 1);
-  return at;
-}
-
-// Walks the units of a share.
-struct Cursor {
-  int b, g, i;
-  int64_t p0;
-  Blocks bl;
-  __device__ __forceinline__ void load(const AttnArgs& a) {
-    p0 = a.pos[b];
-    bl = blocks_of<kUnitKeys>(a, p0, p0 + a.T - 1);
-  }
-  __device__ __forceinline__ void next(const AttnArgs& a, int groups) {
-    if (++i < bl.n) return;
-    i = 0;
-    if (++g < groups) return;
-    g = 0;
-    if (++b < a.B) load(a);
-  }
-};
-
-// A partial result: maxima, sums and accumulators of the rows of one tile.
-template <int D>
-constexpr int kSlotFloats = 16 * (D + 2);
 
 template <int D>
 __global__ void __launch_bounds__(kFewWarps * 32, 2)
@@ -290,48 +325,41 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
   rl::pdl_wait();
   rl::pdl_launch_dependents();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int groups = a.pg.nkv * tiles, all_rows = a.T * a.rep;
-  const UnitAt at = find_unit<kFewWarps * 32>(a, groups, gridDim.x, blockIdx.x);
-  const int64_t u0 = at.u;
-  if (u0 >= at.W) return;
-  const int count = (int)(share_begin(at.W, at.G, blockIdx.x + 1) - u0);
-  Cursor now;
-  now.b = at.b;
-  now.load(a);
-  now.g = (int)((u0 - at.start) / now.bl.n);
-  now.i = (int)((u0 - at.start) - (int64_t)now.g * now.bl.n);
-  Cursor ahead = now;
+  const UnitAt at = find_unit<Few, kFewWarps * 32>(a, tiles, gridDim.x, blockIdx.x);
+  if (at.u >= at.W) return;
+  const int count = (int)(share_begin(at.W, at.G, blockIdx.x + 1) - at.u);
+  Cursor<Few> now;
+  now.init(a, tiles, at);
+  Cursor<Few> ahead = now;
 
   uint16_t* ring = smem + warp * (S * 2 * 16 * D);
   uint16_t* queries = smem + kFewWarps * S * 2 * 16 * D;  // S tiles of 16 query rows, for all warps
 
-  // Loads of unit n (counted from u0) go to stage n % S, and with a group's
+  // Loads of unit n (of the share) go to stage n % S, and with a group's
   // first unit its query rows, a quarter by each warp. Bit n % 32 of `held`
   // says whether this warp has anything to do in unit n.
   uint32_t held = 0;
   int issued = 0, begun = 0, page = -1;
-  auto key0 = [&](const Cursor& c) { return c.bl.index(c.i) * kUnitKeys + warp * 16; };
+  auto key0 = [&](const Cursor<Few>& c) { return c.t.bl.index(c.i) * Few::kBlock + warp * 16; };
   auto fetch_page = [&]() {  // the page of the unit that is loaded next
     page = -1;
     if (issued < count) {
       const int j = key0(ahead);
-      const bool any = j <= ahead.bl.all.hi && (j + 15 >= ahead.bl.all.lo || j < a.sinks);
-      if (any) page = a.pg.table[ahead.b * a.pg.stride + (j >> a.pg.lg)];
+      const Span all = ahead.t.bl.all;
+      const bool any = j <= all.hi && (j + 15 >= all.lo || j < a.sinks);
+      if (any) page = a.pg.table[ahead.t.b * a.pg.stride + (j >> a.pg.lg)];
     }
   };
   auto issue = [&]() {
     if (issued < count) {
-      const int kh = ahead.g / tiles;
       if (issued == 0 || ahead.i == 0) {
-        const int tile = ahead.g - kh * tiles;
         uint16_t* to = queries + (begun % S) * 16 * D;
 #pragma unroll
         for (int x = 0; x < 4 * C / 32; ++x) {
-          const int idx = x * 32 + lane, r = warp * 4 + idx / C, c = idx % C, rr = tile * 16 + r;
-          const bool in = rr < all_rows;
-          const int tok = in ? rr / a.rep : 0, hd = in ? rr - tok * a.rep : 0;
-          cp_async_16z(to + r * D + ((c ^ (r & 7)) * 8),
-                       a.q + (((int64_t)ahead.b * a.T + tok) * a.nh + kh * a.rep + hd) * D + c * 8, in ? 16 : 0);
+          const int idx = x * 32 + lane, r = warp * 4 + idx / C, c = idx % C;
+          const bool in = r < ahead.t.rows;
+          cp_async_16z(to + r * D + ((c ^ (r & 7)) * 8), a.q + head_of(a, ahead.t, ahead.kh, in ? r : 0) * D + c * 8,
+                       in ? 16 : 0);
         }
         ++begun;
       }
@@ -339,13 +367,13 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
       held = (held & ~(1u << (issued & 31))) | ((ok ? 1u : 0u) << (issued & 31));
       if (ok) {
         const int j = key0(ahead);
-        const int64_t row = (((int64_t)page * a.pg.nkv + kh) << a.pg.lg) + (j & ((1 << a.pg.lg) - 1));
+        const int64_t row = (((int64_t)page * a.pg.nkv + ahead.kh) << a.pg.lg) + (j & ((1 << a.pg.lg) - 1));
         uint16_t* ks = ring + (issued % S) * (2 * 16 * D);
         uint16_t* vs = ks + 16 * D;
 #pragma unroll
         for (int x = 0; x < 16 * C / 32; ++x) {
           const int idx = x * 32 + lane, key = idx / C, c = idx % C;
-          const bool in = sees(ahead.bl.all, a.sinks, j + key);
+          const bool in = sees(ahead.t.bl.all, a.sinks, j + key);
           const int64_t off = (row + (in ? key : 0)) * D + c * 8;
           const int to = key * D + ((c ^ (key & 7)) * 8);
           cp_async_16z(ks + to, a.k + off, in ? 16 : 0);
@@ -353,7 +381,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
         }
       }
       ++issued;
-      if (issued < count) ahead.next(a, groups);
+      if (issued < count && ++ahead.i == ahead.t.bl.n) ahead.next_group(a, tiles);
       fetch_page();
     }
     rl::cp_async_commit();
@@ -365,13 +393,11 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
   uint32_t qf[D / 16][4];
   float o[D / 8][4], m[2], l[2];
   Span sp[2];
-  int tile = 0, kh = 0, first = 0, group = 0;
+  int first = 0, group = 0;
   for (int n = 0; n < count; ++n) {
     rl::cp_async_wait<S - 2>();
     if (n == 0 || now.i == 0) {  // a group begins
       __syncthreads();           // every warp's quarter of its query rows has arrived
-      kh = now.g / tiles;
-      tile = now.g - kh * tiles;
       first = n;
       const uint16_t* qs = queries + (group % S) * 16 * D;
       ++group;
@@ -386,10 +412,10 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
         for (int e = 0; e < 4; ++e) o[x][e] = 0.f;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int r = tile * 16 + h * 8 + (lane >> 2);
+        const int r = h * 8 + (lane >> 2);
         m[h] = -INFINITY;
         l[h] = 0.f;
-        sp[h] = r < all_rows ? a.span(now.p0 + r / a.rep) : Span{0, -1};
+        sp[h] = r < now.t.rows ? a.span(now.t.p0 + (now.t.row0 + r) / a.rep - now.t.row0 / a.rep) : Span{0, -1};
       }
     } else {
       __syncwarp();
@@ -411,10 +437,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
         mma_16816(sc[0], qf[x], kf[0], kf[1]);
         mma_16816(sc[1], qf[x], kf[2], kf[3]);
       }
-      // Does any row of the sequence not see one of these keys?
-      const int64_t pl = now.p0 + a.T - 1;
-      const bool edge = j0 + 15 > min(now.p0, a.pg.cap() - 1) ||
-                        (a.window > 0 && j0 < pl - a.window + 1 && j0 + 15 >= a.sinks);
+      const bool edge = is_edge(a, now.t.p0, now.t.p1, j0, j0 + 15);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         float top = -INFINITY;
@@ -451,7 +474,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
           }
         }
       }
-      if (edge && a.T > 1) {
+      if (edge && now.t.p1 > now.t.p0) {
         // A value that is not finite, of a key that some rows see and some
         // do not: 0 times it would reach the latter through the product.
         // It is added to the rows that see it and zeroed for the product.
@@ -509,7 +532,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
     __syncwarp();
     issue();  // into the stage that was read before this one
 
-    const bool whole_end = now.i + 1 == now.bl.n;
+    const bool whole_end = now.i + 1 == now.t.bl.n;
     if (whole_end || n + 1 == count) {
       // The group ends, or this CTA's share of it. Each warp leaves its
       // result in the stage it has just read (2 * 16 * D bf16 hold 16 * D
@@ -529,14 +552,10 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
               make_float2(o[x][2 * h], o[x][2 * h + 1]);
       }
       __syncthreads();
-      // Whole group here: the output. Otherwise the CTA's slot of partial
-      // results, 2 per CTA: one for a group that began in an earlier share
-      // or with this share, one for a group that began inside it.
       const bool whole = whole_end && now.i == n - first;
-      const int rows = min(16, all_rows - tile * 16);
-      float* slot = ws + (2 * (int64_t)blockIdx.x + (first == 0 ? 0 : 1)) * kSlotFloats<D>;
+      float* slot = ws + (2 * (int64_t)blockIdx.x + (first == 0 ? 0 : 1)) * kSlotFloats<Few, D>;
       const float* part = reinterpret_cast<const float*>(smem) + (n % S) * (16 * D);
-      for (int x = threadIdx.x; x < rows * (D / 4); x += kFewWarps * 32) {
+      for (int x = threadIdx.x; x < now.t.rows * (D / 4); x += kFewWarps * 32) {
         const int r = x / (D / 4), c = (x - r * (D / 4)) * 4;
         float M = sm_m[0][r];
 #pragma unroll
@@ -556,14 +575,10 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
           }
         if (whole) {
           const float inv = L == 0.f ? 0.f : __fdiv_rn(1.f, L);
-          const int rr = tile * 16 + r, tok = rr / a.rep, hd = rr - tok * a.rep;
-          *reinterpret_cast<uint2*>(a.out + (((int64_t)now.b * a.T + tok) * a.nh + kh * a.rep + hd) * D + c) =
+          *reinterpret_cast<uint2*>(a.out + head_of(a, now.t, now.kh, r) * D + c) =
               make_uint2(rl::pack_bf16x2(y.x * inv, y.y * inv), rl::pack_bf16x2(y.z * inv, y.w * inv));
         } else {
-          // Two floats at a time: D + 2 floats a row keep 8-byte alignment only.
-          float2* to = reinterpret_cast<float2*>(slot + 32 + r * D + c);
-          to[0] = make_float2(y.x, y.y);
-          to[1] = make_float2(y.z, y.w);
+          *reinterpret_cast<float4*>(slot + 32 + r * D + c) = y;
           if (c == 0) {
             slot[r] = M;
             slot[16 + r] = L;
@@ -572,35 +587,36 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
       }
       __syncthreads();  // before the stages, sm_m and sm_l are written again
     }
-    if (n + 1 < count) now.next(a, groups);
+    if (n + 1 < count && ++now.i == now.t.bl.n) now.next_group(a, tiles);
   }
 }
 
 // CTA c adds up the partial results of the group that the boundary between
-// the shares c and c + 1 cuts, if c is the first that holds part of it.
-// Threads (dimension, row); the weights of the parts are worked out once a
-// row, a part a thread.
+// the shares c and c + 1 cuts, if c is the first that holds part of it; 16
+// rows per CTA. Threads (dimension, row); the weights of the parts are worked
+// out once a row, a part a thread.
 constexpr int kMaxShares = 512;
-template <int D>
+template <typename Sh, int D>
 __global__ void __launch_bounds__(D * 4) join_kernel(const AttnArgs a, int tiles, int G, const float* __restrict__ ws) {
-  constexpr int kRows = 16, kSlot = kSlotFloats<D>, kW = D / 32;
+  constexpr int kSlot = kSlotFloats<Sh, D>, kW = D / 32;
   __shared__ float weight[4][kMaxShares], red[2][4][kW];
   rl::pdl_wait();
   rl::pdl_launch_dependents();
-  const int groups = a.pg.nkv * tiles, c0 = blockIdx.x;
-  const UnitAt at = find_unit<D * 4>(a, groups, G, c0 + 1);
+  const int c0 = blockIdx.x;
+  const UnitAt at = find_unit<Sh, D * 4>(a, tiles, G, c0 + 1);
   if (at.u >= at.W) return;
-  const int64_t g = (at.u - at.start) / at.bl.n, g0 = at.start + g * at.bl.n, g1 = g0 + at.bl.n;
-  if (at.u == g0 || share_of(at.W, at.G, g0) != c0) return;  // not cut here, or cut before as well
+  Cursor<Sh> cut;
+  cut.init(a, tiles, at);
+  const int64_t g0 = at.u - cut.i, g1 = g0 + cut.t.bl.n;
+  if (cut.i == 0 || share_of(at.W, at.G, g0) != c0) return;  // not cut here, or cut before as well
   const int parts = share_of(at.W, at.G, g1 - 1) - c0 + 1;
   // The first part is in its CTA's second slot where the group began inside
   // that CTA's share.
   const float* first = ws + (2 * (int64_t)c0 + (share_begin(at.W, at.G, c0) < g0 ? 1 : 0)) * kSlot;
   const float* rest = ws + 2 * (int64_t)c0 * kSlot;
-  const int kh = (int)(g / tiles), tile = (int)(g - (int64_t)kh * tiles);
-  const int rows = min(kRows, a.T * a.rep - tile * kRows);
+  const int rows = min(cut.t.rows, (int)(blockIdx.y + 1) * 16);
   const int d = threadIdx.x % D, rs = threadIdx.x / D, lane = d & 31, w = d >> 5;
-  for (int r0 = 0; r0 < rows; r0 += 4) {
+  for (int r0 = blockIdx.y * 16; r0 < rows; r0 += 4) {
     const int r = r0 + rs;
     const bool in = r < rows;
     float M = -INFINITY;
@@ -618,7 +634,7 @@ __global__ void __launch_bounds__(D * 4) join_kernel(const AttnArgs a, int tiles
         const float* s = i ? rest + (int64_t)i * 2 * kSlot : first;
         const float f = M == -INFINITY ? 0.f : ex2(__ldcg(s + r) - M);
         weight[rs][i] = f;
-        den = fmaf(f, __ldcg(s + kRows + r), den);
+        den = fmaf(f, __ldcg(s + Sh::R + r), den);
       }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) den += __shfl_xor_sync(0xffffffffu, den, o);
@@ -628,12 +644,11 @@ __global__ void __launch_bounds__(D * 4) join_kernel(const AttnArgs a, int tiles
 #pragma unroll
     for (int x = 0; x < kW; ++x) den += red[1][rs][x];
     if (in) {
-      const int64_t at_d = 2 * kRows + r * D + d;
+      const int64_t at_d = 2 * Sh::R + r * D + d;
       float num = weight[rs][0] * __ldcg(first + at_d);
 #pragma unroll 8
       for (int i = 1; i < parts; ++i) num = fmaf(weight[rs][i], __ldcg(rest + (int64_t)i * 2 * kSlot + at_d), num);
-      const int rr = tile * kRows + r, tok = rr / a.rep, hd = rr - tok * a.rep;
-      a.out[(((int64_t)at.b * a.T + tok) * a.nh + kh * a.rep + hd) * D + d] = f2bf(den == 0.f ? 0.f : num / den);
+      a.out[head_of(a, cut.t, cut.kh, r) * D + d] = f2bf(den == 0.f ? 0.f : num / den);
     }
     __syncthreads();  // weight and red are written again
   }
@@ -650,7 +665,7 @@ FewPlan few_plan(int num_sms, int B, int T, int nh, int nkv, int d, int64_t cap)
   FewPlan p;
   const int64_t rows = (int64_t)T * (nh / nkv);
   p.tiles = (int)((rows + 15) / 16);
-  const int64_t blocks = (cap + kUnitKeys - 1) / kUnitKeys;
+  const int64_t blocks = (cap + Few::kBlock - 1) / Few::kBlock;
   const int64_t most = (int64_t)B * nkv * p.tiles * blocks;
   p.G = (int)std::min<int64_t>(std::min(2 * num_sms, kMaxShares), most);
   p.join = blocks > 1 && p.G > 1;
@@ -668,7 +683,7 @@ int32_t launch_few(riallm_ctx* ctx, const AttnArgs& a, const FewPlan& p, float* 
     return s;
   if (!p.join) return RIALLM_OK;
   return rl::launched(ctx, what,
-                      rl::launch_pdl(join_kernel<D>, dim3(p.G - 1), dim3(D * 4), 0, st, a, p.tiles, p.G,
+                      rl::launch_pdl(join_kernel<Few, D>, dim3(p.G - 1), dim3(D * 4), 0, st, a, p.tiles, p.G,
                                      static_cast<const float*>(ws)));
 }
 
