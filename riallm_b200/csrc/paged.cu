@@ -591,6 +591,521 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
   }
 }
 
+// --------------------------------------------------------------- many rows
+//
+// Attention of a prompt or of a tile of drafted rows on tcgen05: scores
+// S = Q K^T and sums O += P V of 128 rows against blocks of 128 keys, S, P
+// and O in tensor memory. Bound by the matrix rate where d = 128 (1024
+// cycles for 128 x 128 pairs), and as much by 16384 exponentials at 16 a
+// cycle.
+//
+// Two slots of 128 rows each, so that one's products run while the other's
+// weights are worked out:
+//   kTwoTiles  : 256 rows a tile, a slot each half, both against every block
+//                (a block's keys and values are read once for 256 rows);
+//   !kTwoTiles : up to 128 rows a tile, the slots take the blocks in turn
+//                and are added up at the group's end.
+// Roles: warps 0-3 and 4-7 the two slots' weights (a thread a row), warp 8
+// loads blocks by TMA, page by page, warp 9 issues the products, warp 10
+// looks through the values of blocks that some row of the tile does not see
+// whole, warp 11 has none. Keys and values share a ring of kStages blocks in smem.
+constexpr int kManyThreads = 12 * 32;
+// Registers: the launch's 168 a thread, of which the third warpgroup (loads,
+// products) keeps 88 and the weights' two take 208 (2 * 208 + 88 = 3 * 168).
+constexpr int kWeightRegs = 208, kOtherRegs = 88;
+constexpr int kMaxStages = 8;
+template <bool kTwoTiles>
+using Many = Shape<kTwoTiles ? 256 : 128, 128>;
+template <int D>
+constexpr int kManyStages = D == 128 ? 4 : 8;
+template <int D>
+constexpr int kTileBytes = 128 * D * 2;
+// Two query tiles (with !kTwoTiles one, and room to add the slots up), the
+// ring, and slack to start at a multiple of 1024.
+template <int D>
+constexpr int kManySmem = (2 + kManyStages<D>) * kTileBytes<D> + 1024;
+
+struct ManyBars {
+  uint64_t full[kMaxStages], empty[kMaxStages], ok[kMaxStages];  // loaded, read, looked through (values)
+  uint64_t q_full, s_full[2], p_full[2], pv_done[2], merge_full, merge_empty, drain;
+};
+
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort, int* status) {
+  return __all_sync(0xffffffffu, rl::mbar_wait(bar, parity, abort, status));
+}
+// A bounded wait for work in flight on the way out.
+__device__ __forceinline__ void drain_wait(uint64_t* bar, uint32_t parity) {
+  const uint64_t t0 = rl::globaltimer_ns();
+  while (!rl::mbar_try_wait_suspend(bar, parity, 2000u))
+    if (rl::globaltimer_ns() - t0 > rl::kWaitLimitNs) return;
+}
+
+// The part of a group that a share holds: blocks [i0, i1).
+template <typename Sh>
+struct Segments {
+  Cursor<Sh> c;
+  int64_t left;
+  int i0, i1;
+  __device__ __forceinline__ void init(const AttnArgs& a, int tiles, const UnitAt& at, int64_t count) {
+    c.init(a, tiles, at);
+    left = count;
+    i0 = c.i;
+    i1 = (int)min((int64_t)c.t.bl.n, i0 + left);
+  }
+  __device__ __forceinline__ bool next(const AttnArgs& a, int tiles) {
+    left -= i1 - i0;
+    if (left <= 0) return false;
+    c.next_group(a, tiles);
+    i0 = 0;
+    i1 = (int)min((int64_t)c.t.bl.n, left);
+    return true;
+  }
+};
+
+template <int D, bool kTwoTiles>
+__global__ void __launch_bounds__(kManyThreads, 1)
+    many_rows_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap,
+                     const __grid_constant__ CUtensorMap vmap, int tiles, float* __restrict__ ws, int* status) {
+  using Sh = Many<kTwoTiles>;
+  constexpr int S = kManyStages<D>, H = D / 64, kHalf = 128 * 128;  // a tile is H column halves of 128 x 128 B
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ ManyBars bars;
+  __shared__ uint32_t tmem_base;
+  __shared__ int abort_flag;
+  __shared__ uint32_t gone[8];    // block n % 8: its pages that are not held, or that nobody sees
+  __shared__ int poison[16];      // segment n % 16: a value that some rows must not meet is not finite
+  __shared__ float ml[2][128];    // slot 1's maxima and sums, !kTwoTiles
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  uint8_t* qs = smem;                          // 2 tiles
+  uint8_t* ring = smem + 2 * kTileBytes<D>;
+  float* merge = reinterpret_cast<float*>(smem + kTileBytes<D>);  // [D / 2 columns][128 rows], !kTwoTiles
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  volatile int* abort = &abort_flag;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kMaxStages; ++i) {
+      rl::mbar_init(&bars.full[i], 1);
+      rl::mbar_init(&bars.empty[i], 1);
+      rl::mbar_init(&bars.ok[i], 1);
+    }
+    rl::mbar_init(&bars.q_full, 256);
+    for (int i = 0; i < 2; ++i) {
+      rl::mbar_init(&bars.s_full[i], 1);
+      rl::mbar_init(&bars.p_full[i], 128);
+      rl::mbar_init(&bars.pv_done[i], 1);
+    }
+    rl::mbar_init(&bars.merge_full, 128);
+    rl::mbar_init(&bars.merge_empty, 128);
+    rl::mbar_init(&bars.drain, 1);
+    rl::fence_mbar_init();
+    abort_flag = 0;
+    for (int i = 0; i < 16; ++i) poison[i] = 0;
+  }
+  if (warp == 9) {
+    rl::tmem_alloc(&tmem_base, 512);
+    rl::tmem_relinquish();
+  }
+  rl::tc_fence_before();
+  __syncthreads();
+  rl::tc_fence_after();
+  rl::pdl_wait();
+  rl::pdl_launch_dependents();
+  const uint32_t tm = tmem_base;
+
+  const UnitAt at = find_unit<Sh, kManyThreads>(a, tiles, gridDim.x, blockIdx.x);
+  const bool work = at.u < at.W;
+  const int64_t count = work ? share_begin(at.W, at.G, blockIdx.x + 1) - at.u : 0;
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+    Segments<Sh> sg;
+    if (work) sg.init(a, tiles, at, count);
+    if (work && warp == 8) {
+      // ------------------------------------------------ loads
+      const int per_page = 1 << a.pg.lg, pages = 128 >> a.pg.lg;
+      const int none = (int)((int64_t)a.pg.num_pages * a.pg.nkv << a.pg.lg);  // past the pool: zeros
+      int n = 0;  // blocks so far; its keys are load 2n of the ring, its values 2n + 1
+      int loads = 0;
+      bool go = true;
+      do {
+        for (int i = sg.i0; go && i < sg.i1; ++i, ++n) {
+          const int j = sg.c.t.bl.index(i) * 128 + (lane << a.pg.lg);
+          int row = none;
+          if (lane < pages && j <= sg.c.t.bl.all.hi && (j + per_page > sg.c.t.bl.all.lo || j < a.sinks)) {
+            const int64_t r = a.pg.row(sg.c.t.b, sg.c.kh, j);
+            if (r >= 0) row = (int)r;
+          }
+          const uint32_t bad = __ballot_sync(0xffffffffu, lane < pages && row == none);
+#pragma unroll
+          for (int kv = 0; kv < 2; ++kv) {
+            const int ld = 2 * n + kv, st = ld % S;
+            if (ld >= S && !warp_wait(&bars.empty[st], (ld / S - 1) & 1, abort, status)) {
+              go = false;
+              break;
+            }
+            if (lane == 0) {
+              // Its last reader has given block n - 8's values back.
+              if (kv == 0) *(volatile uint32_t*)&gone[n & 7] = bad;
+              rl::mbar_arrive_expect_tx(&bars.full[st], kTileBytes<D>);
+            }
+            __syncwarp();
+            ++loads;
+            if (lane < pages) {
+              uint8_t* to = ring + st * kTileBytes<D> + lane * per_page * 128;
+#pragma unroll
+              for (int h = 0; h < H; ++h)
+                rl::tma_load_2d(to + h * kHalf, kv ? &vmap : &kmap, &bars.full[st], h * 64, row);
+            }
+          }
+        }
+      } while (go && sg.next(a, tiles));
+      if (!go) {  // loads in flight end before the CTA does
+        for (int ld = max(0, loads - S); ld < loads; ++ld) drain_wait(&bars.full[ld % S], (ld / S) & 1);
+      }
+    } else if (work && warp == 9) {
+      // --------------------------------------------- products
+      if (lane == 0) {
+        constexpr uint32_t kIdS = rl::idesc_bf16_f32(128, 128);
+        constexpr uint32_t kIdO = rl::idesc_bf16_f32(128, D) | (1u << 16);  // B (the values) MN-major
+        const uint32_t ring_a = rl::smem_u32(ring), q_a = rl::smem_u32(qs);
+        auto scores = [&](int slot, int st) {
+          const uint32_t qa = q_a + (kTwoTiles ? slot * kTileBytes<D> : 0), ka = ring_a + st * kTileBytes<D>;
+#pragma unroll
+          for (int x = 0; x < D / 16; ++x) {
+            const uint32_t off = (x / 4) * kHalf + (x % 4) * 32;
+            rl::tc_mma_ss(tm + slot * 128, rl::sdesc_kmajor_sw128(qa + off), rl::sdesc_kmajor_sw128(ka + off), kIdS,
+                          x > 0);
+          }
+          rl::tc_commit(&bars.s_full[slot]);
+        };
+        auto sums = [&](int slot, int st, bool add) {
+          const uint32_t va = ring_a + st * kTileBytes<D>;
+#pragma unroll
+          for (int x = 0; x < 8; ++x)
+            rl::tc_mma_ts(tm + 256 + slot * D, tm + slot * 128 + x * 8, rl::sdesc_mnmajor_sw128(va + x * 2048, kHalf),
+                          kIdO, add || x > 0);
+          rl::tc_commit(&bars.pv_done[slot]);
+        };
+        int n0 = 0, seg = 0;      // blocks before this segment, segments
+        uint32_t pc[2] = {0, 0};  // p_full phases waited for
+        bool go = true;
+        do {
+          const int nb = sg.i1 - sg.i0;
+          go = rl::mbar_wait(&bars.q_full, seg & 1, abort, status);
+          rl::tc_fence_after();
+          if constexpr (kTwoTiles) {
+            for (int j = 0; go && j <= nb; ++j) {
+              const int kl = 2 * (n0 + j), vl = kl - 1;  // block j's keys, block j-1's values
+              if (j < nb) go = rl::mbar_wait(&bars.full[kl % S], (kl / S) & 1, abort, status);
+              if (go && j > 0) go = rl::mbar_wait(&bars.ok[vl % S], (vl / S) & 1, abort, status);
+              for (int slot = 0; go && slot < 2; ++slot) {
+                if (j > 0) {
+                  go = rl::mbar_wait(&bars.p_full[slot], pc[slot]++ & 1, abort, status);
+                  if (!go) break;
+                  rl::tc_fence_after();
+                  sums(slot, vl % S, j > 1);
+                }
+                if (j < nb) scores(slot, kl % S);
+              }
+              if (!go) break;
+              if (j < nb) rl::tc_commit(&bars.empty[kl % S]);
+              if (j > 0) rl::tc_commit(&bars.empty[vl % S]);
+            }
+          } else {
+            for (int j = 0; go && j < nb + 2; ++j) {
+              const int slot = j & 1;
+              if (j >= 2) {  // block j - 2
+                const int vl = 2 * (n0 + j - 2) + 1;
+                go = rl::mbar_wait(&bars.ok[vl % S], (vl / S) & 1, abort, status) &&
+                     rl::mbar_wait(&bars.p_full[slot], pc[slot]++ & 1, abort, status);
+                if (!go) break;
+                rl::tc_fence_after();
+                sums(slot, vl % S, j >= 4);
+                rl::tc_commit(&bars.empty[vl % S]);
+              }
+              if (j < nb) {
+                const int kl = 2 * (n0 + j);
+                go = rl::mbar_wait(&bars.full[kl % S], (kl / S) & 1, abort, status);
+                if (!go) break;
+                scores(slot, kl % S);
+                rl::tc_commit(&bars.empty[kl % S]);
+              }
+              if (nb == 1 && j == 0) ++j;  // slot 1 has no block
+            }
+          }
+          n0 += nb;
+          ++seg;
+        } while (go && sg.next(a, tiles));
+        rl::tc_commit(&bars.drain);  // nothing in flight when tensor memory is freed
+        drain_wait(&bars.drain, 0);
+      }
+      __syncwarp();
+    } else if (work && warp == 10) {
+      // ------------------------------------- values looked through
+      int n = 0, seg = 0;
+      bool go = true;
+      do {
+        for (int i = sg.i0; go && i < sg.i1; ++i, ++n) {
+          const int ld = 2 * n + 1, st = ld % S, j0 = sg.c.t.bl.index(i) * 128;
+          go = warp_wait(&bars.full[st], (ld / S) & 1, abort, status);
+          if (!go) break;
+          if (is_edge(a, sg.c.t.p0, sg.c.t.p1, j0, j0 + 127)) {
+            // A weight of 0 times a value that is not finite is not 0. Such
+            // values are zeroed; where some row does see their key, the
+            // group's end adds them to the rows that do.
+            uint8_t* v = ring + st * kTileBytes<D>;
+            bool any = false;
+            for (int x = lane; x < kTileBytes<D> / 16; x += 32) {
+              uint4* at16 = reinterpret_cast<uint4*>(v + x * 16);
+              uint4 w = *at16;
+              if (odd16(w.x) | odd16(w.y) | odd16(w.z) | odd16(w.w)) {
+                uint16_t* e = reinterpret_cast<uint16_t*>(&w);
+#pragma unroll
+                for (int y = 0; y < 8; ++y)
+                  if ((e[y] & 0x7f80u) == 0x7f80u) e[y] = 0;
+                *at16 = w;
+                any |= sees(sg.c.t.bl.all, a.sinks, j0 + (x % (kHalf / 16)) / 8);
+              }
+            }
+            if (__any_sync(0xffffffffu, any) && lane == 0) *(volatile int*)&poison[seg & 15] = 1;
+            rl::fence_proxy_async_smem();
+            __syncwarp();
+          }
+          if (lane == 0) rl::mbar_arrive(&bars.ok[st]);
+        }
+        // The weights' warps are at most 5 segments behind (a segment has a
+        // block or more, the ring holds 4 at most).
+        if (lane == 0) *(volatile int*)&poison[(seg + 8) & 15] = 0;
+        ++seg;
+      } while (go && sg.next(a, tiles));
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kWeightRegs));
+    if (work) {
+      // ---------------------------------------------- weights
+      Segments<Sh> sg;
+      sg.init(a, tiles, at, count);
+      const int slot = warp >> 2, wr = warp & 3;
+      const uint32_t lane_off = (uint32_t)(wr * 32) << 16;
+      const uint32_t ts = tm + slot * 128 + lane_off, to = tm + 256 + slot * D + lane_off;
+      const int r = (kTwoTiles ? slot * 128 : 0) + wr * 32 + lane;  // row of the tile
+      int seg = 0, n0 = 0;  // segments, blocks before this one
+      uint32_t sc = 0;      // blocks of this slot so far: phases of s_full and pv_done
+      bool go = true;
+      do {
+        const Tile& t = sg.c.t;
+        const int nb = sg.i1 - sg.i0;
+        // The query rows, 32 by this warp (16 with one tile), 16 bytes a lane.
+        {
+          constexpr int kRowsPerWarp = kTwoTiles ? 32 : 16, C = D / 8;
+          const int rb = warp * kRowsPerWarp;
+          uint8_t* tile = qs + (kTwoTiles ? slot * kTileBytes<D> : 0);
+#pragma unroll 4
+          for (int x = lane; x < kRowsPerWarp * C; x += 32) {
+            const int rr = rb + x / C, c = x % C, lr = rr & 127;
+            uint4 w = make_uint4(0, 0, 0, 0);
+            if (rr < t.rows) w = *reinterpret_cast<const uint4*>(a.q + head_of(a, t, sg.c.kh, rr) * D + c * 8);
+            *reinterpret_cast<uint4*>(tile + (c / 8) * kHalf + lr * 128 + (((c & 7) ^ (lr & 7)) * 16)) = w;
+          }
+          rl::fence_proxy_async_smem();
+          rl::mbar_arrive(&bars.q_full);
+        }
+        const bool in = r < t.rows;
+        const int base_tok = t.row0 / a.rep;
+        const Span sp = in ? a.span(t.p0 + (t.row0 + r) / a.rep - base_tok) : Span{0, -1};
+        // Positions of this warp's first and last row.
+        const int w0 = r - lane, w1 = min(w0 + 31, t.rows - 1);
+        const int64_t wp0 = t.p0 + (t.row0 + min(w0, t.rows - 1)) / a.rep - base_tok;
+        const int64_t wp1 = t.p0 + (t.row0 + w1) / a.rep - base_tok;
+        float m = -INFINITY, l = 0.f;  // maximum (of scaled scores) that the weights are relative to, and their sum
+        int done = 0;                  // blocks of this segment
+        for (int i = sg.i0 + (kTwoTiles ? 0 : slot); i < sg.i1; i += kTwoTiles ? 1 : 2) {
+          const int j0 = t.bl.index(i) * 128;
+          go = warp_wait(&bars.s_full[slot], sc & 1, abort, status);
+          if (!go) break;
+          rl::tc_fence_after();
+          uint32_t x[4][32];
+#pragma unroll
+          for (int y = 0; y < 4; ++y) rl::tmem_ld_32x32b_x32(ts + y * 32, x[y]);
+          rl::tmem_wait_ld();
+          if (is_edge(a, wp0, wp1, j0, j0 + 127) || w1 < w0) {
+#pragma unroll
+            for (int y = 0; y < 4; ++y)
+#pragma unroll
+              for (int e = 0; e < 32; ++e)
+                if (!sees(sp, a.sinks, j0 + y * 32 + e)) x[y][e] = 0xff800000u;
+          }
+          // Pages that are not held are loaded as zeros; their scores go.
+          const uint32_t bad = *(volatile uint32_t*)&gone[(n0 + i - sg.i0) & 7];
+          if (bad) {
+#pragma unroll
+            for (int y = 0; y < 4; ++y)
+#pragma unroll
+              for (int e = 0; e < 32; ++e)
+                if (bad >> ((y * 32 + e) >> a.pg.lg) & 1) x[y][e] = 0xff800000u;
+          }
+          float top[4];
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            top[y] = -INFINITY;
+#pragma unroll
+            for (int e = 0; e < 32; ++e) top[y] = fmaxf(top[y], __uint_as_float(x[y][e]));
+          }
+          const float mb = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * a.scale_log2;
+          if (done == 0) {
+            m = mb;
+          } else if (__any_sync(0xffffffffu, mb > m + 8.f)) {
+            // Weights may exceed 1 (by up to 2^8) before the sums so far are
+            // brought down to a new maximum: that rarely happens then.
+            const float mn = mb > m + 8.f ? mb : m;
+            const float f = m == mn ? 1.f : ex2(m - mn);
+            m = mn;
+            l *= f;
+            go = warp_wait(&bars.pv_done[slot], (sc - 1) & 1, abort, status);
+            if (!go) break;
+            rl::tc_fence_after();
+#pragma unroll
+            for (int y = 0; y < D / 32; ++y) {
+              uint32_t v[32];
+              rl::tmem_ld_32x32b_x32(to + y * 32, v);
+              rl::tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * f);
+              rl::tmem_st_32x32b_x32(to + y * 32, v);
+            }
+            rl::tmem_wait_st();
+          }
+          const float base = m == -INFINITY ? 0.f : m;
+          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            uint32_t p[32];
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+              const int f = y * 64 + 2 * e;
+              float e0, e1;
+              rl::fma_f32x2(e0, e1, __uint_as_float(x[f / 32][f % 32]), __uint_as_float(x[f / 32][f % 32 + 1]),
+                            a.scale_log2, a.scale_log2, -base, -base);
+              e0 = ex2(e0);
+              e1 = ex2(e1);
+              sum[e & 3] += e0 + e1;
+              p[e] = rl::pack_bf16x2(e0, e1);
+            }
+            rl::tmem_st_32x32b_x32(ts + y * 32, p);
+          }
+          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          rl::tmem_wait_st();
+          rl::tc_fence_before();
+          rl::mbar_arrive(&bars.p_full[slot]);
+          ++sc;
+          ++done;
+        }
+        if (!go) break;
+        // The group ends, or this CTA's share of it.
+        if (done) {
+          go = warp_wait(&bars.pv_done[slot], (sc - 1) & 1, abort, status);
+          if (!go) break;
+          rl::tc_fence_after();
+        }
+        const bool whole = sg.i0 == 0 && sg.i1 == t.bl.n;
+        const bool odd = *(volatile int*)&poison[seg & 15] != 0;
+        float* part = ws + (2 * (int64_t)blockIdx.x + (seg == 0 ? 0 : 1)) * kSlotFloats<Sh, D>;
+        float mine = 1.f, other = 0.f;  // factors of the slots' sums
+        if constexpr (!kTwoTiles) {
+          if (slot == 1) {
+            ml[0][r] = m;
+            ml[1][r] = l;
+          }
+        }
+#pragma unroll 1
+        for (int y = 0; go && y < D / 32; ++y) {
+          uint32_t v[32];
+          if (done) {
+            rl::tmem_ld_32x32b_x32(to + y * 32, v);
+            rl::tmem_wait_ld();
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) v[e] = 0;
+          }
+          if constexpr (!kTwoTiles) {
+            // D / 2 columns at a time through shared memory, slot 1 to slot 0.
+            constexpr int kTurn = D / 64;  // 32-column pieces in a turn
+            const uint32_t turn = (seg * 2 + y / kTurn) & 1;
+            float* mc = merge + (y % kTurn) * 32 * 128 + r;
+            if (slot == 1) {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) mc[e * 128] = __uint_as_float(v[e]);
+              if (y % kTurn == kTurn - 1) {
+                rl::mbar_arrive(&bars.merge_full);
+                go = warp_wait(&bars.merge_empty, turn, abort, status);
+              }
+              continue;
+            }
+            if (y % kTurn == 0) go = warp_wait(&bars.merge_full, turn, abort, status);
+            if (!go) break;
+            if (y == 0) {
+              const float m1 = ml[0][r], M = fmaxf(m, m1), base = M == -INFINITY ? 0.f : M;
+              mine = ex2(m - base);
+              other = ex2(m1 - base);
+              l = l * mine + ml[1][r] * other;
+              m = M;
+            }
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              v[e] = __float_as_uint(fmaf(__uint_as_float(v[e]), mine, mc[e * 128] * other));
+            if (y % kTurn == kTurn - 1) rl::mbar_arrive(&bars.merge_empty);
+          }
+          if (y == 0 && !whole && in) {
+            part[r] = m;
+            part[Sh::R + r] = l;
+          }
+          if (!in) continue;
+          if (odd) {
+            for (int i = sg.i0; i < sg.i1; ++i) {
+              const int j0 = t.bl.index(i) * 128;
+              if (!is_edge(a, t.p0, t.p1, j0, j0 + 127)) continue;
+              for (int j = j0; j < j0 + 128; ++j) {
+                const int64_t row = sees(sp, a.sinks, j) ? a.pg.row(t.b, sg.c.kh, j) : -1;
+                if (row < 0) continue;
+#pragma unroll
+                for (int e = 0; e < 32; ++e) {
+                  const float f = bf2f(a.v[row * D + y * 32 + e]);
+                  if (!isfinite(f)) v[e] = __float_as_uint(__uint_as_float(v[e]) + f);
+                }
+              }
+            }
+          }
+          if (whole) {
+            const float inv = l == 0.f ? 0.f : __fdiv_rn(1.f, l);
+            uint16_t* o = a.out + head_of(a, t, sg.c.kh, r) * D + y * 32;
+#pragma unroll
+            for (int e = 0; e < 32; e += 8) {
+              uint4 w;
+              w.x = rl::pack_bf16x2(__uint_as_float(v[e]) * inv, __uint_as_float(v[e + 1]) * inv);
+              w.y = rl::pack_bf16x2(__uint_as_float(v[e + 2]) * inv, __uint_as_float(v[e + 3]) * inv);
+              w.z = rl::pack_bf16x2(__uint_as_float(v[e + 4]) * inv, __uint_as_float(v[e + 5]) * inv);
+              w.w = rl::pack_bf16x2(__uint_as_float(v[e + 6]) * inv, __uint_as_float(v[e + 7]) * inv);
+              *reinterpret_cast<uint4*>(o + e) = w;
+            }
+          } else {
+            float* o = part + 2 * Sh::R + r * D + y * 32;
+#pragma unroll
+            for (int e = 0; e < 32; e += 4)
+              *reinterpret_cast<uint4*>(o + e) = make_uint4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+          }
+        }
+        if (!go) break;
+        rl::tc_fence_before();  // the next group's first product overwrites O
+        n0 += nb;
+        ++seg;
+      } while (sg.next(a, tiles));
+    }
+  }
+  rl::tc_fence_before();
+  __syncthreads();
+  rl::tc_fence_after();
+  if (warp == 9) rl::tmem_dealloc(tm, 512);
+}
+
 // CTA c adds up the partial results of the group that the boundary between
 // the shares c and c + 1 cuts, if c is the first that holds part of it; 16
 // rows per CTA. Threads (dimension, row); the weights of the parts are worked
@@ -654,37 +1169,72 @@ __global__ void __launch_bounds__(D * 4) join_kernel(const AttnArgs a, int tiles
   }
 }
 
-// The launch of a call with few rows: row tiles of 16, CTAs, and whether a
-// group can be cut at all.
-struct FewPlan {
-  int tiles, G;
+// The kernel for a call, its row tiles and CTAs, and whether a group can be
+// cut at all.
+struct Plan {
+  enum { kFew, kOneTile, kTwoTile } kind;
+  int tiles, G, R;
   bool join;
   uint64_t ws_bytes;
 };
-FewPlan few_plan(int num_sms, int B, int T, int nh, int nkv, int d, int64_t cap) {
-  FewPlan p;
+Plan make_plan(int num_sms, int B, int T, int nh, int nkv, int d, int64_t cap) {
+  Plan p;
   const int64_t rows = (int64_t)T * (nh / nkv);
-  p.tiles = (int)((rows + 15) / 16);
-  const int64_t blocks = (cap + Few::kBlock - 1) / Few::kBlock;
+  p.kind = rows <= 16 ? Plan::kFew : rows <= 128 ? Plan::kOneTile : Plan::kTwoTile;
+  p.R = p.kind == Plan::kFew ? Few::R : p.kind == Plan::kOneTile ? 128 : 256;
+  const int block = p.kind == Plan::kFew ? Few::kBlock : 128;
+  p.tiles = (int)((rows + p.R - 1) / p.R);
+  const int64_t blocks = (cap + block - 1) / block;
   const int64_t most = (int64_t)B * nkv * p.tiles * blocks;
-  p.G = (int)std::min<int64_t>(std::min(2 * num_sms, kMaxShares), most);
+  p.G = (int)std::min<int64_t>(std::min((p.kind == Plan::kFew ? 2 : 1) * num_sms, kMaxShares), most);
   p.join = blocks > 1 && p.G > 1;
-  p.ws_bytes = p.join ? (uint64_t)2 * p.G * 16 * (d + 2) * sizeof(float) : 0;
+  p.ws_bytes = p.join ? (uint64_t)2 * p.G * p.R * (d + 2) * sizeof(float) : 0;
   return p;
 }
 
+template <typename Sh, int D>
+int32_t launch_join(riallm_ctx* ctx, const AttnArgs& a, const Plan& p, const float* ws, cudaStream_t st) {
+  if (!p.join) return RIALLM_OK;
+  return rl::launched(ctx, "paged_attention",
+                      rl::launch_pdl(join_kernel<Sh, D>, dim3(p.G - 1, Sh::R / 16), dim3(D * 4), 0, st, a, p.tiles,
+                                     p.G, ws));
+}
+
 template <int D>
-int32_t launch_few(riallm_ctx* ctx, const AttnArgs& a, const FewPlan& p, float* ws, cudaStream_t st) {
+int32_t launch_few(riallm_ctx* ctx, const AttnArgs& a, const Plan& p, float* ws, cudaStream_t st) {
   const char* what = "paged_attention";
   if (int s = rl::allow_smem(ctx, what, few_rows_kernel<D>, kFewSmem<D>, D / 64 - 1)) return s;
   if (int s = rl::launched(ctx, what,
                            rl::launch_pdl(few_rows_kernel<D>, dim3(p.G), dim3(kFewWarps * 32), kFewSmem<D>, st, a,
                                           p.tiles, ws)))
     return s;
-  if (!p.join) return RIALLM_OK;
-  return rl::launched(ctx, what,
-                      rl::launch_pdl(join_kernel<Few, D>, dim3(p.G - 1), dim3(D * 4), 0, st, a, p.tiles, p.G,
-                                     static_cast<const float*>(ws)));
+  return launch_join<Few, D>(ctx, a, p, ws, st);
+}
+
+template <int D, bool kTwoTiles>
+int32_t launch_many(riallm_ctx* ctx, const AttnArgs& a, const Plan& p, float* ws, cudaStream_t st) {
+  const char* what = "paged_attention";
+  const auto kernel = many_rows_kernel<D, kTwoTiles>;
+  if (int s = rl::allow_smem(ctx, what, kernel, kManySmem<D>, 2 + (D / 64 - 1) * 2 + kTwoTiles)) return s;
+  CUtensorMap map[2];
+  for (int i = 0; i < 2; ++i) {
+    const CUresult r = rl::encode_tensor_map_2d(&map[i], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, i ? a.v : a.k, D,
+                                                (uint64_t)a.pg.num_pages * a.pg.nkv << a.pg.lg, D * 2, 64,
+                                                1u << a.pg.lg, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (r != CUDA_SUCCESS) return rl::refuse(ctx, RIALLM_ERR_CUDA, what, "cuTensorMapEncodeTiled");
+  }
+  if (int s = rl::launched(ctx, what,
+                           rl::launch_pdl(kernel, dim3(p.G), dim3(kManyThreads), kManySmem<D>, st, a, map[0], map[1],
+                                          p.tiles, ws, ctx->d_status)))
+    return s;
+  return launch_join<Many<kTwoTiles>, D>(ctx, a, p, ws, st);
+}
+
+template <int D>
+int32_t launch_attention(riallm_ctx* ctx, const AttnArgs& a, const Plan& p, float* ws, cudaStream_t st) {
+  return p.kind == Plan::kFew       ? launch_few<D>(ctx, a, p, ws, st)
+         : p.kind == Plan::kOneTile ? launch_many<D, false>(ctx, a, p, ws, st)
+                                    : launch_many<D, true>(ctx, a, p, ws, st);
 }
 
 bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -748,7 +1298,7 @@ int32_t riallm_cuda_rope_paged_append(riallm_ctx* ctx, const void* qkv, const in
 uint64_t riallm_cuda_paged_attention_workspace(const riallm_ctx* ctx, int32_t B, int32_t T, int32_t nh, int32_t nkv,
                                                int32_t d, int32_t max_pages, int32_t page_size) {
   if (!ctx || B <= 0 || T <= 0 || nkv <= 0 || nh < nkv || max_pages <= 0 || page_size <= 0) return 0;
-  return few_plan(ctx->num_sms, B, T, nh, nkv, d, (int64_t)max_pages * page_size).ws_bytes;
+  return make_plan(ctx->num_sms, B, T, nh, nkv, d, (int64_t)max_pages * page_size).ws_bytes;
 }
 
 int32_t riallm_cuda_paged_attention(riallm_ctx* ctx, const void* q, const void* k_pages, const void* v_pages,
@@ -765,7 +1315,7 @@ int32_t riallm_cuda_paged_attention(riallm_ctx* ctx, const void* q, const void* 
     return rl::refuse(ctx, RIALLM_ERR_INVALID, what, "NULL argument");
   if (!al16(q) || !al16(out) || !al16(k_pages) || !al16(v_pages))
     return rl::refuse(ctx, RIALLM_ERR_INVALID, what, "buffers must be 16-byte aligned");
-  const FewPlan p = few_plan(ctx->num_sms, B, T, nh, nkv, d, (int64_t)max_pages * page_size);
+  const Plan p = make_plan(ctx->num_sms, B, T, nh, nkv, d, (int64_t)max_pages * page_size);
   if (p.ws_bytes && (!workspace || workspace_bytes < p.ws_bytes || (reinterpret_cast<uintptr_t>(workspace) & 255)))
     return rl::refuse(ctx, RIALLM_ERR_MEMORY, what, "workspace missing, too small or not 256-byte aligned");
   return rl::guarded(ctx, [&]() -> int32_t {
@@ -781,7 +1331,7 @@ int32_t riallm_cuda_paged_attention(riallm_ctx* ctx, const void* q, const void* 
     a.out = static_cast<uint16_t*>(out);
     float* ws = static_cast<float*>(workspace);
     cudaStream_t st = (cudaStream_t)stream;
-    return d == 128 ? launch_few<128>(ctx, a, p, ws, st) : launch_few<64>(ctx, a, p, ws, st);
+    return d == 128 ? launch_attention<128>(ctx, a, p, ws, st) : launch_attention<64>(ctx, a, p, ws, st);
   });
 }
 
