@@ -140,15 +140,17 @@ __device__ __forceinline__ Blocks blocks_of(const AttnArgs& a, int64_t first, in
 }
 
 // The work of a call: the rows of every sequence in tiles of R; a group is
-// one (sequence, tile, kv head), a unit one of its blocks of kBlock keys.
-// Units are ordered by sequence, tile, kv head, block, and cut into as many
-// equal contiguous shares as there are CTAs, whatever the sequences' lengths
-// and the tiles' place under the causal diagonal; a group that a share
-// boundary cuts leaves partial results, which join_kernel adds up. The
-// lengths are the device's, so a captured call follows them.
-template <int R_, int kBlock_>
+// one (sequence, tile, kv head). Groups are laid out in that order along a
+// line, each as kCost units of fixed cost and then a unit for each of its
+// blocks of kBlock keys, and the line is cut into as many equal shares as
+// there are CTAs, whatever the sequences' lengths and the tiles' place under
+// the causal diagonal. A block belongs to the share that its unit lies in; a
+// group with blocks in several shares leaves partial results, which
+// join_kernel adds up. The lengths are the device's, so a captured call
+// follows them.
+template <int R_, int kBlock_, int kCost_>
 struct Shape {
-  static constexpr int R = R_, kBlock = kBlock_;
+  static constexpr int R = R_, kBlock = kBlock_, kCost = kCost_;
 };
 struct Tile {
   int b, row0, rows;    // sequence; first row and rows, of its T * rep
@@ -177,8 +179,8 @@ __device__ __forceinline__ int64_t head_of(const AttnArgs& a, const Tile& t, int
 __device__ __forceinline__ int64_t share_begin(int64_t W, int G, int c) { return W * c / G; }
 __device__ __forceinline__ int share_of(int64_t W, int G, int64_t u) { return (int)(((u + 1) * G - 1) / W); }
 
-// Finds where the first unit of share c (of the call's G shares, fewer where
-// there are fewer units) lies: every thread of a block of N threads sums the
+// Finds the tile that the first unit of share c (of the call's G shares, fewer
+// where there are fewer units) lies in: every thread of a block of N threads sums the
 // units of its slab of tiles, and the thread whose slab holds the unit walks
 // it.
 struct UnitAt {
@@ -196,7 +198,7 @@ __device__ __forceinline__ UnitAt find_unit(const AttnArgs& a, int tiles, int G,
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int all = a.B * tiles, per = (all + N - 1) / N;
   const int x0 = min(all, (int)threadIdx.x * per), x1 = min(all, x0 + per);
-  auto units = [&](int x) { return (int64_t)tile_of<Sh>(a, tiles, x).bl.n * a.pg.nkv; };
+  auto units = [&](int x) { return (int64_t)(tile_of<Sh>(a, tiles, x).bl.n + Sh::kCost) * a.pg.nkv; };
   int64_t mine = 0;
   for (int x = x0; x < x1; ++x) mine += units(x);
   int64_t upto = mine;  // inclusive scan
@@ -236,22 +238,33 @@ __device__ __forceinline__ UnitAt find_unit(const AttnArgs& a, int tiles, int G,
   return at;
 }
 
-// Walks the units from a place on.
+// Walks the blocks of share c from its first on.
 template <typename Sh>
 struct Cursor {
   int x, kh, i;
+  int64_t at0, end;  // unit of the group's block 0; end of the share
   Tile t;
-  __device__ __forceinline__ void init(const AttnArgs& a, int tiles, const UnitAt& at) {
+  __device__ __forceinline__ void init(const AttnArgs& a, int tiles, const UnitAt& at, int c) {
     x = at.x;
     t = tile_of<Sh>(a, tiles, x);
-    kh = (int)((at.u - at.start) / t.bl.n);
-    i = (int)((at.u - at.start) - (int64_t)kh * t.bl.n);
+    const int size = t.bl.n + Sh::kCost;
+    kh = (int)((at.u - at.start) / size);
+    at0 = at.start + (int64_t)kh * size + Sh::kCost;
+    i = (int)max((int64_t)0, at.u - at0);
+    end = share_begin(at.W, at.G, c + 1);
   }
+  __device__ __forceinline__ bool valid() const { return at0 + i < end; }
+  // Block i is the last of its group, or of the share.
+  __device__ __forceinline__ bool last() const { return i + 1 == t.bl.n || at0 + i + 1 >= end; }
   __device__ __forceinline__ void next_group(const AttnArgs& a, int tiles) {
     i = 0;
+    at0 += t.bl.n + Sh::kCost;
     if (++kh < a.pg.nkv) return;
     kh = 0;
     if (++x < a.B * tiles) t = tile_of<Sh>(a, tiles, x);
+  }
+  __device__ __forceinline__ void next(const AttnArgs& a, int tiles) {
+    if (++i == t.bl.n) next_group(a, tiles);
   }
 };
 
@@ -291,9 +304,9 @@ __device__ __forceinline__ void cp_async_16z(void* dst, const void* src, int byt
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(rl::smem_u32(dst)), "l"(src), "r"(bytes)
                : "memory");
 }
-__device__ __forceinline__ bool odd16(uint32_t x) {  // either bf16 of x is infinite or NaN
-  return (x & 0x7f80u) == 0x7f80u || (x & 0x7f800000u) == 0x7f800000u;
-}
+// Not 0 where either bf16 of x is infinite or NaN: an exponent of all ones
+// carries into the sign's place.
+__device__ __forceinline__ uint32_t odd16(uint32_t x) { return ((x & 0x7f807f80u) + 0x00800080u) & 0x80008000u; }
 
 // ---------------------------------------------------------------- few rows
 //
@@ -309,7 +322,7 @@ __device__ __forceinline__ bool odd16(uint32_t x) {  // either bf16 of x is infi
 // nothing is gained by a 128-row tcgen05 tile of which 4 to 16 rows are
 // used.
 constexpr int kFewWarps = 4;
-using Few = Shape<16, 64>;
+using Few = Shape<16, 64, 1>;
 
 template <int D>
 constexpr int kFewStages = D == 128 ? 3 : 6;
@@ -327,9 +340,8 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const UnitAt at = find_unit<Few, kFewWarps * 32>(a, tiles, gridDim.x, blockIdx.x);
   if (at.u >= at.W) return;
-  const int count = (int)(share_begin(at.W, at.G, blockIdx.x + 1) - at.u);
   Cursor<Few> now;
-  now.init(a, tiles, at);
+  now.init(a, tiles, at, blockIdx.x);
   Cursor<Few> ahead = now;
 
   uint16_t* ring = smem + warp * (S * 2 * 16 * D);
@@ -343,7 +355,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
   auto key0 = [&](const Cursor<Few>& c) { return c.t.bl.index(c.i) * Few::kBlock + warp * 16; };
   auto fetch_page = [&]() {  // the page of the unit that is loaded next
     page = -1;
-    if (issued < count) {
+    if (ahead.valid()) {
       const int j = key0(ahead);
       const Span all = ahead.t.bl.all;
       const bool any = j <= all.hi && (j + 15 >= all.lo || j < a.sinks);
@@ -351,7 +363,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
     }
   };
   auto issue = [&]() {
-    if (issued < count) {
+    if (ahead.valid()) {
       if (issued == 0 || ahead.i == 0) {
         uint16_t* to = queries + (begun % S) * 16 * D;
 #pragma unroll
@@ -381,7 +393,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
         }
       }
       ++issued;
-      if (issued < count && ++ahead.i == ahead.t.bl.n) ahead.next_group(a, tiles);
+      ahead.next(a, tiles);
       fetch_page();
     }
     rl::cp_async_commit();
@@ -394,7 +406,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
   float o[D / 8][4], m[2], l[2];
   Span sp[2];
   int first = 0, group = 0;
-  for (int n = 0; n < count; ++n) {
+  for (int n = 0; now.valid(); ++n) {
     rl::cp_async_wait<S - 2>();
     if (n == 0 || now.i == 0) {  // a group begins
       __syncthreads();           // every warp's quarter of its query rows has arrived
@@ -482,7 +494,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
 #pragma unroll
         for (int x = 0; x < 16 * C / 32; ++x) {
           const uint4 w = *reinterpret_cast<const uint4*>(vs + (x * 32 + lane) * 8);
-          odd |= odd16(w.x) | odd16(w.y) | odd16(w.z) | odd16(w.w);
+          odd |= (odd16(w.x) | odd16(w.y) | odd16(w.z) | odd16(w.w)) != 0;
         }
         if (__any_sync(0xffffffffu, odd)) {
           for (int key = 0; key < 16; ++key)
@@ -532,8 +544,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
     __syncwarp();
     issue();  // into the stage that was read before this one
 
-    const bool whole_end = now.i + 1 == now.t.bl.n;
-    if (whole_end || n + 1 == count) {
+    if (now.last()) {
       // The group ends, or this CTA's share of it. Each warp leaves its
       // result in the stage it has just read (2 * 16 * D bf16 hold 16 * D
       // floats), columns swizzled by the row; then all add up the four.
@@ -552,7 +563,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
               make_float2(o[x][2 * h], o[x][2 * h + 1]);
       }
       __syncthreads();
-      const bool whole = whole_end && now.i == n - first;
+      const bool whole = now.i + 1 == now.t.bl.n && now.i == n - first;
       float* slot = ws + (2 * (int64_t)blockIdx.x + (first == 0 ? 0 : 1)) * kSlotFloats<Few, D>;
       const float* part = reinterpret_cast<const float*>(smem) + (n % S) * (16 * D);
       for (int x = threadIdx.x; x < now.t.rows * (D / 4); x += kFewWarps * 32) {
@@ -587,7 +598,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
       }
       __syncthreads();  // before the stages, sm_m and sm_l are written again
     }
-    if (n + 1 < count && ++now.i == now.t.bl.n) now.next_group(a, tiles);
+    now.next(a, tiles);
   }
 }
 
@@ -606,16 +617,16 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
 //   !kTwoTiles : up to 128 rows a tile, the slots take the blocks in turn
 //                and are added up at the group's end.
 // Roles: warps 0-3 and 4-7 the two slots' weights (a thread a row), warp 8
-// loads blocks by TMA, page by page, warp 9 issues the products, warp 10
-// looks through the values of blocks that some row of the tile does not see
-// whole, warp 11 has none. Keys and values share a ring of kStages blocks in smem.
+// loads blocks by TMA, page by page, warp 9 issues the products, warps
+// 10 and 11 look through the values of blocks that some row of the tile does
+// not see whole. Keys and values share a ring of kStages blocks in smem.
 constexpr int kManyThreads = 12 * 32;
 // Registers: the launch's 168 a thread, of which the third warpgroup (loads,
 // products) keeps 88 and the weights' two take 208 (2 * 208 + 88 = 3 * 168).
 constexpr int kWeightRegs = 208, kOtherRegs = 88;
 constexpr int kMaxStages = 8;
 template <bool kTwoTiles>
-using Many = Shape<kTwoTiles ? 256 : 128, 128>;
+using Many = Shape<kTwoTiles ? 256 : 128, 128, 4>;
 template <int D>
 constexpr int kManyStages = D == 128 ? 4 : 8;
 template <int D>
@@ -644,21 +655,20 @@ __device__ __forceinline__ void drain_wait(uint64_t* bar, uint32_t parity) {
 template <typename Sh>
 struct Segments {
   Cursor<Sh> c;
-  int64_t left;
   int i0, i1;
-  __device__ __forceinline__ void init(const AttnArgs& a, int tiles, const UnitAt& at, int64_t count) {
-    c.init(a, tiles, at);
-    left = count;
+  __device__ __forceinline__ bool take() {
     i0 = c.i;
-    i1 = (int)min((int64_t)c.t.bl.n, i0 + left);
+    i1 = (int)min((int64_t)c.t.bl.n, c.end - c.at0);
+    return c.valid();
+  }
+  // False where the share holds no block.
+  __device__ __forceinline__ bool init(const AttnArgs& a, int tiles, const UnitAt& at, int share) {
+    c.init(a, tiles, at, share);
+    return take();
   }
   __device__ __forceinline__ bool next(const AttnArgs& a, int tiles) {
-    left -= i1 - i0;
-    if (left <= 0) return false;
     c.next_group(a, tiles);
-    i0 = 0;
-    i1 = (int)min((int64_t)c.t.bl.n, left);
-    return true;
+    return take();
   }
 };
 
@@ -686,7 +696,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     for (int i = 0; i < kMaxStages; ++i) {
       rl::mbar_init(&bars.full[i], 1);
       rl::mbar_init(&bars.empty[i], 1);
-      rl::mbar_init(&bars.ok[i], 1);
+      rl::mbar_init(&bars.ok[i], 2);
     }
     rl::mbar_init(&bars.q_full, 256);
     for (int i = 0; i < 2; ++i) {
@@ -713,12 +723,10 @@ __global__ void __launch_bounds__(kManyThreads, 1)
   const uint32_t tm = tmem_base;
 
   const UnitAt at = find_unit<Sh, kManyThreads>(a, tiles, gridDim.x, blockIdx.x);
-  const bool work = at.u < at.W;
-  const int64_t count = work ? share_begin(at.W, at.G, blockIdx.x + 1) - at.u : 0;
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
     Segments<Sh> sg;
-    if (work) sg.init(a, tiles, at, count);
+    const bool work = at.u < at.W && sg.init(a, tiles, at, blockIdx.x);
     if (work && warp == 8) {
       // ------------------------------------------------ loads
       const int per_page = 1 << a.pg.lg, pages = 128 >> a.pg.lg;
@@ -839,7 +847,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         drain_wait(&bars.drain, 0);
       }
       __syncwarp();
-    } else if (work && warp == 10) {
+    } else if (work) {
       // ------------------------------------- values looked through
       int n = 0, seg = 0;
       bool go = true;
@@ -852,38 +860,44 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             // A weight of 0 times a value that is not finite is not 0. Such
             // values are zeroed; where some row does see their key, the
             // group's end adds them to the rows that do.
-            uint8_t* v = ring + st * kTileBytes<D>;
+            uint4* v = reinterpret_cast<uint4*>(ring + st * kTileBytes<D>);
             bool any = false;
-            for (int x = lane; x < kTileBytes<D> / 16; x += 32) {
-              uint4* at16 = reinterpret_cast<uint4*>(v + x * 16);
-              uint4 w = *at16;
-              if (odd16(w.x) | odd16(w.y) | odd16(w.z) | odd16(w.w)) {
-                uint16_t* e = reinterpret_cast<uint16_t*>(&w);
+#pragma unroll 1
+            for (int x = (warp - 10) * 32 + lane; x < kTileBytes<D> / 16; x += 8 * 64) {
+              uint4 w[8];
+              uint32_t odd[8];
 #pragma unroll
-                for (int y = 0; y < 8; ++y)
-                  if ((e[y] & 0x7f80u) == 0x7f80u) e[y] = 0;
-                *at16 = w;
-                any |= sees(sg.c.t.bl.all, a.sinks, j0 + (x % (kHalf / 16)) / 8);
+              for (int y = 0; y < 8; ++y) w[y] = v[x + y * 64];
+              uint32_t all = 0;
+#pragma unroll
+              for (int y = 0; y < 8; ++y) all |= odd[y] = odd16(w[y].x) | odd16(w[y].y) | odd16(w[y].z) | odd16(w[y].w);
+              if (!all) continue;
+#pragma unroll
+              for (int y = 0; y < 8; ++y) {
+                if (!odd[y]) continue;
+                uint16_t* e = reinterpret_cast<uint16_t*>(&v[x + y * 64]);
+                for (int z = 0; z < 8; ++z)
+                  if ((e[z] & 0x7f80u) == 0x7f80u) e[z] = 0;
+                any |= sees(sg.c.t.bl.all, a.sinks, j0 + ((x + y * 64) % (kHalf / 16)) / 8);
               }
             }
             if (__any_sync(0xffffffffu, any) && lane == 0) *(volatile int*)&poison[seg & 15] = 1;
             rl::fence_proxy_async_smem();
             __syncwarp();
           }
-          if (lane == 0) rl::mbar_arrive(&bars.ok[st]);
+          if (lane == 0) rl::mbar_arrive(&bars.ok[st]);  // each of the two warps
         }
         // The weights' warps are at most 5 segments behind (a segment has a
         // block or more, the ring holds 4 at most).
-        if (lane == 0) *(volatile int*)&poison[(seg + 8) & 15] = 0;
+        if (warp == 10 && lane == 0) *(volatile int*)&poison[(seg + 8) & 15] = 0;
         ++seg;
       } while (go && sg.next(a, tiles));
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kWeightRegs));
-    if (work) {
+    Segments<Sh> sg;
+    if (at.u < at.W && sg.init(a, tiles, at, blockIdx.x)) {
       // ---------------------------------------------- weights
-      Segments<Sh> sg;
-      sg.init(a, tiles, at, count);
       const int slot = warp >> 2, wr = warp & 3;
       const uint32_t lane_off = (uint32_t)(wr * 32) << 16;
       const uint32_t ts = tm + slot * 128 + lane_off, to = tm + 256 + slot * D + lane_off;
@@ -1106,66 +1120,71 @@ __global__ void __launch_bounds__(kManyThreads, 1)
   if (warp == 9) rl::tmem_dealloc(tm, 512);
 }
 
-// CTA c adds up the partial results of the group that the boundary between
-// the shares c and c + 1 cuts, if c is the first that holds part of it; 16
-// rows per CTA. Threads (dimension, row); the weights of the parts are worked
-// out once a row, a part a thread.
-constexpr int kMaxShares = 512;
+// CTA (c, y) adds up rows 16 y .. 16 y + 15 of the partial results of the
+// group that the boundary between the shares c and c + 1 cuts, if c is the
+// first that holds part of it.
+constexpr int kMaxShares = 512, kJoinThreads = 256;
 template <typename Sh, int D>
-__global__ void __launch_bounds__(D * 4) join_kernel(const AttnArgs a, int tiles, int G, const float* __restrict__ ws) {
-  constexpr int kSlot = kSlotFloats<Sh, D>, kW = D / 32;
-  __shared__ float weight[4][kMaxShares], red[2][4][kW];
+__global__ void __launch_bounds__(kJoinThreads)
+    join_kernel(const AttnArgs a, int tiles, int G, const float* __restrict__ ws) {
+  constexpr int kSlot = kSlotFloats<Sh, D>;
+  __shared__ float weight[16][kMaxShares];  // of the parts
   rl::pdl_wait();
   rl::pdl_launch_dependents();
   const int c0 = blockIdx.x;
-  const UnitAt at = find_unit<Sh, D * 4>(a, tiles, G, c0 + 1);
+  const UnitAt at = find_unit<Sh, kJoinThreads>(a, tiles, G, c0 + 1);
   if (at.u >= at.W) return;
   Cursor<Sh> cut;
-  cut.init(a, tiles, at);
-  const int64_t g0 = at.u - cut.i, g1 = g0 + cut.t.bl.n;
-  if (cut.i == 0 || share_of(at.W, at.G, g0) != c0) return;  // not cut here, or cut before as well
-  const int parts = share_of(at.W, at.G, g1 - 1) - c0 + 1;
-  // The first part is in its CTA's second slot where the group began inside
-  // that CTA's share.
-  const float* first = ws + (2 * (int64_t)c0 + (share_begin(at.W, at.G, c0) < g0 ? 1 : 0)) * kSlot;
+  cut.init(a, tiles, at, c0 + 1);
+  const int64_t last = cut.at0 + cut.t.bl.n - 1;
+  if (cut.i == 0 || share_of(at.W, at.G, cut.at0) != c0) return;  // not cut here, or cut before as well
+  const int row0 = blockIdx.y * 16, rows = min(16, cut.t.rows - row0);
+  if (rows <= 0) return;
+  const int parts = share_of(at.W, at.G, last) - c0 + 1;
+  // The first part is in its CTA's second slot where that share begins with
+  // another group.
+  const float* first =
+      ws + (2 * (int64_t)c0 + (share_begin(at.W, at.G, c0) < cut.at0 - Sh::kCost ? 1 : 0)) * kSlot;
   const float* rest = ws + 2 * (int64_t)c0 * kSlot;
-  const int rows = min(cut.t.rows, (int)(blockIdx.y + 1) * 16);
-  const int d = threadIdx.x % D, rs = threadIdx.x / D, lane = d & 31, w = d >> 5;
-  for (int r0 = blockIdx.y * 16; r0 < rows; r0 += 4) {
-    const int r = r0 + rs;
-    const bool in = r < rows;
+  const int lane = threadIdx.x & 31;
+  for (int r = threadIdx.x >> 5; r < rows; r += kJoinThreads / 32) {
     float M = -INFINITY;
-    if (in)
-      for (int i = d; i < parts; i += D) M = fmaxf(M, __ldcg((i ? rest + (int64_t)i * 2 * kSlot : first) + r));
+    for (int i = lane; i < parts; i += 32) {
+      const float x = __ldcg((i ? rest + (int64_t)i * 2 * kSlot : first) + row0 + r);
+      weight[r][i] = x;
+      M = fmaxf(M, x);
+    }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-    if (lane == 0) red[0][rs][w] = M;
-    __syncthreads();
-#pragma unroll
-    for (int x = 0; x < kW; ++x) M = fmaxf(M, red[0][rs][x]);
     float den = 0.f;
-    if (in)
-      for (int i = d; i < parts; i += D) {
-        const float* s = i ? rest + (int64_t)i * 2 * kSlot : first;
-        const float f = M == -INFINITY ? 0.f : ex2(__ldcg(s + r) - M);
-        weight[rs][i] = f;
-        den = fmaf(f, __ldcg(s + Sh::R + r), den);
-      }
+    for (int i = lane; i < parts; i += 32) {
+      const float f = M == -INFINITY ? 0.f : ex2(weight[r][i] - M);
+      weight[r][i] = f;
+      den = fmaf(f, __ldcg((i ? rest + (int64_t)i * 2 * kSlot : first) + Sh::R + row0 + r), den);
+    }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) den += __shfl_xor_sync(0xffffffffu, den, o);
-    if (lane == 0) red[1][rs][w] = den;
-    __syncthreads();
-    den = 0.f;
-#pragma unroll
-    for (int x = 0; x < kW; ++x) den += red[1][rs][x];
-    if (in) {
-      const int64_t at_d = 2 * Sh::R + r * D + d;
-      float num = weight[rs][0] * __ldcg(first + at_d);
+    const float inv = den == 0.f ? 0.f : __fdiv_rn(1.f, den);
+    for (int i = lane; i < parts; i += 32) weight[r][i] *= inv;
+  }
+  __syncthreads();
+  for (int x = threadIdx.x; x < rows * (D / 4); x += kJoinThreads) {
+    const int r = x / (D / 4), c = (x - r * (D / 4)) * 4;
+    const int64_t off = 2 * Sh::R + (row0 + r) * D + c;
+    float4 y = __ldcg(reinterpret_cast<const float4*>(first + off));
+    const float w0 = weight[r][0];
+    y.x *= w0, y.y *= w0, y.z *= w0, y.w *= w0;
 #pragma unroll 8
-      for (int i = 1; i < parts; ++i) num = fmaf(weight[rs][i], __ldcg(rest + (int64_t)i * 2 * kSlot + at_d), num);
-      a.out[head_of(a, cut.t, cut.kh, r) * D + d] = f2bf(den == 0.f ? 0.f : num / den);
+    for (int i = 1; i < parts; ++i) {
+      const float w = weight[r][i];
+      const float4 z = __ldcg(reinterpret_cast<const float4*>(rest + (int64_t)i * 2 * kSlot + off));
+      y.x = fmaf(w, z.x, y.x);
+      y.y = fmaf(w, z.y, y.y);
+      y.z = fmaf(w, z.z, y.z);
+      y.w = fmaf(w, z.w, y.w);
     }
-    __syncthreads();  // weight and red are written again
+    *reinterpret_cast<uint2*>(a.out + head_of(a, cut.t, cut.kh, row0 + r) * D + c) =
+        make_uint2(rl::pack_bf16x2(y.x, y.y), rl::pack_bf16x2(y.z, y.w));
   }
 }
 
@@ -1196,7 +1215,7 @@ template <typename Sh, int D>
 int32_t launch_join(riallm_ctx* ctx, const AttnArgs& a, const Plan& p, const float* ws, cudaStream_t st) {
   if (!p.join) return RIALLM_OK;
   return rl::launched(ctx, "paged_attention",
-                      rl::launch_pdl(join_kernel<Sh, D>, dim3(p.G - 1, Sh::R / 16), dim3(D * 4), 0, st, a, p.tiles,
+                      rl::launch_pdl(join_kernel<Sh, D>, dim3(p.G - 1, Sh::R / 16), dim3(kJoinThreads), 0, st, a, p.tiles,
                                      p.G, ws));
 }
 
