@@ -100,6 +100,7 @@ struct AttnArgs {
   const int* pos;
   Pages pg;
   int B, T, nh, rep;
+  uint32_t rep_inv;  // 2^32 / rep, rounded up (rep > 1)
   int window, sinks;
   float scale_log2;  // log2(e) / sqrt(d): weights are powers of two
   uint16_t* out;
@@ -153,26 +154,35 @@ struct Shape {
   static constexpr int R = R_, kBlock = kBlock_, kCost = kCost_;
 };
 struct Tile {
-  int b, row0, rows;    // sequence; first row and rows, of its T * rep
+  int b, rows;          // sequence; rows of the tile
+  int tok0, head0;      // its first row is head head0 (of rep) of token tok0
   int64_t p0, p1;       // positions of the first and last row
   Blocks bl;
 };
+// Token of row r of a tile, counted from the tile's first: (head0 + r) / rep.
+// rep is at most 16 and r below 256, so rounding 1 / rep up adds less than
+// 2^-20 to the quotient.
+__device__ __forceinline__ int token_of(const AttnArgs& a, const Tile& t, int r) {
+  return a.rep == 1 ? r : (int)__umulhi((uint32_t)(t.head0 + r), a.rep_inv);
+}
 template <typename Sh>
 __device__ __forceinline__ Tile tile_of(const AttnArgs& a, int tiles, int x) {
   Tile t;
   t.b = x / tiles;
-  t.row0 = (x - t.b * tiles) * Sh::R;
-  t.rows = min(Sh::R, a.T * a.rep - t.row0);
+  const int row0 = (x - t.b * tiles) * Sh::R;
+  t.rows = min(Sh::R, a.T * a.rep - row0);
+  t.tok0 = row0 / a.rep;
+  t.head0 = row0 - t.tok0 * a.rep;
   const int64_t p = a.pos[t.b];
-  t.p0 = p + t.row0 / a.rep;
-  t.p1 = p + (t.row0 + t.rows - 1) / a.rep;
+  t.p0 = p + t.tok0;
+  t.p1 = t.p0 + token_of(a, t, t.rows - 1);
   t.bl = blocks_of<Sh::kBlock>(a, t.p0, t.p1);
   return t;
 }
 // Where row r of a tile lies in q and out, in heads.
 __device__ __forceinline__ int64_t head_of(const AttnArgs& a, const Tile& t, int kh, int r) {
-  const int rr = t.row0 + r, tok = rr / a.rep;
-  return ((int64_t)t.b * a.T + tok) * a.nh + kh * a.rep + (rr - tok * a.rep);
+  const int tok = token_of(a, t, r);
+  return ((int64_t)t.b * a.T + t.tok0 + tok) * a.nh + kh * a.rep + (t.head0 + r - tok * a.rep);
 }
 
 // Share c of G: units [W c / G, W (c+1) / G). The share that unit u is in.
@@ -298,6 +308,23 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float y;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+// (a0, a1) += (b0, b1)
+__device__ __forceinline__ void add_f32x2(float& a0, float& a1, float b0, float b1) {
+  asm("{\n\t.reg .b64 ra, rb;\n\tmov.b64 ra, {%0, %1};\n\tmov.b64 rb, {%2, %3};\n\t"
+      "add.rn.f32x2 ra, ra, rb;\n\tmov.b64 {%0, %1}, ra;\n\t}"
+      : "+f"(a0), "+f"(a1)
+      : "f"(b0), "f"(b1));
+}
+// Bits e for which j + e <= x (0 <= e < 32).
+__device__ __forceinline__ uint32_t bits_upto(int x, int j) {
+  const int n = x - j;
+  return n < 0 ? 0u : n >= 31 ? 0xffffffffu : (2u << n) - 1u;
 }
 // 16 bytes, or 16 zero bytes where `bytes` is 0 (src is not read then).
 __device__ __forceinline__ void cp_async_16z(void* dst, const void* src, int bytes) {
@@ -427,7 +454,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
         const int r = h * 8 + (lane >> 2);
         m[h] = -INFINITY;
         l[h] = 0.f;
-        sp[h] = r < now.t.rows ? a.span(now.t.p0 + (now.t.row0 + r) / a.rep - now.t.row0 / a.rep) : Span{0, -1};
+        sp[h] = r < now.t.rows ? a.span(now.t.p0 + token_of(a, now.t, r)) : Span{0, -1};
       }
     } else {
       __syncwarp();
@@ -911,25 +938,26 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         // The query rows, 32 by this warp (16 with one tile), 16 bytes a lane.
         {
           constexpr int kRowsPerWarp = kTwoTiles ? 32 : 16, C = D / 8;
-          const int rb = warp * kRowsPerWarp;
           uint8_t* tile = qs + (kTwoTiles ? slot * kTileBytes<D> : 0);
-#pragma unroll 4
-          for (int x = lane; x < kRowsPerWarp * C; x += 32) {
-            const int rr = rb + x / C, c = x % C, lr = rr & 127;
-            uint4 w = make_uint4(0, 0, 0, 0);
-            if (rr < t.rows) w = *reinterpret_cast<const uint4*>(a.q + head_of(a, t, sg.c.kh, rr) * D + c * 8);
-            *reinterpret_cast<uint4*>(tile + (c / 8) * kHalf + lr * 128 + (((c & 7) ^ (lr & 7)) * 16)) = w;
+#pragma unroll
+          for (int x = 0; x < kRowsPerWarp * C / 32; ++x) {
+            const int rr = warp * kRowsPerWarp + (x * 32 + lane) / C, c = lane % C, lr = rr & 127;
+            const bool have = rr < t.rows;
+            cp_async_16z(tile + (c / 8) * kHalf + lr * 128 + (((c & 7) ^ (lr & 7)) * 16),
+                         a.q + head_of(a, t, sg.c.kh, have ? rr : 0) * D + c * 8, have ? 16 : 0);
           }
+          rl::cp_async_commit();
+          rl::cp_async_wait<0>();
           rl::fence_proxy_async_smem();
           rl::mbar_arrive(&bars.q_full);
         }
         const bool in = r < t.rows;
-        const int base_tok = t.row0 / a.rep;
-        const Span sp = in ? a.span(t.p0 + (t.row0 + r) / a.rep - base_tok) : Span{0, -1};
-        // Positions of this warp's first and last row.
+        const Span sp = in ? a.span(t.p0 + token_of(a, t, r)) : Span{0, -1};
+        // Blocks that every row of this warp sees whole end at most at
+        // whole_hi, and begin at whole_lo or later, or lie in the sinks.
         const int w0 = r - lane, w1 = min(w0 + 31, t.rows - 1);
-        const int64_t wp0 = t.p0 + (t.row0 + min(w0, t.rows - 1)) / a.rep - base_tok;
-        const int64_t wp1 = t.p0 + (t.row0 + w1) / a.rep - base_tok;
+        const int whole_hi = w1 < w0 ? -1 : a.span(t.p0 + token_of(a, t, w0)).hi;
+        const int whole_lo = w1 < w0 ? 0 : a.span(t.p0 + token_of(a, t, w1)).lo;
         float m = -INFINITY, l = 0.f;  // maximum (of scaled scores) that the weights are relative to, and their sum
         int done = 0;                  // blocks of this segment
         for (int i = sg.i0 + (kTwoTiles ? 0 : slot); i < sg.i1; i += kTwoTiles ? 1 : 2) {
@@ -941,30 +969,32 @@ __global__ void __launch_bounds__(kManyThreads, 1)
 #pragma unroll
           for (int y = 0; y < 4; ++y) rl::tmem_ld_32x32b_x32(ts + y * 32, x[y]);
           rl::tmem_wait_ld();
-          if (is_edge(a, wp0, wp1, j0, j0 + 127) || w1 < w0) {
-#pragma unroll
-            for (int y = 0; y < 4; ++y)
-#pragma unroll
-              for (int e = 0; e < 32; ++e)
-                if (!sees(sp, a.sinks, j0 + y * 32 + e)) x[y][e] = 0xff800000u;
-          }
-          // Pages that are not held are loaded as zeros; their scores go.
+          // Pages that are not held are loaded as zeros; their scores go too.
           const uint32_t bad = *(volatile uint32_t*)&gone[(n0 + i - sg.i0) & 7];
-          if (bad) {
+          if (bad || j0 + 127 > whole_hi || (j0 < whole_lo && j0 + 127 >= a.sinks)) {
 #pragma unroll
-            for (int y = 0; y < 4; ++y)
+            for (int y = 0; y < 4; ++y) {
+              const int j = j0 + y * 32;
+              uint32_t see = bits_upto(sp.hi, j) & (~bits_upto(sp.lo - 1, j) | bits_upto(a.sinks - 1, j));
+              if (a.pg.lg == 4)
+                see &= (bad >> (2 * y) & 1 ? 0xffff0000u : 0xffffffffu) & (bad >> (2 * y + 1) & 1 ? 0xffffu : 0xffffffffu);
+              else if (bad >> (y * 32 >> a.pg.lg) & 1)
+                see = 0;
 #pragma unroll
               for (int e = 0; e < 32; ++e)
-                if (bad >> ((y * 32 + e) >> a.pg.lg) & 1) x[y][e] = 0xff800000u;
+                if (!(see >> e & 1)) x[y][e] = 0xff800000u;
+            }
           }
           float top[4];
 #pragma unroll
           for (int y = 0; y < 4; ++y) {
-            top[y] = -INFINITY;
+            top[y] = __uint_as_float(x[y][0]);
 #pragma unroll
-            for (int e = 0; e < 32; ++e) top[y] = fmaxf(top[y], __uint_as_float(x[y][e]));
+            for (int e = 1; e < 31; e += 2)
+              top[y] = max3(top[y], __uint_as_float(x[y][e]), __uint_as_float(x[y][e + 1]));
+            top[y] = fmaxf(top[y], __uint_as_float(x[y][31]));
           }
-          const float mb = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * a.scale_log2;
+          const float mb = fmaxf(max3(top[0], top[1], top[2]), top[3]) * a.scale_log2;
           if (done == 0) {
             m = mb;
           } else if (__any_sync(0xffffffffu, mb > m + 8.f)) {
@@ -1001,7 +1031,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                             a.scale_log2, a.scale_log2, -base, -base);
               e0 = ex2(e0);
               e1 = ex2(e1);
-              sum[e & 3] += e0 + e1;
+              add_f32x2(sum[2 * (e & 1)], sum[2 * (e & 1) + 1], e0, e1);
               p[e] = rl::pack_bf16x2(e0, e1);
             }
             rl::tmem_st_32x32b_x32(ts + y * 32, p);
@@ -1021,7 +1051,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
           rl::tc_fence_after();
         }
         const bool whole = sg.i0 == 0 && sg.i1 == t.bl.n;
-        const bool odd = *(volatile int*)&poison[seg & 15] != 0;
+        bool odd = false;
         float* part = ws + (2 * (int64_t)blockIdx.x + (seg == 0 ? 0 : 1)) * kSlotFloats<Sh, D>;
         float mine = 1.f, other = 0.f;  // factors of the slots' sums
         if constexpr (!kTwoTiles) {
@@ -1068,9 +1098,14 @@ __global__ void __launch_bounds__(kManyThreads, 1)
               v[e] = __float_as_uint(fmaf(__uint_as_float(v[e]), mine, mc[e * 128] * other));
             if (y % kTurn == kTurn - 1) rl::mbar_arrive(&bars.merge_empty);
           }
-          if (y == 0 && !whole && in) {
-            part[r] = m;
-            part[Sh::R + r] = l;
+          if (y == 0) {
+            // Here every block of the segment has been multiplied, the other
+            // slot's too, so it has been looked through.
+            odd = *(volatile int*)&poison[seg & 15] != 0;
+            if (!whole && in) {
+              part[r] = m;
+              part[Sh::R + r] = l;
+            }
           }
           if (!in) continue;
           if (odd) {
@@ -1090,7 +1125,10 @@ __global__ void __launch_bounds__(kManyThreads, 1)
           }
           if (whole) {
             const float inv = l == 0.f ? 0.f : __fdiv_rn(1.f, l);
+            // Two tiles: by way of the slot's query tile, whose products are
+            // done, to write whole rows at a time.
             uint16_t* o = a.out + head_of(a, t, sg.c.kh, r) * D + y * 32;
+            uint8_t* row = qs + slot * kTileBytes<D> + (y / 2) * kHalf + (r & 127) * 128;
 #pragma unroll
             for (int e = 0; e < 32; e += 8) {
               uint4 w;
@@ -1098,7 +1136,10 @@ __global__ void __launch_bounds__(kManyThreads, 1)
               w.y = rl::pack_bf16x2(__uint_as_float(v[e + 2]) * inv, __uint_as_float(v[e + 3]) * inv);
               w.z = rl::pack_bf16x2(__uint_as_float(v[e + 4]) * inv, __uint_as_float(v[e + 5]) * inv);
               w.w = rl::pack_bf16x2(__uint_as_float(v[e + 6]) * inv, __uint_as_float(v[e + 7]) * inv);
-              *reinterpret_cast<uint4*>(o + e) = w;
+              if (kTwoTiles)
+                *reinterpret_cast<uint4*>(row + ((((y & 1) * 4 + e / 8) ^ (r & 7)) * 16)) = w;
+              else
+                *reinterpret_cast<uint4*>(o + e) = w;
             }
           } else {
             float* o = part + 2 * Sh::R + r * D + y * 32;
@@ -1108,6 +1149,18 @@ __global__ void __launch_bounds__(kManyThreads, 1)
           }
         }
         if (!go) break;
+        if (kTwoTiles && whole) {
+          constexpr int C = D / 8;
+          __syncwarp();
+#pragma unroll
+          for (int x = 0; x < C; ++x) {
+            const int rr = w0 + (x * 32 + lane) / C, c = lane % C, lr = rr & 127;
+            if (rr < t.rows)
+              *reinterpret_cast<uint4*>(a.out + head_of(a, t, sg.c.kh, rr) * D + c * 8) = *reinterpret_cast<const uint4*>(
+                  qs + slot * kTileBytes<D> + (c / 8) * kHalf + lr * 128 + (((c & 7) ^ (lr & 7)) * 16));
+          }
+          __syncwarp();
+        }
         rl::tc_fence_before();  // the next group's first product overwrites O
         n0 += nb;
         ++seg;
@@ -1345,6 +1398,7 @@ int32_t riallm_cuda_paged_attention(riallm_ctx* ctx, const void* q, const void* 
     a.pos = pos;
     a.pg = make_pages(page_table, table_stride, max_pages, num_pages, nkv, page_size);
     a.B = B, a.T = T, a.nh = nh, a.rep = nh / nkv;
+    a.rep_inv = (uint32_t)(((1ull << 32) + a.rep - 1) / a.rep);
     a.window = window, a.sinks = sinks;
     a.scale_log2 = (float)(1.4426950408889634 / sqrt((double)d));
     a.out = static_cast<uint16_t*>(out);
