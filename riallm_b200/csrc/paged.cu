@@ -280,7 +280,10 @@ struct Cursor {
 
 // A share leaves at most two partial results, in slots 2c and 2c + 1: of the
 // group it begins with, and of one that begins inside it. A slot holds the
-// maxima, the sums and the accumulators of a tile's rows.
+// maxima, the sums and the accumulators of a tile's rows, [D][R] (a thread
+// that holds a row writes it column by column) or [R][D].
+template <typename Sh>
+constexpr bool kByColumn = Sh::R > 16;
 template <typename Sh, int D>
 constexpr int kSlotFloats = Sh::R * (D + 2);
 
@@ -649,8 +652,8 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
 // not see whole. Keys and values share a ring of kStages blocks in smem.
 constexpr int kManyThreads = 12 * 32;
 // Registers: the launch's 168 a thread, of which the third warpgroup (loads,
-// products) keeps 88 and the weights' two take 208 (2 * 208 + 88 = 3 * 168).
-constexpr int kWeightRegs = 208, kOtherRegs = 88;
+// products) keeps 56 and the weights' two take 224 (2 * 224 + 56 = 3 * 168).
+constexpr int kWeightRegs = 224, kOtherRegs = 56;
 constexpr int kMaxStages = 8;
 template <bool kTwoTiles>
 using Many = Shape<kTwoTiles ? 256 : 128, 128, 4>;
@@ -665,11 +668,17 @@ constexpr int kManySmem = (2 + kManyStages<D>) * kTileBytes<D> + 1024;
 
 struct ManyBars {
   uint64_t full[kMaxStages], empty[kMaxStages], ok[kMaxStages];  // loaded, read, looked through (values)
-  uint64_t q_full, s_full[2], p_full[2], pv_done[2], merge_full, merge_empty, drain;
+  uint64_t q_full, s_full[2], p_full[2][2], pv_done[2], merge_full, merge_empty, drain;  // p_full: slot, half
 };
 
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort, int* status) {
   return __all_sync(0xffffffffu, rl::mbar_wait(bar, parity, abort, status));
+}
+// True in one lane of the (converged) warp, in a way the compiler knows.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
 }
 // A bounded wait for work in flight on the way out.
 __device__ __forceinline__ void drain_wait(uint64_t* bar, uint32_t parity) {
@@ -725,10 +734,11 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       rl::mbar_init(&bars.empty[i], 1);
       rl::mbar_init(&bars.ok[i], 2);
     }
-    rl::mbar_init(&bars.q_full, 256);
+    rl::mbar_init(&bars.q_full, 8);
     for (int i = 0; i < 2; ++i) {
       rl::mbar_init(&bars.s_full[i], 1);
-      rl::mbar_init(&bars.p_full[i], 128);
+      rl::mbar_init(&bars.p_full[i][0], 4);
+      rl::mbar_init(&bars.p_full[i][1], 4);
       rl::mbar_init(&bars.pv_done[i], 1);
     }
     rl::mbar_init(&bars.merge_full, 128);
@@ -798,71 +808,84 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       }
     } else if (work && warp == 9) {
       // --------------------------------------------- products
-      if (lane == 0) {
+      // The whole warp walks the blocks, so that descriptors are uniform; one
+      // lane issues. Descriptors of one tile differ in their start address
+      // alone (the low word).
+      {
         constexpr uint32_t kIdS = rl::idesc_bf16_f32(128, 128);
         constexpr uint32_t kIdO = rl::idesc_bf16_f32(128, D) | (1u << 16);  // B (the values) MN-major
-        const uint32_t ring_a = rl::smem_u32(ring), q_a = rl::smem_u32(qs);
+        const bool leader = elect_one();
+        const uint64_t q_desc = rl::sdesc_kmajor_sw128(rl::smem_u32(qs));
+        const uint64_t k_desc = rl::sdesc_kmajor_sw128(rl::smem_u32(ring));
+        const uint64_t v_desc = rl::sdesc_mnmajor_sw128(rl::smem_u32(ring), kHalf);
         auto scores = [&](int slot, int st) {
-          const uint32_t qa = q_a + (kTwoTiles ? slot * kTileBytes<D> : 0), ka = ring_a + st * kTileBytes<D>;
+          const uint64_t qd = q_desc + (kTwoTiles ? slot * (kTileBytes<D> >> 4) : 0), kd = k_desc + st * (kTileBytes<D> >> 4);
+          if (leader) {
 #pragma unroll
-          for (int x = 0; x < D / 16; ++x) {
-            const uint32_t off = (x / 4) * kHalf + (x % 4) * 32;
-            rl::tc_mma_ss(tm + slot * 128, rl::sdesc_kmajor_sw128(qa + off), rl::sdesc_kmajor_sw128(ka + off), kIdS,
-                          x > 0);
+            for (int x = 0; x < D / 16; ++x) {
+              const uint32_t off = ((x / 4) * kHalf + (x % 4) * 32) >> 4;
+              rl::tc_mma_ss(tm + slot * 128, qd + off, kd + off, kIdS, x > 0);
+            }
+            rl::tc_commit(&bars.s_full[slot]);
           }
-          rl::tc_commit(&bars.s_full[slot]);
+          __syncwarp();
         };
+        uint32_t pc[2] = {0, 0};  // blocks of each slot whose weights were waited for
         auto sums = [&](int slot, int st, bool add) {
-          const uint32_t va = ring_a + st * kTileBytes<D>;
+          const uint64_t vd = v_desc + st * (kTileBytes<D> >> 4);
 #pragma unroll
-          for (int x = 0; x < 8; ++x)
-            rl::tc_mma_ts(tm + 256 + slot * D, tm + slot * 128 + x * 8, rl::sdesc_mnmajor_sw128(va + x * 2048, kHalf),
-                          kIdO, add || x > 0);
-          rl::tc_commit(&bars.pv_done[slot]);
+          for (int h = 0; h < 2; ++h) {
+            if (!warp_wait(&bars.p_full[slot][h], pc[slot] & 1, abort, status)) return false;
+            rl::tc_fence_after();
+            if (leader) {
+#pragma unroll
+              for (int x = 4 * h; x < 4 * h + 4; ++x)
+                rl::tc_mma_ts(tm + 256 + slot * D, tm + slot * 128 + x * 8, vd + x * (2048 >> 4), kIdO, add || x > 0);
+              if (h == 1) rl::tc_commit(&bars.pv_done[slot]);
+            }
+            __syncwarp();
+          }
+          ++pc[slot];
+          return true;
+        };
+        auto release = [&](int st) {
+          if (leader) rl::tc_commit(&bars.empty[st]);
+          __syncwarp();
         };
         int n0 = 0, seg = 0;      // blocks before this segment, segments
-        uint32_t pc[2] = {0, 0};  // p_full phases waited for
         bool go = true;
         do {
           const int nb = sg.i1 - sg.i0;
-          go = rl::mbar_wait(&bars.q_full, seg & 1, abort, status);
+          go = warp_wait(&bars.q_full, seg & 1, abort, status);
           rl::tc_fence_after();
           if constexpr (kTwoTiles) {
             for (int j = 0; go && j <= nb; ++j) {
               const int kl = 2 * (n0 + j), vl = kl - 1;  // block j's keys, block j-1's values
-              if (j < nb) go = rl::mbar_wait(&bars.full[kl % S], (kl / S) & 1, abort, status);
-              if (go && j > 0) go = rl::mbar_wait(&bars.ok[vl % S], (vl / S) & 1, abort, status);
+              if (j < nb) go = warp_wait(&bars.full[kl % S], (kl / S) & 1, abort, status);
+              if (go && j > 0) go = warp_wait(&bars.ok[vl % S], (vl / S) & 1, abort, status);
               for (int slot = 0; go && slot < 2; ++slot) {
-                if (j > 0) {
-                  go = rl::mbar_wait(&bars.p_full[slot], pc[slot]++ & 1, abort, status);
-                  if (!go) break;
-                  rl::tc_fence_after();
-                  sums(slot, vl % S, j > 1);
-                }
-                if (j < nb) scores(slot, kl % S);
+                if (j > 0) go = sums(slot, vl % S, j > 1);
+                if (go && j < nb) scores(slot, kl % S);
               }
               if (!go) break;
-              if (j < nb) rl::tc_commit(&bars.empty[kl % S]);
-              if (j > 0) rl::tc_commit(&bars.empty[vl % S]);
+              if (j < nb) release(kl % S);
+              if (j > 0) release(vl % S);
             }
           } else {
             for (int j = 0; go && j < nb + 2; ++j) {
               const int slot = j & 1;
               if (j >= 2) {  // block j - 2
                 const int vl = 2 * (n0 + j - 2) + 1;
-                go = rl::mbar_wait(&bars.ok[vl % S], (vl / S) & 1, abort, status) &&
-                     rl::mbar_wait(&bars.p_full[slot], pc[slot]++ & 1, abort, status);
+                go = warp_wait(&bars.ok[vl % S], (vl / S) & 1, abort, status) && sums(slot, vl % S, j >= 4);
                 if (!go) break;
-                rl::tc_fence_after();
-                sums(slot, vl % S, j >= 4);
-                rl::tc_commit(&bars.empty[vl % S]);
+                release(vl % S);
               }
               if (j < nb) {
                 const int kl = 2 * (n0 + j);
-                go = rl::mbar_wait(&bars.full[kl % S], (kl / S) & 1, abort, status);
+                go = warp_wait(&bars.full[kl % S], (kl / S) & 1, abort, status);
                 if (!go) break;
                 scores(slot, kl % S);
-                rl::tc_commit(&bars.empty[kl % S]);
+                release(kl % S);
               }
               if (nb == 1 && j == 0) ++j;  // slot 1 has no block
             }
@@ -870,10 +893,10 @@ __global__ void __launch_bounds__(kManyThreads, 1)
           n0 += nb;
           ++seg;
         } while (go && sg.next(a, tiles));
-        rl::tc_commit(&bars.drain);  // nothing in flight when tensor memory is freed
+        if (leader) rl::tc_commit(&bars.drain);  // nothing in flight when tensor memory is freed
+        __syncwarp();
         drain_wait(&bars.drain, 0);
       }
-      __syncwarp();
     } else if (work) {
       // ------------------------------------- values looked through
       int n = 0, seg = 0;
@@ -949,7 +972,8 @@ __global__ void __launch_bounds__(kManyThreads, 1)
           rl::cp_async_commit();
           rl::cp_async_wait<0>();
           rl::fence_proxy_async_smem();
-          rl::mbar_arrive(&bars.q_full);
+          __syncwarp();
+          if (lane == 0) rl::mbar_arrive(&bars.q_full);
         }
         const bool in = r < t.rows;
         const Span sp = in ? a.span(t.p0 + token_of(a, t, r)) : Span{0, -1};
@@ -1034,12 +1058,14 @@ __global__ void __launch_bounds__(kManyThreads, 1)
               add_f32x2(sum[2 * (e & 1)], sum[2 * (e & 1) + 1], e0, e1);
               p[e] = rl::pack_bf16x2(e0, e1);
             }
+            // A half of the weights at a time, so that their products begin.
             rl::tmem_st_32x32b_x32(ts + y * 32, p);
+            rl::tmem_wait_st();
+            rl::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) rl::mbar_arrive(&bars.p_full[slot][y]);
           }
           l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-          rl::tmem_wait_st();
-          rl::tc_fence_before();
-          rl::mbar_arrive(&bars.p_full[slot]);
           ++sc;
           ++done;
         }
@@ -1142,10 +1168,9 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                 *reinterpret_cast<uint4*>(o + e) = w;
             }
           } else {
-            float* o = part + 2 * Sh::R + r * D + y * 32;
+            float* o = part + 2 * Sh::R + y * 32 * Sh::R + r;
 #pragma unroll
-            for (int e = 0; e < 32; e += 4)
-              *reinterpret_cast<uint4*>(o + e) = make_uint4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+            for (int e = 0; e < 32; ++e) o[e * Sh::R] = __uint_as_float(v[e]);
           }
         }
         if (!go) break;
@@ -1173,15 +1198,17 @@ __global__ void __launch_bounds__(kManyThreads, 1)
   if (warp == 9) rl::tmem_dealloc(tm, 512);
 }
 
-// CTA (c, y) adds up rows 16 y .. 16 y + 15 of the partial results of the
-// group that the boundary between the shares c and c + 1 cuts, if c is the
-// first that holds part of it.
-constexpr int kMaxShares = 512, kJoinThreads = 256;
+// CTA (c, y) adds up rows kJoinRows y .. of the partial results of the group
+// that the boundary between the shares c and c + 1 cuts, if c is the first
+// that holds part of it.
+constexpr int kMaxShares = 320, kJoinThreads = 256;
+template <typename Sh>
+constexpr int kJoinRows = kByColumn<Sh> ? 32 : 16;
 template <typename Sh, int D>
 __global__ void __launch_bounds__(kJoinThreads)
     join_kernel(const AttnArgs a, int tiles, int G, const float* __restrict__ ws) {
-  constexpr int kSlot = kSlotFloats<Sh, D>;
-  __shared__ float weight[16][kMaxShares];  // of the parts
+  constexpr int kSlot = kSlotFloats<Sh, D>, kRows = kJoinRows<Sh>;
+  __shared__ float weight[kRows][kMaxShares + 1];  // of the parts
   rl::pdl_wait();
   rl::pdl_launch_dependents();
   const int c0 = blockIdx.x;
@@ -1191,7 +1218,7 @@ __global__ void __launch_bounds__(kJoinThreads)
   cut.init(a, tiles, at, c0 + 1);
   const int64_t last = cut.at0 + cut.t.bl.n - 1;
   if (cut.i == 0 || share_of(at.W, at.G, cut.at0) != c0) return;  // not cut here, or cut before as well
-  const int row0 = blockIdx.y * 16, rows = min(16, cut.t.rows - row0);
+  const int row0 = blockIdx.y * kRows, rows = min(kRows, cut.t.rows - row0);
   if (rows <= 0) return;
   const int parts = share_of(at.W, at.G, last) - c0 + 1;
   // The first part is in its CTA's second slot where that share begins with
@@ -1199,38 +1226,51 @@ __global__ void __launch_bounds__(kJoinThreads)
   const float* first =
       ws + (2 * (int64_t)c0 + (share_begin(at.W, at.G, c0) < cut.at0 - Sh::kCost ? 1 : 0)) * kSlot;
   const float* rest = ws + 2 * (int64_t)c0 * kSlot;
-  const int lane = threadIdx.x & 31;
-  for (int r = threadIdx.x >> 5; r < rows; r += kJoinThreads / 32) {
+  constexpr int kPer = kJoinThreads / kRows;  // neighbouring threads of a row
+  {
+    const int r = threadIdx.x / kPer, i0 = threadIdx.x % kPer;
+    const bool have = r < rows;
     float M = -INFINITY;
-    for (int i = lane; i < parts; i += 32) {
-      const float x = __ldcg((i ? rest + (int64_t)i * 2 * kSlot : first) + row0 + r);
-      weight[r][i] = x;
-      M = fmaxf(M, x);
-    }
+    if (have)
+      for (int i = i0; i < parts; i += kPer) {
+        const float x = __ldcg((i ? rest + (int64_t)i * 2 * kSlot : first) + row0 + r);
+        weight[r][i] = x;
+        M = fmaxf(M, x);
+      }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    for (int o = kPer / 2; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
     float den = 0.f;
-    for (int i = lane; i < parts; i += 32) {
-      const float f = M == -INFINITY ? 0.f : ex2(weight[r][i] - M);
-      weight[r][i] = f;
-      den = fmaf(f, __ldcg((i ? rest + (int64_t)i * 2 * kSlot : first) + Sh::R + row0 + r), den);
-    }
+    if (have)
+      for (int i = i0; i < parts; i += kPer) {
+        const float f = M == -INFINITY ? 0.f : ex2(weight[r][i] - M);
+        weight[r][i] = f;
+        den = fmaf(f, __ldcg((i ? rest + (int64_t)i * 2 * kSlot : first) + Sh::R + row0 + r), den);
+      }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) den += __shfl_xor_sync(0xffffffffu, den, o);
+    for (int o = kPer / 2; o > 0; o >>= 1) den += __shfl_xor_sync(0xffffffffu, den, o);
     const float inv = den == 0.f ? 0.f : __fdiv_rn(1.f, den);
-    for (int i = lane; i < parts; i += 32) weight[r][i] *= inv;
+    if (have)
+      for (int i = i0; i < parts; i += kPer) weight[r][i] *= inv;
   }
   __syncthreads();
-  for (int x = threadIdx.x; x < rows * (D / 4); x += kJoinThreads) {
-    const int r = x / (D / 4), c = (x - r * (D / 4)) * 4;
-    const int64_t off = 2 * Sh::R + (row0 + r) * D + c;
-    float4 y = __ldcg(reinterpret_cast<const float4*>(first + off));
+  // Four columns of a row a thread; neighbours hold neighbouring rows where
+  // the parts are stored by column.
+  for (int x = threadIdx.x; x < kRows * (D / 4); x += kJoinThreads) {
+    const int r = kByColumn<Sh> ? x % kRows : x / (D / 4), c = (kByColumn<Sh> ? x / kRows : x % (D / 4)) * 4;
+    if (r >= rows) continue;
+    auto load = [&](const float* slot) {
+      const float* p = slot + 2 * Sh::R;
+      if (!kByColumn<Sh>) return __ldcg(reinterpret_cast<const float4*>(p + (row0 + r) * D + c));
+      p += c * Sh::R + row0 + r;
+      return make_float4(__ldcg(p), __ldcg(p + Sh::R), __ldcg(p + 2 * Sh::R), __ldcg(p + 3 * Sh::R));
+    };
+    float4 y = load(first);
     const float w0 = weight[r][0];
     y.x *= w0, y.y *= w0, y.z *= w0, y.w *= w0;
 #pragma unroll 8
     for (int i = 1; i < parts; ++i) {
       const float w = weight[r][i];
-      const float4 z = __ldcg(reinterpret_cast<const float4*>(rest + (int64_t)i * 2 * kSlot + off));
+      const float4 z = load(rest + (int64_t)i * 2 * kSlot);
       y.x = fmaf(w, z.x, y.x);
       y.y = fmaf(w, z.y, y.y);
       y.z = fmaf(w, z.z, y.z);
@@ -1268,7 +1308,7 @@ template <typename Sh, int D>
 int32_t launch_join(riallm_ctx* ctx, const AttnArgs& a, const Plan& p, const float* ws, cudaStream_t st) {
   if (!p.join) return RIALLM_OK;
   return rl::launched(ctx, "paged_attention",
-                      rl::launch_pdl(join_kernel<Sh, D>, dim3(p.G - 1, Sh::R / 16), dim3(kJoinThreads), 0, st, a, p.tiles,
+                      rl::launch_pdl(join_kernel<Sh, D>, dim3(p.G - 1, Sh::R / kJoinRows<Sh>), dim3(kJoinThreads), 0, st, a, p.tiles,
                                      p.G, ws));
 }
 
