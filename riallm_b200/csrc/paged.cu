@@ -858,19 +858,35 @@ __global__ void __launch_bounds__(kManyThreads, 1)
           const int nb = sg.i1 - sg.i0;
           go = warp_wait(&bars.q_full, seg & 1, abort, status);
           rl::tc_fence_after();
+          // Little may come between a slot's last product and the next one
+          // that can be issued: what can be waited for is waited for while
+          // products are queued.
           if constexpr (kTwoTiles) {
-            for (int j = 0; go && j <= nb; ++j) {
-              const int kl = 2 * (n0 + j), vl = kl - 1;  // block j's keys, block j-1's values
-              if (j < nb) go = warp_wait(&bars.full[kl % S], (kl / S) & 1, abort, status);
-              if (go && j > 0) go = warp_wait(&bars.ok[vl % S], (vl / S) & 1, abort, status);
-              for (int slot = 0; go && slot < 2; ++slot) {
-                if (j > 0) go = sums(slot, vl % S, j > 1);
-                if (go && j < nb) scores(slot, kl % S);
-              }
-              if (!go) break;
-              if (j < nb) release(kl % S);
-              if (j > 0) release(vl % S);
+            auto loaded = [&](int j) {  // block j's keys and block j - 1's values
+              const int kl = 2 * (n0 + j), vl = kl - 1;
+              return (j >= nb || warp_wait(&bars.full[kl % S], (kl / S) & 1, abort, status)) &&
+                     (j == 0 || warp_wait(&bars.ok[vl % S], (vl / S) & 1, abort, status));
+            };
+            go = go && loaded(0);
+            if (go) scores(0, 2 * n0 % S);
+            if (go) {
+              scores(1, 2 * n0 % S);
+              release(2 * n0 % S);
             }
+            go = go && loaded(1);
+            for (int j = 1; go && j <= nb; ++j) {
+              const int kl = 2 * (n0 + j), vl = kl - 1;
+              go = sums(0, vl % S, j > 1);
+              if (go && j < nb) scores(0, kl % S);
+              go = go && sums(1, vl % S, j > 1);
+              if (go) release(vl % S);
+              if (go && j < nb) {
+                scores(1, kl % S);
+                release(kl % S);
+              }
+              go = go && (j == nb || loaded(j + 1));
+            }
+
           } else {
             for (int j = 0; go && j < nb + 2; ++j) {
               const int slot = j & 1;
@@ -913,17 +929,17 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             uint4* v = reinterpret_cast<uint4*>(ring + st * kTileBytes<D>);
             bool any = false;
 #pragma unroll 1
-            for (int x = (warp - 10) * 32 + lane; x < kTileBytes<D> / 16; x += 8 * 64) {
-              uint4 w[8];
-              uint32_t odd[8];
+            for (int x = (warp - 10) * 32 + lane; x < kTileBytes<D> / 16; x += 4 * 64) {
+              uint4 w[4];
+              uint32_t odd[4];
 #pragma unroll
-              for (int y = 0; y < 8; ++y) w[y] = v[x + y * 64];
+              for (int y = 0; y < 4; ++y) w[y] = v[x + y * 64];
               uint32_t all = 0;
 #pragma unroll
-              for (int y = 0; y < 8; ++y) all |= odd[y] = odd16(w[y].x) | odd16(w[y].y) | odd16(w[y].z) | odd16(w[y].w);
+              for (int y = 0; y < 4; ++y) all |= odd[y] = odd16(w[y].x) | odd16(w[y].y) | odd16(w[y].z) | odd16(w[y].w);
               if (!all) continue;
 #pragma unroll
-              for (int y = 0; y < 8; ++y) {
+              for (int y = 0; y < 4; ++y) {
                 if (!odd[y]) continue;
                 uint16_t* e = reinterpret_cast<uint16_t*>(&v[x + y * 64]);
                 for (int z = 0; z < 8; ++z)
