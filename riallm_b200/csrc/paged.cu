@@ -50,39 +50,85 @@ __device__ __forceinline__ void rope_angle(int64_t p, float f, float* s, float* 
   sincosf((float)r, s, c);
 }
 
-// CTA (row, head): row b*T + t of qkv at position pos[b] + t.
-__global__ void __launch_bounds__(64)
-    rope_paged_append_kernel(const uint16_t* __restrict__ qkv, const int* __restrict__ pos, Pages pg, int T,
-                             int nh, int d, const float* __restrict__ inv_freq, uint16_t* __restrict__ q_out,
-                             uint16_t* __restrict__ kp, uint16_t* __restrict__ vp) {
+// CTA (rows, heads): up to kAppendRows rows of qkv, row b*T + t at position
+// pos[b] + t, and `hg` of its heads. A thread takes 8 dimensions of a head's
+// first half and the same 8 of its second (two 16-byte pieces): the pieces of
+// its first units are loaded before the angles are worked out, a row's d / 2
+// cosines and sines once for all of its heads. Bound by the bytes: qkv is
+// read once and as much written.
+constexpr int kAppendRows = 4, kAppendThreads = 256, kAppendUnits = 4;  // units a thread
+template <int D>
+__global__ void __launch_bounds__(kAppendThreads)
+    rope_paged_append_kernel(const uint16_t* __restrict__ qkv, const int* __restrict__ pos, Pages pg, int all_rows,
+                             int T, int nh, int rows_per_cta, int hg, const float* __restrict__ inv_freq,
+                             uint16_t* __restrict__ q_out, uint16_t* __restrict__ kp, uint16_t* __restrict__ vp) {
+  constexpr int P = D / 16;  // units of a head
+  __shared__ __align__(16) float cs[kAppendRows * D / 2], sn[kAppendRows * D / 2];
+  __shared__ int64_t at[kAppendRows];  // pool row of the position, kv head 0; -1
   rl::pdl_wait();
   rl::pdl_launch_dependents();
-  const int64_t row = blockIdx.x;
-  const int h = blockIdx.y, half = d >> 1;
-  const int b = (int)(row / T);
-  const int64_t p = (int64_t)pos[b] + (row - (int64_t)b * T);
-  const int nkv = pg.nkv;
-  const uint16_t* src = qkv + (row * (nh + 2 * nkv) + h) * d;
-  uint16_t* dst;
-  if (h < nh) {
-    dst = q_out + (row * nh + h) * d;
-  } else {
-    const int kh = (h - nh) % nkv;
-    const int64_t at = pg.row(b, kh, p);
-    if (at < 0) return;
-    dst = (h < nh + nkv ? kp : vp) + at * d;
-  }
-  for (int j = threadIdx.x; j < half; j += blockDim.x) {
-    if (h >= nh + nkv) {  // v is copied as it is
-      dst[j] = src[j];
-      dst[j + half] = src[j + half];
-      continue;
+  const int nkv = pg.nkv, heads = nh + 2 * nkv;
+  const int row0 = blockIdx.x * rows_per_cta, rows = min(rows_per_cta, all_rows - row0);
+  const int h0 = blockIdx.y * hg, hn = min(hg, heads - h0);
+  const int units = rows * hn * P;
+  uint4 lo[kAppendUnits], hi[kAppendUnits];
+#pragma unroll
+  for (int x = 0; x < kAppendUnits; ++x) {
+    const int u = x * kAppendThreads + threadIdx.x;
+    if (u < units) {
+      const int hu = u / P, r = hu / hn;
+      const uint4* src = reinterpret_cast<const uint4*>(qkv + ((int64_t)(row0 + r) * heads + h0 + (hu - r * hn)) * D);
+      lo[x] = __ldcs(src + u % P);
+      hi[x] = __ldcs(src + P + u % P);
     }
-    const float x1 = bf2f(src[j]), x2 = bf2f(src[j + half]);
-    float s, c;
-    rope_angle(p, inv_freq[j], &s, &c);
-    dst[j] = f2bf(fmaf(x1, c, -x2 * s));
-    dst[j + half] = f2bf(fmaf(x2, c, x1 * s));
+  }
+  if ((int)threadIdx.x < rows * (D / 2)) {
+    const int r = threadIdx.x / (D / 2), j = threadIdx.x % (D / 2);
+    const int b = (row0 + r) / T;
+    const int64_t p = (int64_t)pos[b] + (row0 + r - b * T);
+    if (h0 < nh + nkv) rope_angle(p, inv_freq[j], &sn[threadIdx.x], &cs[threadIdx.x]);
+    if (j == 0) at[r] = h0 + hn > nh ? pg.row(b, 0, p) : -1;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int x = 0; x < kAppendUnits; ++x) {
+    const int u = x * kAppendThreads + threadIdx.x;
+    if (u >= units) break;
+    const int c = u % P, hu = u / P, r = hu / hn, h = h0 + (hu - r * hn);
+    uint4 o1 = lo[x], o2 = hi[x];
+    if (h < nh + nkv) {
+      const float4* cr = reinterpret_cast<const float4*>(cs + r * (D / 2) + c * 8);
+      const float4* sr = reinterpret_cast<const float4*>(sn + r * (D / 2) + c * 8);
+      const uint32_t* a1 = reinterpret_cast<const uint32_t*>(&lo[x]);
+      const uint32_t* a2 = reinterpret_cast<const uint32_t*>(&hi[x]);
+      uint32_t* w1 = reinterpret_cast<uint32_t*>(&o1);
+      uint32_t* w2 = reinterpret_cast<uint32_t*>(&o2);
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        const float4 cc = cr[g], ss = sr[g];
+        const float* cf = reinterpret_cast<const float*>(&cc);
+        const float* sf = reinterpret_cast<const float*>(&ss);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const uint32_t x1 = a1[2 * g + e], x2 = a2[2 * g + e];
+          const float p1 = __uint_as_float(x1 << 16), q1 = __uint_as_float(x1 & 0xffff0000u);
+          const float p2 = __uint_as_float(x2 << 16), q2 = __uint_as_float(x2 & 0xffff0000u);
+          const float c0 = cf[2 * e], c1 = cf[2 * e + 1], s0 = sf[2 * e], s1 = sf[2 * e + 1];
+          w1[2 * g + e] = rl::pack_bf16x2(fmaf(p1, c0, -p2 * s0), fmaf(q1, c1, -q2 * s1));
+          w2[2 * g + e] = rl::pack_bf16x2(fmaf(p2, c0, p1 * s0), fmaf(q2, c1, q1 * s1));
+        }
+      }
+    }
+    uint16_t* dst;
+    if (h < nh) {
+      dst = q_out + ((int64_t)(row0 + r) * nh + h) * D;
+    } else {
+      if (at[r] < 0) continue;
+      const int kh = h < nh + nkv ? h - nh : h - nh - nkv;
+      dst = (h < nh + nkv ? kp : vp) + (at[r] + ((int64_t)kh << pg.lg)) * D;
+    }
+    reinterpret_cast<uint4*>(dst)[c] = o1;
+    reinterpret_cast<uint4*>(dst)[P + c] = o2;
   }
 }
 
@@ -1415,10 +1461,22 @@ int32_t riallm_cuda_rope_paged_append(riallm_ctx* ctx, const void* qkv, const in
     return rl::refuse(ctx, RIALLM_ERR_INVALID, what, "buffers must be 16-byte aligned");
   return rl::guarded(ctx, [&]() -> int32_t {
     const Pages pg = make_pages(page_table, table_stride, max_pages, num_pages, nkv, page_size);
+    // Heads per CTA: all of a row's units where they fit, fewer where the
+    // rows alone would leave SMs idle; then as many rows as still fit.
+    const int rows = B * T, heads = nh + 2 * nkv, per_head = d / 16, fit = kAppendThreads * kAppendUnits;
+    int hg = std::min(heads, fit / per_head);
+    const int64_t want = 2ll * ctx->num_sms;
+    if ((int64_t)rows * ((heads + hg - 1) / hg) < want)
+      hg = (int)std::max<int64_t>(std::min(heads, kAppendThreads / per_head / 4), (int64_t)heads * rows / want);
+    hg = std::min(hg, fit / per_head);
+    int per_cta = std::min(kAppendRows, fit / (hg * per_head));
+    per_cta = (int)std::max<int64_t>(1, std::min<int64_t>(per_cta, rows * (int64_t)((heads + hg - 1) / hg) / want));
+    const auto kernel = d == 128 ? rope_paged_append_kernel<128> : rope_paged_append_kernel<64>;
     return rl::launched(ctx, what,
-                        rl::launch_pdl(rope_paged_append_kernel, dim3(B * T, nh + 2 * nkv), dim3(64), 0,
-                                       (cudaStream_t)stream, static_cast<const uint16_t*>(qkv), pos, pg, T, nh, d,
-                                       inv_freq, static_cast<uint16_t*>(q_out), static_cast<uint16_t*>(k_pages),
+                        rl::launch_pdl(kernel, dim3((rows + per_cta - 1) / per_cta, (heads + hg - 1) / hg),
+                                       dim3(kAppendThreads), 0, (cudaStream_t)stream,
+                                       static_cast<const uint16_t*>(qkv), pos, pg, rows, T, nh, per_cta, hg, inv_freq,
+                                       static_cast<uint16_t*>(q_out), static_cast<uint16_t*>(k_pages),
                                        static_cast<uint16_t*>(v_pages)));
   });
 }

@@ -15,41 +15,37 @@
 // 1e5 tokens would move those borders by more than a rare token's share.
 // Temperature 0 (and a row whose softmax is undefined: a NaN, +inf, or -inf
 // throughout) puts all of p_i on the first maximum.
-#include <cfloat>
+//
+// Two launches:
+//   stats_kernel  : every row's maximum, where it is, and its sum of
+//                   exponentials in float32, a slice of a row per CTA; bound
+//                   by reading the logits once.
+//   sample_kernel : a cluster of 8 CTAs per sequence finds the first
+//                   rejection (a comparison that float32 sums leave within
+//                   1e-4 of equality is made again with 64-bit ones), then
+//                   goes over the one row that the token comes from, in 64
+//                   bits, an eighth of the vocabulary per CTA.
+#include <cooperative_groups.h>
+
+#include <algorithm>
+#include <cmath>
 
 #include "common.cuh"
 #include "internal.h"
 
+namespace cg = cooperative_groups;
+
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256, kCluster = 8, kSampleThreads = 512, kSampleWarps = kSampleThreads / 32;
 
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 __device__ __forceinline__ float load_logit(const void* x, bool bf16, int64_t i) {
   return bf16 ? __uint_as_float((uint32_t)static_cast<const uint16_t*>(x)[i] << 16) : static_cast<const float*>(x)[i];
-}
-
-// One row's distribution: softmax with maximum m, denominator z and 1 / t,
-// or all on `top`.
-struct Dist {
-  double m, z, t;
-  int top;
-  bool greedy;
-  __device__ __forceinline__ double weight(float l, int j) const {  // z * p(j)
-    if (greedy) return j == top ? 1.0 : 0.0;
-    return l == -INFINITY ? 0.0 : exp(((double)l - m) / t);
-  }
-};
-
-template <typename T, typename F>
-__device__ __forceinline__ T block_reduce(T v, T* sh, F f) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = f(v, __shfl_xor_sync(0xffffffffu, v, o));
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = sh[0];
-  for (int w = 1; w < kThreads / 32; ++w) v = f(v, sh[w]);
-  return v;
 }
 
 struct VerifyArgs {
@@ -65,97 +61,386 @@ struct VerifyArgs {
   int* accepted;
 };
 
-// CTA per sequence.
-__global__ void __launch_bounds__(kThreads) verify_draft_kernel(VerifyArgs a) {
-  __shared__ double sd[kThreads / 32];
-  __shared__ long long sl[kThreads / 32];
-  __shared__ double scan[kThreads];
-  __shared__ int found;
+// Of a slice of a row: its maximum (NaN left out), the lowest index that
+// holds it, and the sum of 2^((x - max) c), NaN where the softmax is undefined.
+struct Stat {
+  float m, s;
+  int top, pad;
+};
+// log2(e) / temperature, kept where 0 * c and inf * c are harmless.
+__device__ __forceinline__ float scale_of(float t) {
+  return t > 0.f ? fminf(fmaxf(1.4426950408889634f / t, 1e-30f), 1e30f) : 1.f;
+}
+
+// Adds N values from index j on.
+template <int N>
+__device__ __forceinline__ void add_stat(Stat& st, const float (&x)[N], int j, float c) {
+  float mx = x[0];
+#pragma unroll
+  for (int e = 1; e < N; ++e) mx = fmaxf(mx, x[e]);
+  if (mx > st.m) {
+    int at = 0;
+#pragma unroll
+    for (int e = N - 1; e >= 0; --e)
+      if (x[e] == mx) at = e;
+    st.s *= ex2((st.m - mx) * c);
+    st.m = mx;
+    st.top = j + at;
+  }
+  const float base = st.m == -INFINITY ? 0.f : st.m;
+  float s = 0.f;
+#pragma unroll
+  for (int e = 0; e < N; ++e) s += ex2((x[e] - base) * c);
+  st.s += s;
+}
+// The two slices' statistics together; the lower index where they tie.
+__device__ __forceinline__ void merge_stat(Stat& a, const Stat& b, float c) {
+  const float m = fmaxf(a.m, b.m), base = m == -INFINITY ? 0.f : m;
+  a.top = a.m > b.m ? a.top : b.m > a.m ? b.top : min(a.top, b.top);
+  a.s = a.s * (a.m == m ? 1.f : ex2((a.m - base) * c)) + b.s * (b.m == m ? 1.f : ex2((b.m - base) * c));
+  a.m = m;
+}
+
+// A CTA per slice of a row, row by row. 16 bytes a load where the row's place allows, four loads
+// in flight a thread.
+template <bool kBf16>
+__global__ void __launch_bounds__(kThreads) stats_kernel(const VerifyArgs a, int slices, int slice, Stat* __restrict__ stats) {
+  constexpr int N = kBf16 ? 8 : 4;
+  __shared__ Stat sh[kThreads / 32];
   rl::pdl_wait();
   rl::pdl_launch_dependents();
-  const int b = blockIdx.x, tid = threadIdx.x, V = a.V;
-  const float temp = a.temperature[b];
-  Dist ds;
-  int64_t base = 0;
-  int acc = 0, x = -1;
-  for (;; ++acc) {
-    base = ((int64_t)b * (a.n + 1) + acc) * V;
-    // Maximum with the lowest index: order key = (value, -index).
-    float m = -INFINITY;
-    int top = 0x7fffffff;
-    int nan = 0;
-    for (int j = tid; j < V; j += kThreads) {
-      const float l = load_logit(a.logits, a.bf16, base + j);
-      nan |= l != l;
-      if (l > m) m = l, top = j;
+  const int row = blockIdx.x / slices;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int begin = min(a.V, (int)(blockIdx.x - row * slices) * slice), end = min(a.V, begin + slice);
+  const float c = scale_of(a.temperature[row / (a.n + 1)]);
+  const int64_t base = (int64_t)row * a.V;
+  // Whole vectors of the slice: [v0, v1) as row indices, the rest one by one.
+  const int skew = (int)((base + begin) & (N - 1));
+  const int v0 = min(end, begin + (skew ? N - skew : 0)), v1 = v0 + (end - v0) / N * N;
+  Stat st{-INFINITY, 0.f, 0x7fffffff, 0};
+  const uint4* vec = reinterpret_cast<const uint4*>(static_cast<const char*>(a.logits) + (base + v0) * (kBf16 ? 2 : 4));
+  const int nv = (v1 - v0) / N;
+  for (int i = tid; i < nv; i += 4 * kThreads) {
+    uint4 w[4];
+#pragma unroll
+    for (int y = 0; y < 4; ++y)
+      if (i + y * kThreads < nv) w[y] = __ldcs(vec + i + y * kThreads);
+#pragma unroll
+    for (int y = 0; y < 4; ++y) {
+      if (i + y * kThreads >= nv) break;
+      float x[N];
+      const uint32_t* u = reinterpret_cast<const uint32_t*>(&w[y]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (kBf16) {
+          x[(2 * e) % N] = __uint_as_float(u[e] << 16);
+          x[(2 * e + 1) % N] = __uint_as_float(u[e] & 0xffff0000u);
+        } else {
+          x[e] = __uint_as_float(u[e]);
+        }
+      }
+      add_stat<N>(st, x, v0 + (i + y * kThreads) * N, c);
     }
-    nan = __syncthreads_or(nan);
-    const double bm = block_reduce((double)m, sd, [](double p, double q) { return p > q ? p : q; });
-    long long at = (double)m == bm && top != 0x7fffffff ? top : 0x7fffffffffffffffll;
-    at = block_reduce(at, sl, [](long long p, long long q) { return p < q ? p : q; });
-    ds.m = bm;
-    ds.t = temp;
-    ds.top = at == 0x7fffffffffffffffll ? 0 : (int)at;
-    ds.greedy = !(temp > 0.f) || nan || bm == INFINITY || bm == -INFINITY;
-    double z = 0.0;
-    for (int j = tid; j < V; j += kThreads) z += ds.weight(load_logit(a.logits, a.bf16, base + j), j);
-    ds.z = block_reduce(z, sd, [](double p, double q) { return p + q; });
-    x = acc < a.n ? a.drafts[(int64_t)b * a.n + acc] : -1;
-    if ((unsigned)x >= (unsigned)V) x = -1;
-    if (x < 0) break;  // no draft here
-    const int64_t qrow = ((int64_t)b * a.n + acc) * V;
-    const double qx = a.probs ? (double)a.probs[qrow + x] : 1.0;
-    const double px = ds.weight(load_logit(a.logits, a.bf16, base + x), x);
-    if (!((double)a.accept_u[(int64_t)b * a.n + acc] * qx * ds.z < px)) break;
   }
-  // The sample: weights z * max(0, p - q) after a rejection, z * p otherwise.
-  const float* qrow = x >= 0 && a.probs ? a.probs + ((int64_t)b * a.n + acc) * V : nullptr;
-  const int per = (V + kThreads - 1) / kThreads;
-  const int j0 = min(V, tid * per), j1 = min(V, j0 + per);
-  double total = 0.0, mine = 0.0;
-  bool residual = x >= 0;
-  auto weight = [&](int j) {
-    const double w = ds.weight(load_logit(a.logits, a.bf16, base + j), j);
-    if (!residual) return w;
-    return fmax(0.0, w - (qrow ? (double)qrow[j] * ds.z : j == x ? ds.z : 0.0));
+  const int ends = (v0 - begin) + (end - v1);
+  for (int i = tid; i < ends; i += kThreads) {
+    const int j = i < v0 - begin ? begin + i : v1 + (i - (v0 - begin));
+    const float x[1] = {load_logit(a.logits, kBf16, base + j)};
+    // One thread may see a later vector before an early single value: the
+    // lower index counts where they tie.
+    if (x[0] == st.m) st.top = min(st.top, j);
+    add_stat<1>(st, x, j, c);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    Stat b;
+    b.m = __shfl_xor_sync(0xffffffffu, st.m, o);
+    b.s = __shfl_xor_sync(0xffffffffu, st.s, o);
+    b.top = __shfl_xor_sync(0xffffffffu, st.top, o);
+    // Both partners add in the same order.
+    if (lane & o) {
+      merge_stat(b, st, c);
+      st = b;
+    } else {
+      merge_stat(st, b, c);
+    }
+  }
+  if (lane == 0) sh[warp] = st;
+  __syncthreads();
+  if (tid == 0) {
+    for (int w = 1; w < kThreads / 32; ++w) merge_stat(st, sh[w], c);
+    st.pad = 0;
+    stats[blockIdx.x] = st;
+  }
+}
+
+// ------------------------------------------------------------ 64 bits
+//
+// e^((l - m) / t): 2^(k / 64) from a table and the rest, at most 1 / 128
+// octave, by the Taylor series to the 4th power (error 4e-14).
+struct Exp64 {
+  const double* table;  // 2^(i / 64), i < 64, in shared memory
+  double m, k64;        // 64 log2(e) / t
+  __device__ __forceinline__ double operator()(float l) const {
+    constexpr double kMagic = 6755399441055744.0;  // 1.5 * 2^52
+    constexpr double a = 0.010830424696249145;     // ln(2) / 64
+    const double t = ((double)l - m) * k64;
+    if (!(t > -64000.0)) return 0.0;  // below 2^-1000; -inf
+    const double kf = t + kMagic;
+    const int k = __double2loint(kf);
+    const double r = t - (kf - kMagic);
+    double p = fma(r, a * a * a * a / 24.0, a * a * a / 6.0);
+    p = fma(r, p, a * a / 2.0);
+    p = fma(r, p, a);
+    p = fma(r, p, 1.0);
+    p *= table[k & 63];
+    return __hiloint2double(__double2hiint(p) + ((k >> 6) << 20), __double2loint(p));
+  }
+};
+
+__device__ __forceinline__ double warp_sum(double v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// What a row's slices say together.
+struct Row {
+  double z;  // its sum of exponentials, relative to m
+  float m;
+  int top;
+  bool greedy;
+};
+__device__ __forceinline__ Row row_of(const Stat* s, int slices, float t) {
+  Row r;
+  r.m = -INFINITY;
+  r.top = 0x7fffffff;
+  for (int i = 0; i < slices; ++i) {
+    const float m = __ldcg(&s[i].m);
+    const int top = __ldcg(&s[i].top);
+    if (m > r.m || (m == r.m && top < r.top)) {
+      r.m = m;
+      r.top = top;
+    }
+  }
+  r.z = 0.0;
+  for (int i = 0; i < slices; ++i) {
+    const float m = __ldcg(&s[i].m);
+    const double d = m == r.m ? 1.0 : (double)ex2((m - r.m) * scale_of(t));
+    r.z += (double)__ldcg(&s[i].s) * d;
+  }
+  if (r.top == 0x7fffffff) r.top = 0;
+  r.greedy = !(t > 0.f) || !(fabs(r.z) <= 1.7e308) || isinf(r.m);
+  return r;
+}
+
+// Cluster of kCluster CTAs per sequence.
+__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kSampleThreads)
+    sample_kernel(const VerifyArgs a, int slices, const Stat* __restrict__ stats) {
+  __shared__ double table[64];
+  __shared__ double part[kSampleWarps];
+  __shared__ double shared_sum[2];  // this CTA's sum, read by the cluster
+  __shared__ int shared_last;
+  __shared__ unsigned verdict[kSampleWarps];  // bits: drafts not plainly accepted
+  __shared__ unsigned close[kSampleWarps];
+  __shared__ int found;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = (int)cluster.block_rank();
+  const int b = blockIdx.x / kCluster, V = a.V, n = a.n;
+  if (tid < 64) table[tid] = exp2((double)tid / 64.0);
+  if (tid == 0) found = 0x7fffffff;
+  rl::pdl_wait();
+  rl::pdl_launch_dependents();
+  const float t = a.temperature[b];
+  const double k64 = 64.0 * 1.4426950408889634 / (double)t;
+  const Stat* st = stats + (int64_t)b * (n + 1) * slices;
+  const int64_t row0 = (int64_t)b * (n + 1);
+  auto draft = [&](int i) {
+    const int x = i < n ? a.drafts[(int64_t)b * n + i] : -1;
+    return (unsigned)x < (unsigned)V ? x : -1;
   };
+  __syncthreads();
+
+  // A draft a thread (n is below 256): accepted, rejected, or too close to say.
+  bool no = false, near = false;
+  if (tid <= n) {
+    const int x = draft(tid);
+    no = true;
+    if (x >= 0) {
+      const Row r = row_of(st + (int64_t)tid * slices, slices, t);
+      const double q = a.probs ? (double)a.probs[((int64_t)b * n + tid) * V + x] : 1.0;
+      const double lhs = (double)a.accept_u[(int64_t)b * n + tid] * q;
+      if (r.greedy) {
+        no = !(lhs < (x == r.top ? 1.0 : 0.0));
+      } else {
+        const double p = Exp64{table, (double)r.m, k64}(load_logit(a.logits, a.bf16, (row0 + tid) * V + x));
+        near = p > 0.0 && fabs(lhs * r.z - p) <= 1e-4 * p;
+        no = !(lhs * r.z < p);
+      }
+    }
+  }
+  const unsigned vno = __ballot_sync(0xffffffffu, no), vnear = __ballot_sync(0xffffffffu, near);
+  if (lane == 0) {
+    verdict[warp] = vno;
+    close[warp] = vnear;
+  }
+  __syncthreads();
+  int acc = 0;
+  for (;; ++acc) {  // up to n: there is no draft n
+    const unsigned bit = 1u << (acc & 31);
+    bool rejected = verdict[acc >> 5] & bit;
+    if (close[acc >> 5] & bit) {
+      // The whole CTA sums this row in 64 bits.
+      const int x = draft(acc);
+      const Row r = row_of(st + (int64_t)acc * slices, slices, t);
+      const Exp64 ex{table, (double)r.m, k64};
+      double z = 0.0;
+      for (int j = tid; j < V; j += kSampleThreads) z += ex(load_logit(a.logits, a.bf16, (row0 + acc) * V + j));
+      z = warp_sum(z);
+      __syncthreads();
+      if (lane == 0) part[warp] = z;
+      __syncthreads();
+      z = 0.0;
+      for (int w = 0; w < kSampleWarps; ++w) z += part[w];
+      const double q = a.probs ? (double)a.probs[((int64_t)b * n + acc) * V + x] : 1.0;
+      rejected = !((double)a.accept_u[(int64_t)b * n + acc] * q * z <
+                   ex(load_logit(a.logits, a.bf16, (row0 + acc) * V + x)));
+    }
+    if (rejected) break;
+  }
+
+  // The token after them: weights z * max(0, p - q) or z * p of row acc. Each
+  // CTA takes an eighth of the vocabulary, each warp a sixteenth of that.
+  const Row r = row_of(st + (int64_t)acc * slices, slices, t);
+  const Exp64 ex{table, (double)r.m, k64};
+  const int x = draft(acc);
+  const int64_t base = (row0 + acc) * V;
+  const float* q = x >= 0 && a.probs ? a.probs + ((int64_t)b * n + acc) * V : nullptr;
+  const int per_cta = (V + kCluster - 1) / kCluster, c0 = min(V, rank * per_cta), c1 = min(V, c0 + per_cta);
+  const int per_warp = (per_cta + kSampleWarps - 1) / kSampleWarps;
+  const int j0 = min(c1, c0 + warp * per_warp), j1 = min(c1, j0 + per_warp);
+  bool residual = x >= 0;
+  double z = 1.0;
+  if (residual && q && !r.greedy) {
+    double s = 0.0;
+    for (int j = j0 + lane; j < j1; j += 32) s += ex(load_logit(a.logits, a.bf16, base + j));
+    s = warp_sum(s);
+    __syncthreads();
+    if (lane == 0) part[warp] = s;
+    __syncthreads();
+    if (tid == 0) {
+      s = 0.0;
+      for (int w = 0; w < kSampleWarps; ++w) s += part[w];
+      shared_sum[1] = s;
+    }
+    cluster.sync();
+    z = 0.0;
+    for (int c = 0; c < kCluster; ++c) z += *cluster.map_shared_rank(&shared_sum[1], c);
+  }
+  auto weight = [&](int j) {
+    const double w = r.greedy ? (j == r.top ? 1.0 : 0.0) : ex(load_logit(a.logits, a.bf16, base + j));
+    if (!residual) return w;
+    return fmax(0.0, w - (q ? (double)q[j] * z : j == x ? w : 0.0));
+  };
+  double mine, before, total;
   for (;;) {
     mine = 0.0;
-    for (int j = j0; j < j1; ++j) mine += weight(j);
+    int last = -1;
+    for (int j = j0 + lane; j < j1; j += 32) {
+      const double w = weight(j);
+      mine += w;
+      if (w > 0.0) last = j;
+    }
+    mine = warp_sum(mine);
+    last = __reduce_max_sync(0xffffffffu, last);
     __syncthreads();
-    scan[tid] = mine;
+    if (tid == 0) shared_last = -1;
+    if (lane == 0) part[warp] = mine;
     __syncthreads();
-    total = 0.0;
-    for (int i = 0; i < kThreads; ++i) total += scan[i];
+    if (lane == 0) atomicMax(&shared_last, last);
+    if (tid == 0) {
+      double s = 0.0;
+      for (int w = 0; w < kSampleWarps; ++w) s += part[w];
+      shared_sum[0] = s;
+    }
+    cluster.sync();
+    total = before = 0.0;
+    for (int c = 0; c < kCluster; ++c) {
+      const double s = *cluster.map_shared_rank(&shared_sum[0], c);
+      if (c < rank) before += s;
+      total += s;
+    }
     if (total > 0.0 || !residual) break;
     residual = false;  // p == q: nothing is left over
+    cluster.sync();    // every CTA has read the sums
   }
-  double before = 0.0;
-  for (int i = 0; i < tid; ++i) before += scan[i];
+  // The first token whose cumulative weight exceeds the target lies in the
+  // first part (CTA, then warp) whose end does.
   const double target = (double)a.sample_u[b] * total;
-  // The first token whose cumulative weight exceeds the target; the last one
-  // with weight where rounding leaves none.
-  if (tid == 0) found = 0x7fffffff;
-  __syncthreads();
-  double c = before;
-  int hit = 0x7fffffff, last = -1;
-  for (int j = j0; j < j1; ++j) {
-    const double w = weight(j);
-    if (w > 0.0) {
-      c += w;
-      last = j;
-      if (c > target && hit == 0x7fffffff) hit = j;
+  bool owner = shared_sum[0] > 0.0 && before + shared_sum[0] > target;
+  if (owner && rank > 0) {  // no earlier one
+    double c = 0.0;
+    for (int i = 0; i < rank; ++i) {
+      const double s = *cluster.map_shared_rank(&shared_sum[0], i);
+      c += s;
+      if (s > 0.0 && c > target) owner = false;
     }
   }
-  atomicMin(&found, hit);
-  const long long lastpos = block_reduce((long long)last, sl, [](long long p, long long q) { return p > q ? p : q; });
-  __syncthreads();
-  for (int i = tid; i <= a.n; i += kThreads)
-    a.tokens[(int64_t)b * (a.n + 1) + i] = i < acc   ? a.drafts[(int64_t)b * a.n + i]
-                                           : i > acc ? -1
-                                           : found != 0x7fffffff ? found
-                                                                 : (int)(lastpos < 0 ? ds.top : lastpos);
-  if (tid == 0) a.accepted[b] = acc;
+  if (owner) {
+    double c = before;
+    int w0 = -1;
+    double start = 0.0;
+    for (int w = 0; w < kSampleWarps; ++w) {
+      if (w0 < 0 && part[w] > 0.0 && (c + part[w] > target)) {
+        w0 = w;
+        start = c;
+      }
+      c += part[w];
+    }
+    if (w0 < 0)  // the parts' sums round below their total: the last with weight
+      for (int w = 0; w < kSampleWarps; ++w)
+        if (part[w] > 0.0) w0 = w;
+    if (warp == w0) {
+      int hit = 0x7fffffff, last = -1;
+      for (int j = j0; j < j1; j += 32) {
+        const double w = j + lane < j1 ? weight(j + lane) : 0.0;
+        double s = w;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const double y = __shfl_up_sync(0xffffffffu, s, o);
+          if (lane >= o) s += y;
+        }
+        const unsigned over = __ballot_sync(0xffffffffu, w > 0.0 && start + s > target);
+        const unsigned some = __ballot_sync(0xffffffffu, w > 0.0);
+        if (over) {
+          hit = j + __ffs(over) - 1;
+          break;
+        }
+        if (some) last = j + 31 - __clz(some);
+        start += __shfl_sync(0xffffffffu, s, 31);
+      }
+      if (lane == 0) a.tokens[row0 + acc] = hit != 0x7fffffff ? hit : last;
+    }
+  }
+  // A number of 1 or more, or none (NaN): the last token with weight.
+  if (rank == 0 && !(total > target)) {
+    int last = -1;
+    for (int c = 0; c < kCluster; ++c) last = max(last, *cluster.map_shared_rank(&shared_last, c));
+    if (tid == 0) a.tokens[row0 + acc] = last < 0 ? r.top : last;
+  }
+  if (rank == 0) {
+    for (int i = tid; i <= n; i += kSampleThreads)
+      if (i != acc) a.tokens[row0 + i] = i < acc ? a.drafts[(int64_t)b * n + i] : -1;
+    if (tid == 0) a.accepted[b] = acc;
+  }
+  cluster.sync();  // no CTA leaves while another reads its sums
+}
+
+// Slices of a row: as many as fill the GPU, of 1024 to 16384 tokens.
+int slices_of(int num_sms, int64_t rows, int V) {
+  const int most = (V + 1023) / 1024, least = (V + 16383) / 16384;
+  const int64_t want = (8ll * num_sms + rows - 1) / std::max<int64_t>(rows, 1);
+  return (int)std::max<int64_t>(least, std::min<int64_t>(want, most));
 }
 
 }  // namespace
@@ -163,8 +448,9 @@ __global__ void __launch_bounds__(kThreads) verify_draft_kernel(VerifyArgs a) {
 extern "C" {
 
 uint64_t riallm_cuda_verify_draft_workspace(const riallm_ctx* ctx, int32_t B, int32_t n, int32_t V) {
-  (void)ctx, (void)B, (void)n, (void)V;
-  return 0;
+  if (!ctx || B <= 0 || n < 0 || V <= 0) return 0;
+  const int64_t rows = (int64_t)B * (n + 1);
+  return (uint64_t)rows * slices_of(ctx->num_sms, rows, V) * sizeof(Stat);
 }
 
 int32_t riallm_cuda_verify_draft(riallm_ctx* ctx, const void* logits, int32_t logits_dtype, const int32_t* draft_tokens,
@@ -172,19 +458,36 @@ int32_t riallm_cuda_verify_draft(riallm_ctx* ctx, const void* logits, int32_t lo
                                  const float* sample_u, int32_t B, int32_t n, int32_t V, int32_t* tokens,
                                  int32_t* accepted, void* workspace, uint64_t workspace_bytes, void* stream) {
   const char* what = "verify_draft";
-  if (B < 0 || n < 0 || n > 255 || V <= 0)
+  if (B < 0 || n < 0 || n > 255 || V <= 0 || V > (1 << 30))
     return rl::refuse(ctx, RIALLM_ERR_CONFIG, what, "bad dimensions (at most 255 drafted tokens)");
   if (logits_dtype != RIALLM_DTYPE_F32 && logits_dtype != RIALLM_DTYPE_BF16)
     return rl::refuse(ctx, RIALLM_ERR_CONFIG, what, "logits must be float32 or bf16");
+  if ((int64_t)B * (n + 1) * ((V + 1023) / 1024) > INT32_MAX)
+    return rl::refuse(ctx, RIALLM_ERR_CONFIG, what, "too many logits");
   if (ctx && B == 0) return RIALLM_OK;
   if (!ctx || !logits || !temperature || !sample_u || !tokens || !accepted || (n > 0 && (!draft_tokens || !accept_u)))
     return rl::refuse(ctx, RIALLM_ERR_INVALID, what, "NULL argument");
-  (void)workspace, (void)workspace_bytes;
+  if (reinterpret_cast<uintptr_t>(logits) & 15)
+    return rl::refuse(ctx, RIALLM_ERR_INVALID, what, "logits must be 16-byte aligned");
+  const int64_t rows = (int64_t)B * (n + 1);
+  const int slices = slices_of(ctx->num_sms, rows, V);
+  if (!workspace || workspace_bytes < (uint64_t)rows * slices * sizeof(Stat) ||
+      (reinterpret_cast<uintptr_t>(workspace) & 15))
+    return rl::refuse(ctx, RIALLM_ERR_MEMORY, what, "workspace missing, too small or not 16-byte aligned");
   return rl::guarded(ctx, [&]() -> int32_t {
     const VerifyArgs a{logits, logits_dtype == RIALLM_DTYPE_BF16, draft_tokens, draft_probs, temperature, accept_u,
                        sample_u, n, V, tokens, accepted};
+    Stat* stats = static_cast<Stat*>(workspace);
+    const int slice = (V + slices - 1) / slices;
+    const cudaStream_t st = (cudaStream_t)stream;
+    if (int s = rl::launched(ctx, what,
+                             rl::launch_pdl(a.bf16 ? stats_kernel<true> : stats_kernel<false>,
+                                            dim3((unsigned)rows * slices), dim3(kThreads), 0, st, a, slices, slice,
+                                            stats)))
+      return s;
     return rl::launched(ctx, what,
-                        rl::launch_pdl(verify_draft_kernel, dim3(B), dim3(kThreads), 0, (cudaStream_t)stream, a));
+                        rl::launch_pdl(sample_kernel, dim3(B * kCluster), dim3(kSampleThreads), 0, st, a, slices,
+                                       static_cast<const Stat*>(stats)));
   });
 }
 
