@@ -38,12 +38,10 @@ namespace cg = cooperative_groups;
 namespace {
 
 constexpr int kThreads = 256, kCluster = 8, kSampleThreads = 512, kSampleWarps = kSampleThreads / 32;
+constexpr int kBatch = 8;  // loads a lane has in flight
 
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
+using rl::ex2;
+
 __device__ __forceinline__ float load_logit(const void* x, bool bf16, int64_t i) {
   return bf16 ? __uint_as_float((uint32_t)static_cast<const uint16_t*>(x)[i] << 16) : static_cast<const float*>(x)[i];
 }
@@ -74,10 +72,11 @@ __device__ __forceinline__ float scale_of(float t) {
 
 // Adds N values from index j on.
 template <int N>
-__device__ __forceinline__ void add_stat(Stat& st, const float (&x)[N], int j, float c) {
+__device__ __forceinline__ void add_stat(Stat& st, float (&x)[N], int j, float c) {
   float mx = x[0];
 #pragma unroll
-  for (int e = 1; e < N; ++e) mx = fmaxf(mx, x[e]);
+  for (int e = 1; e + 1 < N; e += 2) mx = rl::max3(mx, x[e], x[e + 1]);
+  if (N > 1) mx = fmaxf(mx, x[N - 1]);
   if (mx > st.m) {
     int at = 0;
 #pragma unroll
@@ -88,10 +87,18 @@ __device__ __forceinline__ void add_stat(Stat& st, const float (&x)[N], int j, f
     st.top = j + at;
   }
   const float base = st.m == -INFINITY ? 0.f : st.m;
-  float s = 0.f;
+  if (N == 1) {
+    st.s += ex2((x[0] - base) * c);
+    return;
+  }
+  float s0 = 0.f, s1 = 0.f;
 #pragma unroll
-  for (int e = 0; e < N; ++e) s += ex2((x[e] - base) * c);
-  st.s += s;
+  for (int e = 0; e + 1 < N; e += 2) {
+    rl::add_f32x2(x[e], x[e + 1], -base, -base);
+    rl::mul_f32x2(x[e], x[e + 1], c, c);
+    rl::add_f32x2(s0, s1, ex2(x[e]), ex2(x[e + 1]));
+  }
+  st.s += s0 + s1;
 }
 // The two slices' statistics together; the lower index where they tie.
 __device__ __forceinline__ void merge_stat(Stat& a, const Stat& b, float c) {
@@ -120,11 +127,18 @@ __global__ void __launch_bounds__(kThreads) stats_kernel(const VerifyArgs a, int
   Stat st{-INFINITY, 0.f, 0x7fffffff, 0};
   const uint4* vec = reinterpret_cast<const uint4*>(static_cast<const char*>(a.logits) + (base + v0) * (kBf16 ? 2 : 4));
   const int nv = (v1 - v0) / N;
+  uint4 next[4];
+  auto fetch = [&](int i) {
+#pragma unroll
+    for (int y = 0; y < 4; ++y)
+      if (i + y * kThreads < nv) next[y] = __ldcs(vec + i + y * kThreads);
+  };
+  fetch(tid);
   for (int i = tid; i < nv; i += 4 * kThreads) {
     uint4 w[4];
 #pragma unroll
-    for (int y = 0; y < 4; ++y)
-      if (i + y * kThreads < nv) w[y] = __ldcs(vec + i + y * kThreads);
+    for (int y = 0; y < 4; ++y) w[y] = next[y];
+    fetch(i + 4 * kThreads);
 #pragma unroll
     for (int y = 0; y < 4; ++y) {
       if (i + y * kThreads >= nv) break;
@@ -145,7 +159,7 @@ __global__ void __launch_bounds__(kThreads) stats_kernel(const VerifyArgs a, int
   const int ends = (v0 - begin) + (end - v1);
   for (int i = tid; i < ends; i += kThreads) {
     const int j = i < v0 - begin ? begin + i : v1 + (i - (v0 - begin));
-    const float x[1] = {load_logit(a.logits, kBf16, base + j)};
+    float x[1] = {load_logit(a.logits, kBf16, base + j)};
     // One thread may see a later vector before an early single value: the
     // lower index counts where they tie.
     if (x[0] == st.m) st.top = min(st.top, j);
@@ -204,34 +218,35 @@ __device__ __forceinline__ double warp_sum(double v) {
   return v;
 }
 
-// What a row's slices say together.
+// What a row's slices say together: its sum of exponentials relative to m, its
+// maximum and where it is. By a warp, a slice a lane.
 struct Row {
-  double z;  // its sum of exponentials, relative to m
+  double z;
   float m;
-  int top;
-  bool greedy;
+  int top;  // negative where all of p lies on ~top
 };
 __device__ __forceinline__ Row row_of(const Stat* s, int slices, float t) {
-  Row r;
-  r.m = -INFINITY;
-  r.top = 0x7fffffff;
-  for (int i = 0; i < slices; ++i) {
-    const float m = __ldcg(&s[i].m);
-    const int top = __ldcg(&s[i].top);
-    if (m > r.m || (m == r.m && top < r.top)) {
-      r.m = m;
-      r.top = top;
-    }
+  const int lane = threadIdx.x & 31;
+  const float c = scale_of(t);
+  Stat st{-INFINITY, 0.f, 0x7fffffff, 0};
+  double z = 0.0;
+  for (int i = lane; i < slices; i += 32) {
+    const uint4 u = __ldcg(reinterpret_cast<const uint4*>(s + i));
+    const float m = __uint_as_float(u.x), mn = fmaxf(st.m, m), base = mn == -INFINITY ? 0.f : mn;
+    st.top = m > st.m ? (int)u.z : m < st.m ? st.top : min(st.top, (int)u.z);
+    z = z * (double)(st.m == mn ? 1.f : ex2((st.m - base) * c)) +
+        (double)__uint_as_float(u.y) * (double)(m == mn ? 1.f : ex2((m - base) * c));
+    st.m = mn;
   }
-  r.z = 0.0;
-  for (int i = 0; i < slices; ++i) {
-    const float m = __ldcg(&s[i].m);
-    const double d = m == r.m ? 1.0 : (double)ex2((m - r.m) * scale_of(t));
-    r.z += (double)__ldcg(&s[i].s) * d;
-  }
-  if (r.top == 0x7fffffff) r.top = 0;
-  r.greedy = !(t > 0.f) || !(fabs(r.z) <= 1.7e308) || isinf(r.m);
-  return r;
+  float M = st.m;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+  int top = __reduce_min_sync(0xffffffffu, st.m == M ? st.top : 0x7fffffff);
+  const float base = M == -INFINITY ? 0.f : M;
+  z = warp_sum(z * (double)(st.m == M ? 1.f : ex2((st.m - base) * c)));
+  if (top == 0x7fffffff) top = 0;
+  const bool greedy = !(t > 0.f) || !(fabs(z) <= 1.7e308) || isinf(M);
+  return Row{z, M, greedy ? ~top : top};
 }
 
 // Cluster of kCluster CTAs per sequence.
@@ -243,12 +258,11 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kSampleThread
   __shared__ int shared_last;
   __shared__ unsigned verdict[kSampleWarps];  // bits: drafts not plainly accepted
   __shared__ unsigned close[kSampleWarps];
-  __shared__ int found;
+  __shared__ Row rows[256];
   cg::cluster_group cluster = cg::this_cluster();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = (int)cluster.block_rank();
   const int b = blockIdx.x / kCluster, V = a.V, n = a.n;
   if (tid < 64) table[tid] = exp2((double)tid / 64.0);
-  if (tid == 0) found = 0x7fffffff;
   rl::pdl_wait();
   rl::pdl_launch_dependents();
   const float t = a.temperature[b];
@@ -259,6 +273,10 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kSampleThread
     const int x = i < n ? a.drafts[(int64_t)b * n + i] : -1;
     return (unsigned)x < (unsigned)V ? x : -1;
   };
+  for (int i = warp; i <= n; i += kSampleWarps) {
+    const Row r = row_of(st + (int64_t)i * slices, slices, t);
+    if (lane == 0) rows[i] = r;
+  }
   __syncthreads();
 
   // A draft a thread (n is below 256): accepted, rejected, or too close to say.
@@ -267,11 +285,11 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kSampleThread
     const int x = draft(tid);
     no = true;
     if (x >= 0) {
-      const Row r = row_of(st + (int64_t)tid * slices, slices, t);
+      const Row r = rows[tid];
       const double q = a.probs ? (double)a.probs[((int64_t)b * n + tid) * V + x] : 1.0;
       const double lhs = (double)a.accept_u[(int64_t)b * n + tid] * q;
-      if (r.greedy) {
-        no = !(lhs < (x == r.top ? 1.0 : 0.0));
+      if (r.top < 0) {
+        no = !(lhs < (x == ~r.top ? 1.0 : 0.0));
       } else {
         const double p = Exp64{table, (double)r.m, k64}(load_logit(a.logits, a.bf16, (row0 + tid) * V + x));
         near = p > 0.0 && fabs(lhs * r.z - p) <= 1e-4 * p;
@@ -292,9 +310,9 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kSampleThread
     if (close[acc >> 5] & bit) {
       // The whole CTA sums this row in 64 bits.
       const int x = draft(acc);
-      const Row r = row_of(st + (int64_t)acc * slices, slices, t);
-      const Exp64 ex{table, (double)r.m, k64};
+      const Exp64 ex{table, (double)rows[acc].m, k64};
       double z = 0.0;
+#pragma unroll 4
       for (int j = tid; j < V; j += kSampleThreads) z += ex(load_logit(a.logits, a.bf16, (row0 + acc) * V + j));
       z = warp_sum(z);
       __syncthreads();
@@ -311,8 +329,9 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kSampleThread
 
   // The token after them: weights z * max(0, p - q) or z * p of row acc. Each
   // CTA takes an eighth of the vocabulary, each warp a sixteenth of that.
-  const Row r = row_of(st + (int64_t)acc * slices, slices, t);
-  const Exp64 ex{table, (double)r.m, k64};
+  const bool greedy = rows[acc].top < 0;
+  const int top = greedy ? ~rows[acc].top : rows[acc].top;
+  const Exp64 ex{table, (double)rows[acc].m, k64};
   const int x = draft(acc);
   const int64_t base = (row0 + acc) * V;
   const float* q = x >= 0 && a.probs ? a.probs + ((int64_t)b * n + acc) * V : nullptr;
@@ -321,9 +340,16 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kSampleThread
   const int j0 = min(c1, c0 + warp * per_warp), j1 = min(c1, j0 + per_warp);
   bool residual = x >= 0;
   double z = 1.0;
-  if (residual && q && !r.greedy) {
+  if (residual && q && !greedy) {
     double s = 0.0;
-    for (int j = j0 + lane; j < j1; j += 32) s += ex(load_logit(a.logits, a.bf16, base + j));
+    for (int j = j0 + lane; j < j1; j += 32 * kBatch) {
+      float l[kBatch];
+#pragma unroll
+      for (int e = 0; e < kBatch; ++e)
+        l[e] = j + 32 * e < j1 ? load_logit(a.logits, a.bf16, base + j + 32 * e) : -INFINITY;
+#pragma unroll
+      for (int e = 0; e < kBatch; ++e) s += ex(l[e]);
+    }
     s = warp_sum(s);
     __syncthreads();
     if (lane == 0) part[warp] = s;
@@ -337,19 +363,30 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kSampleThread
     z = 0.0;
     for (int c = 0; c < kCluster; ++c) z += *cluster.map_shared_rank(&shared_sum[1], c);
   }
-  auto weight = [&](int j) {
-    const double w = r.greedy ? (j == r.top ? 1.0 : 0.0) : ex(load_logit(a.logits, a.bf16, base + j));
+  auto weight = [&](int j, float l, float qj) {
+    const double w = greedy ? (j == top ? 1.0 : 0.0) : ex(l);
     if (!residual) return w;
-    return fmax(0.0, w - (q ? (double)q[j] * z : j == x ? w : 0.0));
+    return fmax(0.0, w - (q ? (double)qj * z : j == x ? w : 0.0));
   };
   double mine, before, total;
   for (;;) {
     mine = 0.0;
     int last = -1;
-    for (int j = j0 + lane; j < j1; j += 32) {
-      const double w = weight(j);
-      mine += w;
-      if (w > 0.0) last = j;
+    for (int j = j0 + lane; j < j1; j += 32 * kBatch) {
+      float l[kBatch], qj[kBatch];
+#pragma unroll
+      for (int e = 0; e < kBatch; ++e) {
+        const bool in = j + 32 * e < j1;
+        l[e] = in ? load_logit(a.logits, a.bf16, base + j + 32 * e) : 0.f;
+        qj[e] = in && q ? q[j + 32 * e] : 0.f;
+      }
+#pragma unroll
+      for (int e = 0; e < kBatch; ++e) {
+        if (j + 32 * e >= j1) break;
+        const double w = weight(j + 32 * e, l[e], qj[e]);
+        mine += w;
+        if (w > 0.0) last = j + 32 * e;
+      }
     }
     mine = warp_sum(mine);
     last = __reduce_max_sync(0xffffffffu, last);
@@ -402,8 +439,17 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kSampleThread
         if (part[w] > 0.0) w0 = w;
     if (warp == w0) {
       int hit = 0x7fffffff, last = -1;
+      float l = 0.f, qj = 0.f;
+      auto fetch = [&](int j) {
+        if (j < j1) {
+          l = load_logit(a.logits, a.bf16, base + j);
+          if (q) qj = q[j];
+        }
+      };
+      fetch(j0 + lane);
       for (int j = j0; j < j1; j += 32) {
-        const double w = j + lane < j1 ? weight(j + lane) : 0.0;
+        const double w = j + lane < j1 ? weight(j + lane, l, qj) : 0.0;
+        fetch(j + 32 + lane);
         double s = w;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -426,7 +472,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kSampleThread
   if (rank == 0 && !(total > target)) {
     int last = -1;
     for (int c = 0; c < kCluster; ++c) last = max(last, *cluster.map_shared_rank(&shared_last, c));
-    if (tid == 0) a.tokens[row0 + acc] = last < 0 ? r.top : last;
+    if (tid == 0) a.tokens[row0 + acc] = last < 0 ? top : last;
   }
   if (rank == 0) {
     for (int i = tid; i <= n; i += kSampleThreads)
@@ -436,9 +482,9 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kSampleThread
   cluster.sync();  // no CTA leaves while another reads its sums
 }
 
-// Slices of a row: as many as fill the GPU, of 1024 to 16384 tokens.
+// Slices of a row: as many as fill the GPU, of 1024 to 65536 tokens.
 int slices_of(int num_sms, int64_t rows, int V) {
-  const int most = (V + 1023) / 1024, least = (V + 16383) / 16384;
+  const int most = (V + 1023) / 1024, least = (V + 65535) / 65536;
   const int64_t want = (8ll * num_sms + rows - 1) / std::max<int64_t>(rows, 1);
   return (int)std::max<int64_t>(least, std::min<int64_t>(want, most));
 }
