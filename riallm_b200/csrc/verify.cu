@@ -16,29 +16,28 @@
 // Temperature 0 (and a row whose softmax is undefined: a NaN, +inf, or -inf
 // throughout) puts all of p_i on the first maximum.
 //
-// Two launches:
-//   stats_kernel  : every row's maximum, where it is, and its sum of
-//                   exponentials in float32, a slice of a row per CTA; bound
-//                   by reading the logits once.
-//   sample_kernel : a cluster of 8 CTAs per sequence finds the first
-//                   rejection (a comparison that float32 sums leave within
-//                   1e-4 of equality is made again with 64-bit ones), then
-//                   goes over the one row that the token comes from, in 64
-//                   bits, an eighth of the vocabulary per CTA.
-#include <cooperative_groups.h>
-
+// Three launches:
+//   stats_kernel : every row's maximum and sum of exponentials in float32, a
+//                  slice of a row per CTA; bound by reading the logits once
+//                  and, nearly, by the exponentials;
+//   weigh_kernel : finds a sequence's first rejection (a comparison that
+//                  float32 sums leave within 1e-4 of equality is made again
+//                  with 64-bit ones) and goes over the one row that the token
+//                  comes from, in 64 bits, a chunk of the vocabulary per CTA;
+//   pick_kernel  : the chunks' weights after the draft's distribution is taken
+//                  off; a sequence's last CTA finds the token.
+// (A cluster of CTAs per sequence in place of the last two takes 280 us for
+// 128 sequences of 128001 tokens: its fixed cost, 10 us, comes 8 times over.)
 #include <algorithm>
 #include <cmath>
 
 #include "common.cuh"
 #include "internal.h"
 
-namespace cg = cooperative_groups;
-
 namespace {
 
-constexpr int kThreads = 256, kCluster = 8, kSampleThreads = 512, kSampleWarps = kSampleThreads / 32;
-constexpr int kBatch = 8;  // loads a lane has in flight
+constexpr int kThreads = 256, kWarps = kThreads / 32;
+constexpr int kBatch = 8;  // loads of an array that a thread has in flight
 
 using rl::ex2;
 
@@ -59,8 +58,30 @@ struct VerifyArgs {
   int* accepted;
 };
 
-// Of a slice of a row: its maximum (NaN left out), the lowest index that
-// holds it, and the sum of 2^((x - max) c), NaN where the softmax is undefined.
+struct Stat;
+// What the first rejection of a sequence comes to.
+struct Verdict {
+  int acc;    // accepted drafts: the token comes from row acc
+  int draft;  // the rejected draft, or -1
+  float m;    // the row's maximum
+  int done;   // the row's p lies on one token, which has been written
+};
+// The workspace: statistics of the rows' slices; per sequence and chunk the
+// sum of exponentials, the sum of weights and the last token with weight; per
+// sequence the verdict and a count of finished chunks.
+struct Space {
+  Stat* stats;
+  double* z;
+  double* w;
+  int* last;
+  Verdict* verdict;
+  unsigned* done;
+  int slices, slice, chunks, chunk;
+};
+
+// Of a slice of a row: its maximum (NaN left out); the sum of
+// 2^((x - max) c), NaN where the softmax is undefined; at temperature 0 the
+// lowest index that holds the maximum, and no sum.
 struct Stat {
   float m, s;
   int top, pad;
@@ -70,121 +91,137 @@ __device__ __forceinline__ float scale_of(float t) {
   return t > 0.f ? fminf(fmaxf(1.4426950408889634f / t, 1e-30f), 1e30f) : 1.f;
 }
 
-// Adds N values from index j on.
-template <int N>
-__device__ __forceinline__ void add_stat(Stat& st, float (&x)[N], int j, float c) {
-  float mx = x[0];
+// A thread's part of a slice. Its sum is relative to `base`, at most 60
+// octaves below the maximum, so that a new maximum seldom costs more than
+// being noted.
+struct Part {
+  float m = -INFINITY, base = 0.f, s0 = 0.f, s1 = 0.f;
+  int top = 0x7fffffff;
+  bool begun = false;
+  template <int N>
+  __device__ __forceinline__ void sum(float (&x)[N], float c) {
+    float mx = x[0];
 #pragma unroll
-  for (int e = 1; e + 1 < N; e += 2) mx = rl::max3(mx, x[e], x[e + 1]);
-  if (N > 1) mx = fmaxf(mx, x[N - 1]);
-  if (mx > st.m) {
-    int at = 0;
+    for (int e = 1; e + 1 < N; e += 2) mx = rl::max3(mx, x[e], x[e + 1]);
+    m = N > 1 ? rl::max3(m, mx, x[N - 1]) : fmaxf(m, mx);
+    if ((m - base) * c > 60.f || !begun) {  // -inf and NaN leave base as it is
+      begun = m > -INFINITY;
+      const float b = begun ? m : 0.f, f = ex2((base - b) * c);
+      s0 *= f;
+      s1 *= f;
+      base = b;
+    }
+    if (N == 1) {
+      s0 += ex2((x[0] - base) * c);
+    } else {
 #pragma unroll
-    for (int e = N - 1; e >= 0; --e)
-      if (x[e] == mx) at = e;
-    st.s *= ex2((st.m - mx) * c);
-    st.m = mx;
-    st.top = j + at;
+      for (int e = 0; e + 1 < N; e += 2) {
+        rl::add_f32x2(x[e], x[e + 1], -base, -base);
+        rl::mul_f32x2(x[e], x[e + 1], c, c);
+        rl::add_f32x2(s0, s1, ex2(x[e]), ex2(x[e + 1]));
+      }
+    }
   }
-  const float base = st.m == -INFINITY ? 0.f : st.m;
-  if (N == 1) {
-    st.s += ex2((x[0] - base) * c);
-    return;
-  }
-  float s0 = 0.f, s1 = 0.f;
+  template <int N>
+  __device__ __forceinline__ void first(const float (&x)[N], int j) {
 #pragma unroll
-  for (int e = 0; e + 1 < N; e += 2) {
-    rl::add_f32x2(x[e], x[e + 1], -base, -base);
-    rl::mul_f32x2(x[e], x[e + 1], c, c);
-    rl::add_f32x2(s0, s1, ex2(x[e]), ex2(x[e + 1]));
+    for (int e = 0; e < N; ++e)
+      if (x[e] > m || (x[e] == m && j + e < top)) {
+        m = x[e];
+        top = j + e;
+      }
   }
-  st.s += s0 + s1;
-}
-// The two slices' statistics together; the lower index where they tie.
-__device__ __forceinline__ void merge_stat(Stat& a, const Stat& b, float c) {
-  const float m = fmaxf(a.m, b.m), base = m == -INFINITY ? 0.f : m;
-  a.top = a.m > b.m ? a.top : b.m > a.m ? b.top : min(a.top, b.top);
-  a.s = a.s * (a.m == m ? 1.f : ex2((a.m - base) * c)) + b.s * (b.m == m ? 1.f : ex2((b.m - base) * c));
-  a.m = m;
-}
+};
 
-// A CTA per slice of a row, row by row. 16 bytes a load where the row's place allows, four loads
-// in flight a thread.
+// A CTA per slice of a row, row by row. 16 bytes a load where the row's place
+// allows, four loads of a thread in flight and four at work.
 template <bool kBf16>
-__global__ void __launch_bounds__(kThreads) stats_kernel(const VerifyArgs a, int slices, int slice, Stat* __restrict__ stats) {
+__global__ void __launch_bounds__(kThreads)
+    stats_kernel(const VerifyArgs a, const Space ws) {
   constexpr int N = kBf16 ? 8 : 4;
-  __shared__ Stat sh[kThreads / 32];
+  __shared__ float sh_m[kWarps], sh_s[kWarps];
+  __shared__ int sh_top[kWarps];
   rl::pdl_wait();
   rl::pdl_launch_dependents();
-  const int row = blockIdx.x / slices;
+  const int row = blockIdx.x / ws.slices, slice = ws.slice;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int begin = min(a.V, (int)(blockIdx.x - row * slices) * slice), end = min(a.V, begin + slice);
-  const float c = scale_of(a.temperature[row / (a.n + 1)]);
+  const int begin = min(a.V, (int)(blockIdx.x - row * ws.slices) * slice), end = min(a.V, begin + slice);
+  const float temp = a.temperature[row / (a.n + 1)], c = scale_of(temp);
+  const bool greedy = !(temp > 0.f);
   const int64_t base = (int64_t)row * a.V;
   // Whole vectors of the slice: [v0, v1) as row indices, the rest one by one.
   const int skew = (int)((base + begin) & (N - 1));
   const int v0 = min(end, begin + (skew ? N - skew : 0)), v1 = v0 + (end - v0) / N * N;
-  Stat st{-INFINITY, 0.f, 0x7fffffff, 0};
   const uint4* vec = reinterpret_cast<const uint4*>(static_cast<const char*>(a.logits) + (base + v0) * (kBf16 ? 2 : 4));
   const int nv = (v1 - v0) / N;
+  Part part;
   uint4 next[4];
   auto fetch = [&](int i) {
 #pragma unroll
     for (int y = 0; y < 4; ++y)
       if (i + y * kThreads < nv) next[y] = __ldcs(vec + i + y * kThreads);
   };
-  fetch(tid);
-  for (int i = tid; i < nv; i += 4 * kThreads) {
-    uint4 w[4];
+  auto vectors = [&](auto&& use) {
+    fetch(tid);
+    for (int i = tid; i < nv; i += 4 * kThreads) {
+      uint4 w[4];
 #pragma unroll
-    for (int y = 0; y < 4; ++y) w[y] = next[y];
-    fetch(i + 4 * kThreads);
+      for (int y = 0; y < 4; ++y) w[y] = next[y];
+      fetch(i + 4 * kThreads);
 #pragma unroll
-    for (int y = 0; y < 4; ++y) {
-      if (i + y * kThreads >= nv) break;
-      float x[N];
-      const uint32_t* u = reinterpret_cast<const uint32_t*>(&w[y]);
+      for (int y = 0; y < 4; ++y) {
+        if (i + y * kThreads >= nv) break;
+        float x[N];
+        const uint32_t* u = reinterpret_cast<const uint32_t*>(&w[y]);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if (kBf16) {
-          x[(2 * e) % N] = __uint_as_float(u[e] << 16);
-          x[(2 * e + 1) % N] = __uint_as_float(u[e] & 0xffff0000u);
-        } else {
-          x[e] = __uint_as_float(u[e]);
+        for (int e = 0; e < 4; ++e) {
+          if (kBf16) {
+            x[(2 * e) % N] = __uint_as_float(u[e] << 16);
+            x[(2 * e + 1) % N] = __uint_as_float(u[e] & 0xffff0000u);
+          } else {
+            x[e] = __uint_as_float(u[e]);
+          }
         }
+        use(x, v0 + (i + y * kThreads) * N);
       }
-      add_stat<N>(st, x, v0 + (i + y * kThreads) * N, c);
     }
-  }
-  const int ends = (v0 - begin) + (end - v1);
-  for (int i = tid; i < ends; i += kThreads) {
-    const int j = i < v0 - begin ? begin + i : v1 + (i - (v0 - begin));
-    float x[1] = {load_logit(a.logits, kBf16, base + j)};
-    // One thread may see a later vector before an early single value: the
-    // lower index counts where they tie.
-    if (x[0] == st.m) st.top = min(st.top, j);
-    add_stat<1>(st, x, j, c);
-  }
+    const int ends = (v0 - begin) + (end - v1);
+    for (int i = tid; i < ends; i += kThreads) {
+      const int j = i < v0 - begin ? begin + i : v1 + (i - (v0 - begin));
+      float x[1] = {load_logit(a.logits, kBf16, base + j)};
+      use(x, j);
+    }
+  };
+  if (greedy)
+    vectors([&](auto& x, int j) { part.first(x, j); });
+  else
+    vectors([&](auto& x, int) { part.sum(x, c); });
+  float m = part.m;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    Stat b;
-    b.m = __shfl_xor_sync(0xffffffffu, st.m, o);
-    b.s = __shfl_xor_sync(0xffffffffu, st.s, o);
-    b.top = __shfl_xor_sync(0xffffffffu, st.top, o);
-    // Both partners add in the same order.
-    if (lane & o) {
-      merge_stat(b, st, c);
-      st = b;
-    } else {
-      merge_stat(st, b, c);
-    }
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if (lane == 0) sh_m[warp] = m;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) m = fmaxf(m, sh_m[w]);
+  const float ref = m == -INFINITY ? 0.f : m;
+  // What has not begun holds 0, or NaN, and so it stays.
+  float s = (part.s0 + part.s1) * (part.begun ? ex2((part.base - ref) * c) : 1.f);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  const int top = __reduce_min_sync(0xffffffffu, part.m == m ? part.top : 0x7fffffff);
+  if (lane == 0) {
+    sh_s[warp] = s;
+    sh_top[warp] = top;
   }
-  if (lane == 0) sh[warp] = st;
   __syncthreads();
   if (tid == 0) {
-    for (int w = 1; w < kThreads / 32; ++w) merge_stat(st, sh[w], c);
-    st.pad = 0;
-    stats[blockIdx.x] = st;
+    Stat st{m, 0.f, 0x7fffffff, 0};
+    for (int w = 0; w < kWarps; ++w) {
+      st.s += sh_s[w];
+      st.top = min(st.top, sh_top[w]);
+    }
+    ws.stats[blockIdx.x] = st;
+    if (row * ws.slices == (int)blockIdx.x && row % (a.n + 1) == 0) ws.done[row / (a.n + 1)] = 0;
   }
 }
 
@@ -194,12 +231,15 @@ __global__ void __launch_bounds__(kThreads) stats_kernel(const VerifyArgs a, int
 // octave, by the Taylor series to the 4th power (error 4e-14).
 struct Exp64 {
   const double* table;  // 2^(i / 64), i < 64, in shared memory
-  double m, k64;        // 64 log2(e) / t
+  double k64, mk;       // 64 log2(e) / t, and m times that
+  __device__ __forceinline__ Exp64(const double* table_, float m, float t) : table(table_) {
+    k64 = 64.0 * 1.4426950408889634 / (double)t;
+    mk = (double)m * k64;
+  }
   __device__ __forceinline__ double operator()(float l) const {
     constexpr double kMagic = 6755399441055744.0;  // 1.5 * 2^52
     constexpr double a = 0.010830424696249145;     // ln(2) / 64
-    const double t = ((double)l - m) * k64;
-    if (!(t > -64000.0)) return 0.0;  // below 2^-1000; -inf
+    const double t = fma((double)l, k64, -mk);
     const double kf = t + kMagic;
     const int k = __double2loint(kf);
     const double r = t - (kf - kMagic);
@@ -208,7 +248,8 @@ struct Exp64 {
     p = fma(r, p, a);
     p = fma(r, p, 1.0);
     p *= table[k & 63];
-    return __hiloint2double(__double2hiint(p) + ((k >> 6) << 20), __double2loint(p));
+    p = __hiloint2double(__double2hiint(p) + ((k >> 6) << 20), __double2loint(p));
+    return t > -64000.0 ? p : 0.0;  // 0 below 2^-1000, and for -inf
   }
 };
 
@@ -218,13 +259,15 @@ __device__ __forceinline__ double warp_sum(double v) {
   return v;
 }
 
-// What a row's slices say together: its sum of exponentials relative to m, its
-// maximum and where it is. By a warp, a slice a lane.
+// What a row's slices say together: its sum of exponentials relative to m and
+// its maximum; where all of p lies on one token, that (otherwise -1). By a
+// warp, a slice a lane.
 struct Row {
   double z;
   float m;
-  int top;  // negative where all of p lies on ~top
+  int top;
 };
+constexpr int kUndefined = 0x7fffffff;  // all on the first maximum, not known yet
 __device__ __forceinline__ Row row_of(const Stat* s, int slices, float t) {
   const int lane = threadIdx.x & 31;
   const float c = scale_of(t);
@@ -244,42 +287,90 @@ __device__ __forceinline__ Row row_of(const Stat* s, int slices, float t) {
   int top = __reduce_min_sync(0xffffffffu, st.m == M ? st.top : 0x7fffffff);
   const float base = M == -INFINITY ? 0.f : M;
   z = warp_sum(z * (double)(st.m == M ? 1.f : ex2((st.m - base) * c)));
-  if (top == 0x7fffffff) top = 0;
-  const bool greedy = !(t > 0.f) || !(fabs(z) <= 1.7e308) || isinf(M);
-  return Row{z, M, greedy ? ~top : top};
+  if (t > 0.f) top = !(fabs(z) <= 1.7e308) || isinf(M) ? kUndefined : -1;
+  else if (top == 0x7fffffff) top = 0;  // nothing but NaN
+  return Row{z, M, top};
 }
 
-// Cluster of kCluster CTAs per sequence.
-__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kSampleThreads)
-    sample_kernel(const VerifyArgs a, int slices, const Stat* __restrict__ stats) {
-  __shared__ double table[64];
-  __shared__ double part[kSampleWarps];
-  __shared__ double shared_sum[2];  // this CTA's sum, read by the cluster
-  __shared__ int shared_last;
-  __shared__ unsigned verdict[kSampleWarps];  // bits: drafts not plainly accepted
-  __shared__ unsigned close[kSampleWarps];
+__device__ __forceinline__ double block_sum(double v, double* part) {  // of all threads, in warp order
+  v = warp_sum(v);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = 0.0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) v += part[w];
+  return v;
+}
+// One row of logits.
+template <bool kBf16>
+struct Logits {
+  const void* p;
+  __device__ __forceinline__ Logits(const VerifyArgs& a, int64_t row)
+      : p(static_cast<const char*>(a.logits) + row * a.V * (kBf16 ? 2 : 4)) {}
+  __device__ __forceinline__ float operator()(int j) const { return load_logit(p, kBf16, j); }
+};
+// Calls use(j, logit j, draft probability j) for j = j0, j0 + step, ... below
+// j1, kBatch loads of each array at a time.
+template <bool kQ, typename L, typename F>
+__device__ __forceinline__ void over(const L& logit, const float* q, int j0, int j1, int step, F&& use) {
+  int j = j0;
+  for (; j + (kBatch - 1) * step < j1; j += kBatch * step) {
+    float l[kBatch], x[kBatch];
+#pragma unroll
+    for (int e = 0; e < kBatch; ++e) {
+      l[e] = logit(j + e * step);
+      x[e] = kQ ? __ldg(q + j + e * step) : 0.f;
+    }
+#pragma unroll
+    for (int e = 0; e < kBatch; ++e) use(j + e * step, l[e], x[e]);
+  }
+  for (; j < j1; j += step) use(j, logit(j), kQ ? __ldg(q + j) : 0.f);
+}
+
+// CTA (sequence, chunk). Every CTA of a sequence finds the verdict; the first
+// writes it, and what is known of the result.
+template <bool kBf16>
+__global__ void __launch_bounds__(kThreads) weigh_kernel(const VerifyArgs a, const Space ws) {
+  __shared__ double table[64], part[kWarps];
+  __shared__ unsigned verdict[kWarps], close[kWarps];  // bits: rejected; too close to say
   __shared__ Row rows[256];
-  cg::cluster_group cluster = cg::this_cluster();
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = (int)cluster.block_rank();
-  const int b = blockIdx.x / kCluster, V = a.V, n = a.n;
+  __shared__ int shared_last;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int b = blockIdx.x / ws.chunks, chunk = blockIdx.x - b * ws.chunks, V = a.V, n = a.n;
   if (tid < 64) table[tid] = exp2((double)tid / 64.0);
+  if (tid == 0) shared_last = -1;
   rl::pdl_wait();
   rl::pdl_launch_dependents();
   const float t = a.temperature[b];
-  const double k64 = 64.0 * 1.4426950408889634 / (double)t;
-  const Stat* st = stats + (int64_t)b * (n + 1) * slices;
   const int64_t row0 = (int64_t)b * (n + 1);
   auto draft = [&](int i) {
     const int x = i < n ? a.drafts[(int64_t)b * n + i] : -1;
     return (unsigned)x < (unsigned)V ? x : -1;
   };
-  for (int i = warp; i <= n; i += kSampleWarps) {
-    const Row r = row_of(st + (int64_t)i * slices, slices, t);
+  for (int i = warp; i <= n; i += kWarps) {
+    const Row r = row_of(ws.stats + (row0 + i) * ws.slices, ws.slices, t);
     if (lane == 0) rows[i] = r;
   }
   __syncthreads();
+  if (t > 0.f) {
+    for (int i = 0; i <= n; ++i) {  // a row whose softmax is undefined: look for its first maximum
+      if (rows[i].top != kUndefined) continue;
+      const float m = rows[i].m;
+      const Logits<kBf16> logit(a, row0 + i);
+      int at = m == -INFINITY ? 0 : kUndefined;
+      for (int j = tid; j < V && at == kUndefined; j += kThreads)
+        if (logit(j) == m) at = j;
+      __syncthreads();  // rows[i] has been read
+      if (tid == 0) rows[i].top = V - 1;
+      __syncthreads();
+      at = __reduce_min_sync(0xffffffffu, at);
+      if (lane == 0) atomicMin(&rows[i].top, at);
+      __syncthreads();
+    }
+  }
 
-  // A draft a thread (n is below 256): accepted, rejected, or too close to say.
+  // A draft a thread (n is below 256).
   bool no = false, near = false;
   if (tid <= n) {
     const int x = draft(tid);
@@ -288,10 +379,10 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kSampleThread
       const Row r = rows[tid];
       const double q = a.probs ? (double)a.probs[((int64_t)b * n + tid) * V + x] : 1.0;
       const double lhs = (double)a.accept_u[(int64_t)b * n + tid] * q;
-      if (r.top < 0) {
-        no = !(lhs < (x == ~r.top ? 1.0 : 0.0));
+      if (r.top >= 0) {
+        no = !(lhs < (x == r.top ? 1.0 : 0.0));
       } else {
-        const double p = Exp64{table, (double)r.m, k64}(load_logit(a.logits, a.bf16, (row0 + tid) * V + x));
+        const double p = Exp64(table, r.m, t)(Logits<kBf16>(a, row0 + tid)(x));
         near = p > 0.0 && fabs(lhs * r.z - p) <= 1e-4 * p;
         no = !(lhs * r.z < p);
       }
@@ -304,189 +395,251 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kSampleThread
   }
   __syncthreads();
   int acc = 0;
-  for (;; ++acc) {  // up to n: there is no draft n
+  for (;; ++acc) {  // at most to n: there is no draft n
     const unsigned bit = 1u << (acc & 31);
     bool rejected = verdict[acc >> 5] & bit;
     if (close[acc >> 5] & bit) {
       // The whole CTA sums this row in 64 bits.
       const int x = draft(acc);
-      const Exp64 ex{table, (double)rows[acc].m, k64};
+      const Exp64 ex(table, rows[acc].m, t);
+      const Logits<kBf16> logit(a, row0 + acc);
       double z = 0.0;
-#pragma unroll 4
-      for (int j = tid; j < V; j += kSampleThreads) z += ex(load_logit(a.logits, a.bf16, (row0 + acc) * V + j));
-      z = warp_sum(z);
-      __syncthreads();
-      if (lane == 0) part[warp] = z;
-      __syncthreads();
-      z = 0.0;
-      for (int w = 0; w < kSampleWarps; ++w) z += part[w];
+      over<false>(logit, nullptr, tid, V, kThreads, [&](int, float l, float) { z += ex(l); });
+      z = block_sum(z, part);
       const double q = a.probs ? (double)a.probs[((int64_t)b * n + acc) * V + x] : 1.0;
-      rejected = !((double)a.accept_u[(int64_t)b * n + acc] * q * z <
-                   ex(load_logit(a.logits, a.bf16, (row0 + acc) * V + x)));
+      rejected = !((double)a.accept_u[(int64_t)b * n + acc] * q * z < ex(logit(x)));
     }
     if (rejected) break;
   }
+  const int top = rows[acc].top, x = draft(acc);
+  if (chunk == 0) {
+    for (int i = tid; i <= n; i += kThreads)
+      if (i != acc || top >= 0)
+        a.tokens[row0 + i] = i < acc ? a.drafts[(int64_t)b * n + i] : i == acc ? top : -1;
+    if (tid == 0) {
+      a.accepted[b] = acc;
+      // All of p on one token: so is what a rejected draft leaves of it.
+      ws.verdict[b] = Verdict{acc, x, rows[acc].m, top >= 0};
+    }
+  }
+  if (top >= 0) return;
 
-  // The token after them: weights z * max(0, p - q) or z * p of row acc. Each
-  // CTA takes an eighth of the vocabulary, each warp a sixteenth of that.
-  const bool greedy = rows[acc].top < 0;
-  const int top = greedy ? ~rows[acc].top : rows[acc].top;
-  const Exp64 ex{table, (double)rows[acc].m, k64};
-  const int x = draft(acc);
-  const int64_t base = (row0 + acc) * V;
-  const float* q = x >= 0 && a.probs ? a.probs + ((int64_t)b * n + acc) * V : nullptr;
-  const int per_cta = (V + kCluster - 1) / kCluster, c0 = min(V, rank * per_cta), c1 = min(V, c0 + per_cta);
-  const int per_warp = (per_cta + kSampleWarps - 1) / kSampleWarps;
-  const int j0 = min(c1, c0 + warp * per_warp), j1 = min(c1, j0 + per_warp);
-  bool residual = x >= 0;
-  double z = 1.0;
-  if (residual && q && !greedy) {
-    double s = 0.0;
-    for (int j = j0 + lane; j < j1; j += 32 * kBatch) {
-      float l[kBatch];
-#pragma unroll
-      for (int e = 0; e < kBatch; ++e)
-        l[e] = j + 32 * e < j1 ? load_logit(a.logits, a.bf16, base + j + 32 * e) : -INFINITY;
-#pragma unroll
-      for (int e = 0; e < kBatch; ++e) s += ex(l[e]);
+  // The chunk's sum of exponentials, of which a draft that was chosen outright
+  // (q = 1 there) leaves all but its own.
+  const Exp64 ex(table, rows[acc].m, t);
+  const int drop = a.probs ? -1 : x, c0 = min(V, chunk * ws.chunk), c1 = min(V, c0 + ws.chunk);
+  double sum = 0.0;
+  int last = -1;
+  over<false>(Logits<kBf16>(a, row0 + acc), nullptr, c0 + tid, c1, kThreads, [&](int j, float l, float) {
+    const double w = ex(l);
+    if (w > 0.0 && j != drop) {
+      sum += w;
+      last = j;
     }
-    s = warp_sum(s);
-    __syncthreads();
-    if (lane == 0) part[warp] = s;
-    __syncthreads();
-    if (tid == 0) {
-      s = 0.0;
-      for (int w = 0; w < kSampleWarps; ++w) s += part[w];
-      shared_sum[1] = s;
-    }
-    cluster.sync();
-    z = 0.0;
-    for (int c = 0; c < kCluster; ++c) z += *cluster.map_shared_rank(&shared_sum[1], c);
+  });
+  sum = block_sum(sum, part);
+  last = __reduce_max_sync(0xffffffffu, last);
+  if (lane == 0 && last >= 0) atomicMax(&shared_last, last);
+  __syncthreads();
+  if (tid == 0) {
+    const int64_t at = (int64_t)b * ws.chunks + chunk;
+    ws.z[at] = ws.w[at] = sum;
+    ws.last[at] = shared_last;
   }
-  auto weight = [&](int j, float l, float qj) {
-    const double w = greedy ? (j == top ? 1.0 : 0.0) : ex(l);
-    if (!residual) return w;
-    return fmax(0.0, w - (q ? (double)qj * z : j == x ? w : 0.0));
-  };
-  double mine, before, total;
-  for (;;) {
-    mine = 0.0;
-    int last = -1;
-    for (int j = j0 + lane; j < j1; j += 32 * kBatch) {
-      float l[kBatch], qj[kBatch];
-#pragma unroll
-      for (int e = 0; e < kBatch; ++e) {
-        const bool in = j + 32 * e < j1;
-        l[e] = in ? load_logit(a.logits, a.bf16, base + j + 32 * e) : 0.f;
-        qj[e] = in && q ? q[j + 32 * e] : 0.f;
-      }
-#pragma unroll
-      for (int e = 0; e < kBatch; ++e) {
-        if (j + 32 * e >= j1) break;
-        const double w = weight(j + 32 * e, l[e], qj[e]);
-        mine += w;
-        if (w > 0.0) last = j + 32 * e;
-      }
-    }
-    mine = warp_sum(mine);
-    last = __reduce_max_sync(0xffffffffu, last);
-    __syncthreads();
-    if (tid == 0) shared_last = -1;
-    if (lane == 0) part[warp] = mine;
-    __syncthreads();
-    if (lane == 0) atomicMax(&shared_last, last);
-    if (tid == 0) {
-      double s = 0.0;
-      for (int w = 0; w < kSampleWarps; ++w) s += part[w];
-      shared_sum[0] = s;
-    }
-    cluster.sync();
-    total = before = 0.0;
-    for (int c = 0; c < kCluster; ++c) {
-      const double s = *cluster.map_shared_rank(&shared_sum[0], c);
-      if (c < rank) before += s;
-      total += s;
-    }
-    if (total > 0.0 || !residual) break;
-    residual = false;  // p == q: nothing is left over
-    cluster.sync();    // every CTA has read the sums
-  }
-  // The first token whose cumulative weight exceeds the target lies in the
-  // first part (CTA, then warp) whose end does.
-  const double target = (double)a.sample_u[b] * total;
-  bool owner = shared_sum[0] > 0.0 && before + shared_sum[0] > target;
-  if (owner && rank > 0) {  // no earlier one
-    double c = 0.0;
-    for (int i = 0; i < rank; ++i) {
-      const double s = *cluster.map_shared_rank(&shared_sum[0], i);
-      c += s;
-      if (s > 0.0 && c > target) owner = false;
-    }
-  }
-  if (owner) {
-    double c = before;
-    int w0 = -1;
-    double start = 0.0;
-    for (int w = 0; w < kSampleWarps; ++w) {
-      if (w0 < 0 && part[w] > 0.0 && (c + part[w] > target)) {
-        w0 = w;
-        start = c;
-      }
-      c += part[w];
-    }
-    if (w0 < 0)  // the parts' sums round below their total: the last with weight
-      for (int w = 0; w < kSampleWarps; ++w)
-        if (part[w] > 0.0) w0 = w;
-    if (warp == w0) {
-      int hit = 0x7fffffff, last = -1;
-      float l = 0.f, qj = 0.f;
-      auto fetch = [&](int j) {
-        if (j < j1) {
-          l = load_logit(a.logits, a.bf16, base + j);
-          if (q) qj = q[j];
-        }
-      };
-      fetch(j0 + lane);
-      for (int j = j0; j < j1; j += 32) {
-        const double w = j + lane < j1 ? weight(j + lane, l, qj) : 0.0;
-        fetch(j + 32 + lane);
-        double s = w;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const double y = __shfl_up_sync(0xffffffffu, s, o);
-          if (lane >= o) s += y;
-        }
-        const unsigned over = __ballot_sync(0xffffffffu, w > 0.0 && start + s > target);
-        const unsigned some = __ballot_sync(0xffffffffu, w > 0.0);
-        if (over) {
-          hit = j + __ffs(over) - 1;
-          break;
-        }
-        if (some) last = j + 31 - __clz(some);
-        start += __shfl_sync(0xffffffffu, s, 31);
-      }
-      if (lane == 0) a.tokens[row0 + acc] = hit != 0x7fffffff ? hit : last;
-    }
-  }
-  // A number of 1 or more, or none (NaN): the last token with weight.
-  if (rank == 0 && !(total > target)) {
-    int last = -1;
-    for (int c = 0; c < kCluster; ++c) last = max(last, *cluster.map_shared_rank(&shared_last, c));
-    if (tid == 0) a.tokens[row0 + acc] = last < 0 ? top : last;
-  }
-  if (rank == 0) {
-    for (int i = tid; i <= n; i += kSampleThreads)
-      if (i != acc) a.tokens[row0 + i] = i < acc ? a.drafts[(int64_t)b * n + i] : -1;
-    if (tid == 0) a.accepted[b] = acc;
-  }
-  cluster.sync();  // no CTA leaves while another reads its sums
 }
 
-// Slices of a row: as many as fill the GPU, of 1024 to 65536 tokens.
-int slices_of(int num_sms, int64_t rows, int V) {
-  const int most = (V + 1023) / 1024, least = (V + 65535) / 65536;
-  const int64_t want = (8ll * num_sms + rows - 1) / std::max<int64_t>(rows, 1);
-  return (int)std::max<int64_t>(least, std::min<int64_t>(want, most));
+// CTA (sequence, chunk): what the draft's distribution leaves of the chunk's
+// weights, where there is one to take off; the last CTA of a sequence to be
+// done (its only one otherwise) takes the token.
+template <bool kBf16>
+__global__ void __launch_bounds__(kThreads) pick_kernel(const VerifyArgs a, const Space ws) {
+  __shared__ double table[64], part[kWarps];
+  __shared__ int shared_last;
+  __shared__ bool is_last;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int b = blockIdx.x / ws.chunks, chunk = blockIdx.x - b * ws.chunks, V = a.V, n = a.n;
+  if (tid < 64) table[tid] = exp2((double)tid / 64.0);
+  if (tid == 0) shared_last = -1;
+  rl::pdl_wait();
+  rl::pdl_launch_dependents();
+  __syncthreads();
+  const Verdict v = ws.verdict[b];
+  if (v.done) return;
+  const bool residual = v.draft >= 0 && a.probs;
+  const int64_t row = (int64_t)b * (n + 1) + v.acc, first = (int64_t)b * ws.chunks;
+  const float* q = residual ? a.probs + ((int64_t)b * n + v.acc) * V : nullptr;
+  const Logits<kBf16> logit(a, row);
+  const Exp64 ex(table, v.m, a.temperature[b]);
+  double z = 0.0;
+  bool taken_off = residual;  // weights are max(0, e - q z), or e
+  auto weight = [&](float l, float x) {
+    const double e = ex(l);
+    return taken_off ? fma(-(double)x, z, e) : e;
+  };
+  if (residual) {
+    for (int c = 0; c < ws.chunks; ++c) z += ws.z[first + c];
+    const int c0 = min(V, chunk * ws.chunk), c1 = min(V, c0 + ws.chunk);
+    double sum = 0.0;
+    int last = -1;
+    over<true>(logit, q, c0 + tid, c1, kThreads, [&](int j, float l, float x) {
+      const double w = weight(l, x);
+      if (w > 0.0) {
+        sum += w;
+        last = j;
+      }
+    });
+    sum = block_sum(sum, part);
+    last = __reduce_max_sync(0xffffffffu, last);
+    if (lane == 0 && last >= 0) atomicMax(&shared_last, last);
+    __syncthreads();
+    if (tid == 0) {
+      ws.w[first + chunk] = sum;
+      ws.last[first + chunk] = shared_last;
+      __threadfence();
+      is_last = atomicAdd(&ws.done[b], 1u) == (unsigned)ws.chunks - 1;
+    }
+    __syncthreads();
+    if (!is_last) return;
+    __threadfence();
+  } else if (chunk != 0) {
+    return;
+  }
+
+  // The total; where nothing is left over (p == q), p itself.
+  const double* w = ws.w + first;
+  double total = 0.0;
+  for (int c = 0; c < ws.chunks; ++c) total += __ldcg(w + c);
+  if (!(total > 0.0) && residual) {
+    taken_off = false;
+    w = ws.z + first;
+    total = z;
+  }
+  const int drop = a.probs ? -1 : v.draft;
+  if (!(total > 0.0)) {  // all of p on the draft that was chosen outright
+    if (tid == 0) a.tokens[row] = max(drop, 0);
+    return;
+  }
+  // The first token whose cumulative weight exceeds the target lies in the
+  // first chunk whose end does.
+  const double target = (double)a.sample_u[b] * total;
+  int at = -1, some = -1;
+  double start = 0.0, sum = 0.0;
+  for (int c = 0; c < ws.chunks && at < 0; ++c) {
+    const double y = __ldcg(w + c);
+    if (y > 0.0) {
+      some = c;
+      if (sum + y > target) {
+        at = c;
+        start = sum;
+      }
+    }
+    sum += y;
+  }
+  if (at < 0) {
+    // A number of 1 or more, or none (NaN), or one that rounds up to the
+    // total: the last token with weight.
+    int last = 0;
+    if (taken_off || !residual)
+      last = __ldcg(ws.last + first + some);
+    else
+      for (int j = V - 1; j >= 0; --j)  // p itself: seldom, and short
+        if (ex(logit(j)) > 0.0) {
+          last = j;
+          break;
+        }
+    if (tid == 0) a.tokens[row] = last;
+    return;
+  }
+  // Within the chunk a warp takes an eighth.
+  const int c0 = min(V, at * ws.chunk), c1 = min(V, c0 + ws.chunk), per = (c1 - c0 + kWarps - 1) / kWarps;
+  const int j0 = min(c1, c0 + warp * per), j1 = min(c1, j0 + per);
+  double mine = 0.0;
+  auto add = [&](int j, float l, float x) {
+    const double y = weight(l, x);
+    if (y > 0.0 && j != drop) mine += y;
+  };
+  if (taken_off) over<true>(logit, q, j0 + lane, j1, 32, add);
+  else over<false>(logit, nullptr, j0 + lane, j1, 32, add);
+  block_sum(mine, part);  // leaves the warps' sums in part
+  int owner = -1, upto = -1;
+  sum = start;
+  for (int i = 0; i < kWarps; ++i) {
+    if (part[i] > 0.0) {
+      upto = i;
+      if (owner < 0 && sum + part[i] > target) {
+        owner = i;
+        start = sum;
+      }
+    }
+    sum += part[i];
+  }
+  if (owner < 0) owner = upto;  // the parts' ends round below their sum
+  if (warp != owner) return;
+  int hit = -1, last = 0;
+  float l = 0.f, x = 0.f;
+  auto fetch = [&](int j) {
+    if (j < j1) {
+      l = logit(j);
+      if (taken_off) x = q[j];
+    }
+  };
+  fetch(j0 + lane);
+  for (int j = j0; j < j1 && hit < 0; j += 32) {
+    double y = j + lane < j1 && j + lane != drop ? fmax(0.0, weight(l, x)) : 0.0;
+    fetch(j + 32 + lane);
+    const unsigned with = __ballot_sync(0xffffffffu, y > 0.0);
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double u = __shfl_up_sync(0xffffffffu, y, o);
+      if (lane >= o) y += u;
+    }
+    const unsigned beyond = __ballot_sync(0xffffffffu, start + y > target) & with;
+    if (beyond) hit = j + __ffs(beyond) - 1;
+    if (with) last = j + 31 - __clz(with);
+    start += __shfl_sync(0xffffffffu, y, 31);
+  }
+  if (lane == 0) a.tokens[row] = hit >= 0 ? hit : last;
+}
+
+// Slices of a row (1024 to 65536 tokens) and chunks of the row that a token
+// comes from (1024 to 8192): as many as fill the GPU.
+Space space_of(int num_sms, int B, int n, int V, void* base, uint64_t* bytes) {
+  Space s;
+  const int64_t rows = (int64_t)B * (n + 1);
+  const int most = (V + 1023) / 1024;
+  auto pick = [&](int64_t ctas, int64_t each, int largest) {
+    const int64_t least = (V + largest - 1) / largest;
+    return (int)std::max<int64_t>(least, std::min<int64_t>((ctas + each - 1) / each, most));
+  };
+  s.slices = pick(8ll * num_sms, rows, 65536);
+  s.slice = (V + s.slices - 1) / s.slices;
+  s.chunks = pick(4ll * num_sms, B, 8192);
+  s.chunk = (V + s.chunks - 1) / s.chunks;
+  uint64_t at = 0;
+  auto take = [&](uint64_t size) {
+    char* p = static_cast<char*>(base) + at;
+    at += (size + 15) / 16 * 16;
+    return p;
+  };
+  const uint64_t chunks = (uint64_t)B * s.chunks;
+  s.stats = reinterpret_cast<Stat*>(take((uint64_t)rows * s.slices * sizeof(Stat)));
+  s.z = reinterpret_cast<double*>(take(chunks * 8));
+  s.w = reinterpret_cast<double*>(take(chunks * 8));
+  s.last = reinterpret_cast<int*>(take(chunks * 4));
+  s.verdict = reinterpret_cast<Verdict*>(take((uint64_t)B * sizeof(Verdict)));
+  s.done = reinterpret_cast<unsigned*>(take((uint64_t)B * 4));
+  *bytes = at;
+  return s;
+}
+
+template <bool kBf16>
+int32_t launch_verify(riallm_ctx* ctx, const char* what, const VerifyArgs& a, int B, const Space& ws, cudaStream_t st) {
+  const unsigned rows = (unsigned)B * (a.n + 1);
+  if (int r = rl::launched(ctx, what, rl::launch_pdl(stats_kernel<kBf16>, dim3(rows * ws.slices), dim3(kThreads), 0, st, a, ws)))
+    return r;
+  if (int r = rl::launched(ctx, what, rl::launch_pdl(weigh_kernel<kBf16>, dim3(B * ws.chunks), dim3(kThreads), 0, st, a, ws)))
+    return r;
+  return rl::launched(ctx, what, rl::launch_pdl(pick_kernel<kBf16>, dim3(B * ws.chunks), dim3(kThreads), 0, st, a, ws));
 }
 
 }  // namespace
@@ -495,8 +648,9 @@ extern "C" {
 
 uint64_t riallm_cuda_verify_draft_workspace(const riallm_ctx* ctx, int32_t B, int32_t n, int32_t V) {
   if (!ctx || B <= 0 || n < 0 || V <= 0) return 0;
-  const int64_t rows = (int64_t)B * (n + 1);
-  return (uint64_t)rows * slices_of(ctx->num_sms, rows, V) * sizeof(Stat);
+  uint64_t bytes;
+  space_of(ctx->num_sms, B, n, V, nullptr, &bytes);
+  return bytes;
 }
 
 int32_t riallm_cuda_verify_draft(riallm_ctx* ctx, const void* logits, int32_t logits_dtype, const int32_t* draft_tokens,
@@ -515,25 +669,15 @@ int32_t riallm_cuda_verify_draft(riallm_ctx* ctx, const void* logits, int32_t lo
     return rl::refuse(ctx, RIALLM_ERR_INVALID, what, "NULL argument");
   if (reinterpret_cast<uintptr_t>(logits) & 15)
     return rl::refuse(ctx, RIALLM_ERR_INVALID, what, "logits must be 16-byte aligned");
-  const int64_t rows = (int64_t)B * (n + 1);
-  const int slices = slices_of(ctx->num_sms, rows, V);
-  if (!workspace || workspace_bytes < (uint64_t)rows * slices * sizeof(Stat) ||
-      (reinterpret_cast<uintptr_t>(workspace) & 15))
+  uint64_t bytes;
+  const Space ws = space_of(ctx->num_sms, B, n, V, workspace, &bytes);
+  if (!workspace || workspace_bytes < bytes || (reinterpret_cast<uintptr_t>(workspace) & 15))
     return rl::refuse(ctx, RIALLM_ERR_MEMORY, what, "workspace missing, too small or not 16-byte aligned");
   return rl::guarded(ctx, [&]() -> int32_t {
     const VerifyArgs a{logits, logits_dtype == RIALLM_DTYPE_BF16, draft_tokens, draft_probs, temperature, accept_u,
                        sample_u, n, V, tokens, accepted};
-    Stat* stats = static_cast<Stat*>(workspace);
-    const int slice = (V + slices - 1) / slices;
     const cudaStream_t st = (cudaStream_t)stream;
-    if (int s = rl::launched(ctx, what,
-                             rl::launch_pdl(a.bf16 ? stats_kernel<true> : stats_kernel<false>,
-                                            dim3((unsigned)rows * slices), dim3(kThreads), 0, st, a, slices, slice,
-                                            stats)))
-      return s;
-    return rl::launched(ctx, what,
-                        rl::launch_pdl(sample_kernel, dim3(B * kCluster), dim3(kSampleThreads), 0, st, a, slices,
-                                       static_cast<const Stat*>(stats)));
+    return a.bf16 ? launch_verify<true>(ctx, what, a, B, ws, st) : launch_verify<false>(ctx, what, a, B, ws, st);
   });
 }
 
