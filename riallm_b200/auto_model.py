@@ -205,6 +205,21 @@ class MoeCausalLM:
         new = self.decoder.generate(ids.to(self.device), int(max_new_tokens))
         return ids.tolist() + [int(t) for t in new]
 
+    def generate_drafted(self, input_ids, max_new_tokens: int, drafts: int = 4, temperature: float = 0.0,
+                         seed: Optional[int] = None) -> List[int]:
+        """No counterpart in the reference: decoding with drafted tokens
+        (Decoder.generate_drafted; drafts are looked up in the sequence
+        itself). temperature 0 gives greedy decoding; otherwise tokens are
+        sampled, with the random numbers of `seed`. Returns the prompt ids
+        followed by the new ones."""
+        ids = torch.as_tensor(input_ids).reshape(-1).to(torch.long)
+        if max_new_tokens <= 0:
+            return ids.tolist()
+        gen = None if seed is None else torch.Generator(device=self.device).manual_seed(seed)
+        new = self.decoder.generate_drafted(ids.to(self.device), int(max_new_tokens), drafts=drafts,
+                                            temperature=temperature, generator=gen)
+        return ids.tolist() + [int(t) for t in new]
+
     def stream_stats(self) -> Optional[dict]:
         return self.streamer.stats() if self.streamer is not None else None
 
@@ -222,7 +237,8 @@ class AutoModel:
     @staticmethod
     def from_pretrained(model_id: str, options: Optional[ModelOptions] = None,
                         cache_dir: Optional[str] = None, max_batch: int = 1,
-                        max_seq: Optional[int] = None, routed_streaming: bool = False) -> MoeCausalLM:
+                        max_seq: Optional[int] = None, routed_streaming: bool = False, page_size: int = 0,
+                        num_pages: Optional[int] = None, sinks: int = 0) -> MoeCausalLM:
         """Loads a local Mixtral-architecture checkpoint directory
         (config.json plus safetensors shards). routed_streaming (with
         ModelOptions.prefetch_layers; no counterpart in the reference): decode
@@ -230,7 +246,12 @@ class AutoModel:
         device-resident routers. cache_dir holds the quantized
         per-layer shards (default: <model_id>/riallm_quantized); max_seq
         defaults to ModelOptions.max_seq_len, else the config's
-        max_position_embeddings capped at 4096."""
+        max_position_embeddings capped at 4096. page_size (no counterpart in
+        the reference) pages the key-value cache, of num_pages pages; the
+        attention then keeps to the config's sliding_window, if it has one,
+        and to the first `sinks` positions. Without it the cache is one
+        contiguous tensor per layer and, as in the reference, sliding_window
+        is not acted on."""
         from . import Context
         from .decoder import Decoder, DecoderConfig
         from .loader import CheckpointIndex, QuantizedShardCache, mixtral_moe_layer
@@ -285,7 +306,9 @@ class AutoModel:
             for l, moe in enumerate(moe_layers):
                 for name, t in moe.items():
                     weights[f"model.layers.{l}.{name}"] = _to_device(t, device)
-        decoder = Decoder(cfg, weights, max_batch=max_batch, max_seq=max_seq, device=dev, streamer=streamer)
+        decoder = Decoder(cfg, weights, max_batch=max_batch, max_seq=max_seq, device=dev, streamer=streamer,
+                          page_size=page_size, num_pages=num_pages,
+                          window=(config.sliding_window or 0) if page_size else 0, sinks=sinks)
         return MoeCausalLM(config, options, decoder, streamer, packed)
 
 

@@ -302,6 +302,12 @@ __device__ __forceinline__ double block_sum(double v, double* part) {  // of all
   for (int w = 0; w < kWarps; ++w) v += part[w];
   return v;
 }
+// Sum of v[0 .. n), the same in every warp.
+__device__ __forceinline__ double sum_of(const double* v, int n) {
+  double s = 0.0;
+  for (int i = threadIdx.x & 31; i < n; i += 32) s += __ldcg(v + i);
+  return warp_sum(s);
+}
 // One row of logits.
 template <bool kBf16>
 struct Logits {
@@ -477,7 +483,7 @@ __global__ void __launch_bounds__(kThreads) pick_kernel(const VerifyArgs a, cons
     return taken_off ? fma(-(double)x, z, e) : e;
   };
   if (residual) {
-    for (int c = 0; c < ws.chunks; ++c) z += ws.z[first + c];
+    z = sum_of(ws.z + first, ws.chunks);
     const int c0 = min(V, chunk * ws.chunk), c1 = min(V, c0 + ws.chunk);
     double sum = 0.0;
     int last = -1;
@@ -507,8 +513,7 @@ __global__ void __launch_bounds__(kThreads) pick_kernel(const VerifyArgs a, cons
 
   // The total; where nothing is left over (p == q), p itself.
   const double* w = ws.w + first;
-  double total = 0.0;
-  for (int c = 0; c < ws.chunks; ++c) total += __ldcg(w + c);
+  double total = sum_of(w, ws.chunks);
   if (!(total > 0.0) && residual) {
     taken_off = false;
     w = ws.z + first;
@@ -523,17 +528,26 @@ __global__ void __launch_bounds__(kThreads) pick_kernel(const VerifyArgs a, cons
   // first chunk whose end does.
   const double target = (double)a.sample_u[b] * total;
   int at = -1, some = -1;
-  double start = 0.0, sum = 0.0;
-  for (int c = 0; c < ws.chunks && at < 0; ++c) {
-    const double y = __ldcg(w + c);
-    if (y > 0.0) {
-      some = c;
-      if (sum + y > target) {
-        at = c;
-        start = sum;
-      }
+  double start = 0.0;
+  for (int c = 0; c < ws.chunks && at < 0; c += 32) {
+    const double y = c + lane < ws.chunks ? __ldcg(w + c + lane) : 0.0;
+    double upto = y;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double u = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += u;
     }
-    sum += y;
+    const unsigned with = __ballot_sync(0xffffffffu, y > 0.0);
+    const unsigned beyond = __ballot_sync(0xffffffffu, start + upto > target) & with;
+    if (with) some = c + 31 - __clz(with);
+    if (beyond) {
+      const int i = __ffs(beyond) - 1;
+      at = c + i;
+      const double before = __shfl_sync(0xffffffffu, upto, max(i - 1, 0));
+      if (i > 0) start += before;
+    } else {
+      start += __shfl_sync(0xffffffffu, upto, 31);
+    }
   }
   if (at < 0) {
     // A number of 1 or more, or none (NaN), or one that rounds up to the
@@ -562,7 +576,7 @@ __global__ void __launch_bounds__(kThreads) pick_kernel(const VerifyArgs a, cons
   else over<false>(logit, nullptr, j0 + lane, j1, 32, add);
   block_sum(mine, part);  // leaves the warps' sums in part
   int owner = -1, upto = -1;
-  sum = start;
+  double sum = start;
   for (int i = 0; i < kWarps; ++i) {
     if (part[i] > 0.0) {
       upto = i;

@@ -18,6 +18,13 @@ once) for single-row decode steps, cuBLAS GEMMs otherwise. Positions live in a d
 one decode step (all layers, LM head and the greedy argmax) is captured
 once in a CUDA graph and replayed per token.
 
+With page_size the cache is paged (riallm_b200.paged): sequences hold the
+pages that they have reached, of a pool that may be smaller than max_batch *
+max_seq, and a sliding window (with a few first tokens that stay visible)
+gives its pages back as it moves. generate_drafted runs the model over the
+last token and several drafted ones at a time and keeps those that the model
+itself would have sampled (riallm_b200.sampling).
+
 The MoE tensors (router gate and experts) of at least 4096 elements are
 quantized (compress_layer_state_dict's rule, src/quantization.rs:291-295)
 and stay quantized; attention, embedding and LM-head weights are bf16
@@ -36,11 +43,13 @@ every token to the same experts).
 from __future__ import annotations
 
 from dataclasses import dataclass
-from typing import Dict
+from typing import Callable, Dict, List, Optional, Sequence
 
 import torch
 
 from . import (CompressionType, ConfigError, Context, QuantizedTensor, apply_moe, lib, quantize_tensor, route)
+from .paged import PagedKVCache, paged_attention, rope_paged_append
+from .sampling import lookup_drafts, verify_draft
 
 
 @dataclass
@@ -173,7 +182,8 @@ class Decoder:
     KV cache of `max_seq` positions per sequence."""
 
     def __init__(self, cfg: DecoderConfig, qweights: Dict[str, object], max_batch: int = 1,
-                 max_seq: int = 2048, device: int = 0, streamer=None, ep=None):
+                 max_seq: int = 2048, device: int = 0, streamer=None, ep=None, page_size: int = 0,
+                 num_pages: Optional[int] = None, window: int = 0, sinks: int = 0):
         """streamer: a LayerStreamer over the layers' MoE tensors (router
         gate and experts, one PackedLayer per layer, in layer order); they
         are then not taken from qweights but copied from pinned host memory
@@ -188,7 +198,16 @@ class Decoder:
         attention, norms, embedding and LM head are replicated. Each MoE
         block all-gathers the ranks' tokens, runs the local experts and
         reduce-scatters the partial sums (NCCL collectives, which the decode
-        graph captures)."""
+        graph captures).
+
+        page_size: a paged cache of num_pages pages (default: enough for
+        max_batch sequences of max_seq positions); 0 keeps one contiguous
+        cache. window and sinks (paged only): a position sees the last
+        `window` positions, itself among them, and the first `sinks`."""
+        if not page_size and (num_pages is not None or window or sinks):
+            raise ConfigError("num_pages, window and sinks need a paged cache (page_size)")
+        if window < 0 or sinks < 0:
+            raise ConfigError("window and sinks must not be negative")
         if streamer is not None and ep is not None:
             raise ConfigError("layer streaming and expert parallelism do not combine")
         c = self.cfg = cfg
@@ -226,17 +245,29 @@ class Decoder:
         self.gates = ([pl.tensor("mlp.gate.weight", self.dev) for pl in streamer.layers]
                       if streamer is not None and streamer.routed else None)
         self.max_batch, self.max_seq = max_batch, max_seq
-        shape = (max_batch, c.kv_heads, max_seq, c.head_dim)
-        self.k_cache = [torch.zeros(shape, dtype=torch.bfloat16, device=self.dev) for _ in range(c.layers)]
-        self.v_cache = [torch.zeros(shape, dtype=torch.bfloat16, device=self.dev) for _ in range(c.layers)]
+        self.window, self.sinks = window, sinks
+        self.pages = None
+        if page_size:
+            per_seq = -(-max_seq // page_size) if page_size > 0 else 0
+            self.pages = PagedKVCache(c.layers, c.kv_heads, c.head_dim,
+                                      max_batch * per_seq if num_pages is None else num_pages, page_size, max_batch,
+                                      per_seq, device)
+        else:
+            shape = (max_batch, c.kv_heads, max_seq, c.head_dim)
+            self.k_cache = [torch.zeros(shape, dtype=torch.bfloat16, device=self.dev) for _ in range(c.layers)]
+            self.v_cache = [torch.zeros(shape, dtype=torch.bfloat16, device=self.dev) for _ in range(c.layers)]
         self.inv_freq = inv_freq(c.head_dim, c.theta, self.dev)
         self.pos = torch.zeros(max_batch, dtype=torch.int32, device=self.dev)
         self.length = 0
+        self._lengths = [0] * max_batch  # positions each sequence holds (self.length: the most of any)
         self._graphs: Dict[int, tuple] = {}
 
     def reset(self):
         self.pos.zero_()
         self.length = 0
+        self._lengths = [0] * self.max_batch
+        if self.pages is not None:
+            self.pages.release()
 
     # ------------------------------------------------------------ kernels
     def _st(self):
@@ -260,20 +291,36 @@ class Decoder:
                                                      w.shape[0], K, self._st()))
         return y
 
-    def _forward(self, ids: torch.Tensor, experts_used: list = None) -> torch.Tensor:
-        """ids [B, T] on the device -> last-position logits [B, V] float32.
-        Appends T positions to every sequence (pos += T on the device).
+    def _attend(self, layer: int, qkv: torch.Tensor, q: torch.Tensor, out: torch.Tensor, B: int, T: int):
+        """Rotates and appends a layer's q, k and v, and attends."""
+        c = self.cfg
+        if self.pages is not None:
+            pg = self.pages
+            k, v, pos, table = pg.k_pages[layer], pg.v_pages[layer], self.pos[:B], pg.table[:B]
+            rope_paged_append(qkv, pos, table, k, v, self.inv_freq, q_out=q, ctx=self.ctx)
+            paged_attention(q, pos, table, k, v, window=self.window, sinks=self.sinks, out=out, ctx=self.ctx)
+            return
+        L, nh, nkv, d = lib(), c.heads, c.kv_heads, c.head_dim
+        kc, vc = self.k_cache[layer], self.v_cache[layer]
+        self.ctx.check(L.riallm_cuda_rope_kv_append(self.ctx.ptr, qkv.data_ptr(), self.pos.data_ptr(), B, T, nh, nkv,
+                                                    d, self.inv_freq.data_ptr(), q.data_ptr(), kc.data_ptr(),
+                                                    vc.data_ptr(), self.max_seq, self._st()))
+        self.ctx.check(L.riallm_cuda_attention(self.ctx.ptr, q.data_ptr(), kc.data_ptr(), vc.data_ptr(),
+                                               self.pos.data_ptr(), B, T, nh, nkv, d, self.max_seq, out.data_ptr(),
+                                               self._st()))
+
+    def _forward(self, ids: torch.Tensor, experts_used: list = None, all_logits: bool = False) -> torch.Tensor:
+        """ids [B, T] on the device -> last-position logits [B, V] float32
+        (with all_logits every position's, [B, T, V]). Appends T positions to every sequence (pos += T on the device).
         With experts_used (a list), the number of distinct experts each
         layer's MoE block routes to is appended to it (an extra router pass;
         eager use only)."""
         c, B, T = self.cfg, ids.shape[0], ids.shape[1]
         moe_ctx = self.ctx_step if T == 1 else self.ctx
-        nh, nkv, d = c.heads, c.kv_heads, c.head_dim
         h = self.embed.index_select(0, ids.reshape(-1))          # [B*T, H] residual stream
         n = torch.empty_like(h)
-        q = torch.empty(B * T, nh * d, dtype=torch.bfloat16, device=self.dev)
+        q = torch.empty(B * T, c.heads * c.head_dim, dtype=torch.bfloat16, device=self.dev)
         att = torch.empty_like(q)
-        L = lib()
         st = self.streamer
         routed = st is not None and st.routed and T == 1
         if st is not None and not routed:
@@ -282,13 +329,7 @@ class Decoder:
         for i, layer in enumerate(self.layers):
             self._norm(h, layer["in_norm"], n)
             qkv = self._linear(n, layer["wqkv"])
-            kc, vc = self.k_cache[i], self.v_cache[i]
-            self.ctx.check(L.riallm_cuda_rope_kv_append(self.ctx.ptr, qkv.data_ptr(), self.pos.data_ptr(), B, T,
-                                                        nh, nkv, d, self.inv_freq.data_ptr(), q.data_ptr(),
-                                                        kc.data_ptr(), vc.data_ptr(), self.max_seq, self._st()))
-            self.ctx.check(L.riallm_cuda_attention(self.ctx.ptr, q.data_ptr(), kc.data_ptr(), vc.data_ptr(),
-                                                   self.pos.data_ptr(), B, T, nh, nkv, d, self.max_seq,
-                                                   att.data_ptr(), self._st()))
+            self._attend(i, qkv, q, att, B, T)
             o = self._linear(att, layer["wo"])
             self._norm(h, layer["post_norm"], n, delta=o)         # h += o; n = norm(h)
             if st is None:
@@ -314,17 +355,26 @@ class Decoder:
                 if not routed:
                     st.prefetch(i + st.depth)
         self.pos[:B].add_(T)
-        last = h.view(B, T, -1)[:, -1].contiguous()
+        last = h if all_logits else h.view(B, T, -1)[:, -1].contiguous()
         nl = torch.empty_like(last)
         self._norm(last, self.final_norm, nl)
-        return self._linear(nl, self.lm_head).float()
+        logits = self._linear(nl, self.lm_head).float()
+        return logits.view(B, T, -1) if all_logits else logits
 
-    def _advance(self, B: int, T: int):
+    def _advance(self, B: int, T: int, idle: Sequence[int] = ()):
+        """Room for T more positions of B sequences; `idle` ones get no pages
+        for them (what is written there is dropped)."""
         if B > self.max_batch:
             raise ConfigError(f"batch {B} > max_batch {self.max_batch}")
         if self.length + T > self.max_seq:
             raise ConfigError(f"sequence length {self.length + T} > max_seq {self.max_seq}")
+        if self.pages is not None:
+            if self.window:
+                self.pages.release_before([n - self.window + 1 for n in self._lengths[:B]], self.sinks)
+            self.pages.reserve([n if b in idle else n + T for b, n in enumerate(self._lengths[:B])])
         self.length += T
+        for b in range(B):
+            self._lengths[b] += T
 
     def forward(self, ids: torch.Tensor) -> torch.Tensor:
         """ids [B, T] (or [T] for one sequence) -> last-position logits [B, V]."""
@@ -393,6 +443,71 @@ class Decoder:
             lk = torch.stack(kept, 1)
             return res, (lk[0] if one else lk)
         return res
+
+    def generate_drafted(self, prompt: torch.Tensor, new_tokens: int, drafts: int = 4,
+                         propose: Optional[Callable[[List[int], int], Sequence[int]]] = None,
+                         temperature: float = 0.0, generator: Optional[torch.Generator] = None):
+        """Decoding with drafted tokens: each step runs the model once over a
+        sequence's last token and up to `drafts` proposed ones, and keeps the
+        proposals that verify_draft accepts and the token it takes after them.
+        propose(tokens, n) returns up to n guesses at what follows a
+        sequence's tokens (default: lookup_drafts, what followed the same
+        tokens earlier in it). temperature 0 decodes greedily; otherwise the
+        tokens are distributed as if sampled one by one, with random numbers
+        from `generator` (a CUDA generator). Returns the new ids as generate
+        does; draft_stats then tells the model steps taken and the drafts
+        proposed and accepted."""
+        if drafts < 0 or drafts > 255:
+            raise ConfigError("drafts must be in 0..255")
+        if new_tokens <= 0:
+            raise ConfigError("new_tokens must be positive")
+        one = prompt.dim() == 1
+        if one:
+            prompt = prompt[None]
+        propose = propose or lookup_drafts
+        B, dev = prompt.shape[0], self.dev
+        self.reset()
+        temp = torch.full((B,), float(temperature), dtype=torch.float32, device=dev)
+
+        def uniform(*shape):
+            return torch.rand(shape, dtype=torch.float32, device=dev, generator=generator)
+
+        seqs = [list(map(int, row)) for row in prompt.tolist()]
+        done = [len(s) + new_tokens for s in seqs]
+        first, _ = verify_draft(self.forward(prompt)[:, None].contiguous(), None, None, uniform(B), temp, ctx=self.ctx)
+        for s, t in zip(seqs, first[:, 0].tolist()):
+            s.append(t)
+        stats = {"steps": 1, "proposed": 0, "accepted": 0}
+        while any(len(s) < d for s, d in zip(seqs, done)):
+            n = min(drafts, self.max_seq - self.length - 1)
+            want = [min(n, d - len(s) - 1) for s, d in zip(seqs, done)]
+            guess = [list(propose(list(s), w))[:w] if w > 0 else [] for s, w in zip(seqs, want)]
+            n = max(0, min(n, max(map(len, guess))))
+            guess = [g + [-1] * (n - len(g)) for g in guess]
+            before = self._lengths[:B]
+            self._advance(B, n + 1, [b for b in range(B) if len(seqs[b]) >= done[b]])
+            draft = torch.tensor(guess, dtype=torch.int32, device=dev).view(B, n)
+            last = torch.tensor([[s[-1]] for s in seqs], dtype=torch.long, device=dev)
+            # A guess outside the vocabulary ends its sequence's drafts; the
+            # model still wants an id there.
+            ids = torch.cat([last, draft.long().clamp(0, self.cfg.vocab - 1)], 1)
+            logits = self._forward(ids, all_logits=True)
+            out, accepted = verify_draft(logits, draft, uniform(B, n), uniform(B), temp, ctx=self.ctx)
+            stats["steps"] += 1
+            for b, (toks, a) in enumerate(zip(out.tolist(), accepted.tolist())):
+                if len(seqs[b]) >= done[b]:
+                    self._lengths[b] = before[b]  # finished: it waits for the others
+                    continue
+                stats["proposed"] += sum(0 <= g < self.cfg.vocab for g in guess[b])
+                stats["accepted"] += a
+                seqs[b] += toks[:a + 1]
+                self._lengths[b] = before[b] + 1 + a
+            # What follows the accepted drafts is written over by the next step.
+            self.pos[:B].copy_(torch.tensor(self._lengths[:B], dtype=torch.int32))
+            self.length = max(self._lengths[:B])
+        self.draft_stats = stats
+        new = [s[d - new_tokens:d] for s, d in zip(seqs, done)]
+        return new[0] if one else torch.tensor(new, device=dev)
 
     def decode_forced(self, ids: torch.Tensor) -> None:
         """Decode steps fed given ids (teacher forcing): ids [S, B, 1] on the

@@ -22,23 +22,44 @@ def _need(ok: bool, what: str) -> None:
 
 
 def _check_cache(what, x, pos, page_table, k_pages, v_pages):
-    """The checks both operators share; returns (B, T)."""
-    dev = x.device
-    _need(x.is_cuda and x.dtype is torch.bfloat16 and x.dim() == 2 and x.is_contiguous(),
+    """The checks both operators share; returns (device, B, T, pages' shape).
+    A decode step makes them for every layer, so what holds costs little and
+    the message is worked out only for what does not."""
+    bf16, i32 = torch.bfloat16, torch.int32
+    dev = x.get_device()
+    shape, table = k_pages.shape, page_table.shape
+    B, rows = pos.shape[0] if pos.dim() == 1 else -1, x.shape[0] if x.dim() == 2 else -1
+    if (dev >= 0 and dev == k_pages.get_device() == v_pages.get_device() == pos.get_device()
+            == page_table.get_device()
+            and x.dtype is bf16 and k_pages.dtype is bf16 and v_pages.dtype is bf16 and pos.dtype is i32
+            and page_table.dtype is i32 and B >= 0 and rows >= 0 and len(shape) == 4 and shape == v_pages.shape
+            and len(table) == 2 and table[0] == B and (rows % B == 0 if B else rows == 0)
+            and x.is_contiguous() and k_pages.is_contiguous() and v_pages.is_contiguous() and pos.is_contiguous()
+            and (page_table.is_contiguous() or page_table.stride(1) == 1 or table[1] == 1)):
+        return dev, B, (rows // B if B else 0), shape
+    _need(x.is_cuda and x.dtype is bf16 and rows >= 0 and x.is_contiguous(),
           f"{what}: rows must be a contiguous 2-D bf16 CUDA tensor")
     for t in (k_pages, v_pages):
-        _need(t.dtype is torch.bfloat16 and t.dim() == 4 and t.is_contiguous() and t.device == dev,
+        _need(t.dtype is bf16 and t.dim() == 4 and t.is_contiguous() and t.device == x.device,
               f"{what}: pages must be contiguous bf16 [num_pages, kv_heads, page_size, head_dim] on the rows' device")
     _need(k_pages.shape == v_pages.shape, f"{what}: k_pages and v_pages differ in shape")
-    _need(pos.dtype is torch.int32 and pos.dim() == 1 and pos.is_contiguous() and pos.device == dev,
+    _need(pos.dtype is i32 and B >= 0 and pos.is_contiguous() and pos.device == x.device,
           f"{what}: pos must be a contiguous int32 [B] tensor on the rows' device")
-    B = pos.shape[0]
-    _need(page_table.dtype is torch.int32 and page_table.dim() == 2 and page_table.shape[0] == B
-          and page_table.device == dev and (page_table.stride(1) == 1 or page_table.shape[1] == 1),
-          f"{what}: page_table must be int32 [B, max_pages] with unit stride along the pages, on the rows' device")
-    rows = x.shape[0]
     _need(rows == 0 if B == 0 else rows % B == 0, f"{what}: {rows} rows are no multiple of {B} sequences")
-    return B, (rows // B if B else 0)
+    raise ConfigError(f"{what}: page_table must be int32 [B, max_pages] with unit stride along the pages, on the "
+                      "rows' device")
+
+
+def _context(what: str, ctx: Optional[Context], dev: int) -> Context:
+    if ctx is None:
+        return Context._by_device.get(dev) or Context.get(dev)
+    _need(ctx.device == dev, f"{what}: the context is another device's")
+    return ctx
+
+
+# The raw handle of the current stream of a device.
+_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
+    lambda dev: torch.cuda.current_stream(dev).cuda_stream)
 
 
 def _table_stride(page_table: torch.Tensor) -> int:
@@ -52,25 +73,25 @@ def rope_paged_append(qkv: torch.Tensor, pos: torch.Tensor, page_table: torch.Te
     """Rotates the q and k heads of qkv [B*T, (nh + 2*nkv) * d] (bf16; row
     b*T + t at position pos[b] + t), writes k and v into the sequences' pages
     and returns the rotated q [B*T, nh*d]. inv_freq is float32 [d/2]."""
-    B, T = _check_cache("rope_paged_append", qkv, pos, page_table, k_pages, v_pages)
-    num_pages, nkv, ps, d = k_pages.shape
-    _need(d > 0 and qkv.shape[1] % d == 0 and qkv.shape[1] // d > 2 * nkv,
+    dev, B, T, (num_pages, nkv, ps, d) = _check_cache("rope_paged_append", qkv, pos, page_table, k_pages, v_pages)
+    rows, width = qkv.shape
+    _need(d > 0 and width % d == 0 and width // d > 2 * nkv,
           "rope_paged_append: qkv rows must hold q heads and 2 * kv_heads more of head_dim")
-    nh = qkv.shape[1] // d - 2 * nkv
-    _need(inv_freq.dtype is torch.float32 and inv_freq.is_contiguous() and inv_freq.numel() == d // 2
-          and inv_freq.device == qkv.device, "rope_paged_append: inv_freq must be float32 [head_dim / 2]")
+    nh = width // d - 2 * nkv
+    _need(inv_freq.dtype is torch.float32 and inv_freq.numel() == d // 2 and inv_freq.get_device() == dev
+          and inv_freq.is_contiguous(), "rope_paged_append: inv_freq must be float32 [head_dim / 2]")
     if q_out is None:
-        q_out = torch.empty((qkv.shape[0], nh * d), dtype=torch.bfloat16, device=qkv.device)
+        q_out = torch.empty((rows, nh * d), dtype=torch.bfloat16, device=qkv.device)
     else:
-        _need(q_out.dtype is torch.bfloat16 and q_out.shape == (qkv.shape[0], nh * d) and q_out.is_contiguous()
-              and q_out.device == qkv.device, "rope_paged_append: q_out must be contiguous bf16 [B*T, heads*head_dim]")
-    dev = qkv.device.index
-    ctx = ctx or Context.get(dev)
-    _need(ctx.device == dev, "rope_paged_append: the context is another device's")
-    ctx.check(lib().riallm_cuda_rope_paged_append(
+        _need(q_out.dtype is torch.bfloat16 and q_out.shape == (rows, nh * d) and q_out.get_device() == dev
+              and q_out.is_contiguous(), "rope_paged_append: q_out must be contiguous bf16 [B*T, heads*head_dim]")
+    ctx = _context("rope_paged_append", ctx, dev)
+    status = lib().riallm_cuda_rope_paged_append(
         ctx.ptr, qkv.data_ptr(), pos.data_ptr(), page_table.data_ptr(), _table_stride(page_table),
         page_table.shape[1], B, T, nh, nkv, d, inv_freq.data_ptr(), q_out.data_ptr(), k_pages.data_ptr(),
-        v_pages.data_ptr(), num_pages, ps, torch.cuda.current_stream(dev).cuda_stream))
+        v_pages.data_ptr(), num_pages, ps, _stream(dev))
+    if status:
+        ctx.check(status)
     return q_out
 
 
@@ -85,18 +106,16 @@ def paged_attention(q: torch.Tensor, pos: torch.Tensor, page_table: torch.Tensor
     position p = pos[b] + t) over the sequences' pages: positions j <= p, and
     with a window only j > p - window or j < sinks. Rows that see nothing are
     zero. Returns out [B*T, nh*d]."""
-    B, T = _check_cache("paged_attention", q, pos, page_table, k_pages, v_pages)
-    num_pages, nkv, ps, d = k_pages.shape
-    _need(d > 0 and q.shape[1] % d == 0, "paged_attention: q rows must hold whole heads")
-    nh = q.shape[1] // d
+    dev, B, T, (num_pages, nkv, ps, d) = _check_cache("paged_attention", q, pos, page_table, k_pages, v_pages)
+    width = q.shape[1]
+    _need(d > 0 and width % d == 0, "paged_attention: q rows must hold whole heads")
+    nh = width // d
     if out is None:
         out = torch.empty_like(q)
     else:
-        _need(out.dtype is torch.bfloat16 and out.shape == q.shape and out.is_contiguous() and out.device == q.device,
+        _need(out.dtype is torch.bfloat16 and out.shape == q.shape and out.get_device() == dev and out.is_contiguous(),
               "paged_attention: out must be contiguous bf16 of q's shape")
-    dev = q.device.index
-    ctx = ctx or Context.get(dev)
-    _need(ctx.device == dev, "paged_attention: the context is another device's")
+    ctx = _context("paged_attention", ctx, dev)
     L = lib()
     max_pages = page_table.shape[1]
     key = (dev, B, T, nh, nkv, d, max_pages, ps)
@@ -108,10 +127,12 @@ def paged_attention(q: torch.Tensor, pos: torch.Tensor, page_table: torch.Tensor
     # From the caching allocator, in the order of the call's stream: two calls
     # never share one, whatever streams or graphs they are in.
     ws = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
-    ctx.check(L.riallm_cuda_paged_attention(
+    status = L.riallm_cuda_paged_attention(
         ctx.ptr, q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), pos.data_ptr(), page_table.data_ptr(),
         _table_stride(page_table), max_pages, B, T, nh, nkv, d, num_pages, ps, window, sinks, out.data_ptr(),
-        ws.data_ptr() if ws is not None else None, size, torch.cuda.current_stream(dev).cuda_stream))
+        ws.data_ptr() if size else None, size, _stream(dev))
+    if status:
+        ctx.check(status)
     return out
 
 

@@ -10,7 +10,10 @@ from typing import Dict, List, Optional, Sequence, Tuple, Union
 
 import torch
 
-from . import ConfigError, Context, _act_dtype, lib
+from . import ConfigError, Context, lib
+from .paged import _context, _stream
+
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1}
 
 # Workspace bytes by call shape.
 _workspace: Dict[Tuple[int, ...], int] = {}
@@ -38,42 +41,46 @@ def verify_draft(logits: torch.Tensor, draft_tokens: Optional[torch.Tensor], acc
     Returns (tokens int32 [B, n + 1]: the accepted drafts, the token taken
     after them, then -1; accepted int32 [B]). The definition is
     riallm_cuda_verify_draft's (include/riallm_cuda.h)."""
-    _need(logits.is_cuda and logits.dim() == 3 and logits.is_contiguous() and logits.shape[1] > 0,
+    dev = logits.get_device()
+    _need(dev >= 0 and logits.dim() == 3 and logits.is_contiguous() and logits.shape[1] > 0,
           "logits must be a contiguous CUDA tensor [B, n + 1, V]")
+    dtype = _DTYPES.get(logits.dtype)
+    _need(dtype is not None, "logits must be float32 or bf16")
     B, n1, V = logits.shape
-    n, dev = n1 - 1, logits.device
+    n, device, f32 = n1 - 1, logits.device, torch.float32
 
     def check(t, dtype, shape, name):
-        _need(t.dtype is dtype and t.shape == shape and t.is_contiguous() and t.device == dev,
-              f"{name} must be contiguous {dtype} {list(shape)} on the logits' device")
+        if not (t.dtype is dtype and t.shape == shape and t.get_device() == dev and t.is_contiguous()):
+            raise ConfigError(f"verify_draft: {name} must be contiguous {dtype} {list(shape)} on the logits' device")
 
     if n or draft_tokens is not None:
         _need(draft_tokens is not None and accept_u is not None, "draft_tokens and accept_u are wanted")
         check(draft_tokens, torch.int32, (B, n), "draft_tokens")
-        check(accept_u, torch.float32, (B, n), "accept_u")
-    check(sample_u, torch.float32, (B,), "sample_u")
+        check(accept_u, f32, (B, n), "accept_u")
+    check(sample_u, f32, (B,), "sample_u")
     if draft_probs is not None:
-        check(draft_probs, torch.float32, (B, n, V), "draft_probs")
+        check(draft_probs, f32, (B, n, V), "draft_probs")
     if not isinstance(temperature, torch.Tensor):
-        temperature = torch.full((B,), float(temperature), dtype=torch.float32, device=dev)
-    check(temperature, torch.float32, (B,), "temperature")
-    tokens = torch.empty((B, n1), dtype=torch.int32, device=dev)
-    accepted = torch.empty((B,), dtype=torch.int32, device=dev)
-    ctx = ctx or Context.get(dev.index)
-    _need(ctx.device == dev.index, "the context is another device's")
+        temperature = torch.full((B,), float(temperature), dtype=f32, device=device)
+    check(temperature, f32, (B,), "temperature")
+    tokens = torch.empty((B, n1), dtype=torch.int32, device=device)
+    accepted = torch.empty((B,), dtype=torch.int32, device=device)
+    ctx = _context("verify_draft", ctx, dev)
     L = lib()
-    key = (dev.index, B, n, V)
+    key = (dev, B, n, V)
     size = _workspace.get(key)
     if size is None:
         if len(_workspace) > 4096:
             _workspace.clear()
         size = _workspace[key] = L.riallm_cuda_verify_draft_workspace(ctx.ptr, B, n, V)
-    ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
-    ctx.check(L.riallm_cuda_verify_draft(
-        ctx.ptr, logits.data_ptr(), _act_dtype(logits.dtype), draft_tokens.data_ptr() if n else None,
+    ws = torch.empty(size, dtype=torch.uint8, device=device)
+    status = L.riallm_cuda_verify_draft(
+        ctx.ptr, logits.data_ptr(), dtype, draft_tokens.data_ptr() if n else None,
         draft_probs.data_ptr() if draft_probs is not None and n else None, temperature.data_ptr(),
         accept_u.data_ptr() if n else None, sample_u.data_ptr(), B, n, V, tokens.data_ptr(), accepted.data_ptr(),
-        ws.data_ptr() if ws is not None else None, size, torch.cuda.current_stream(dev).cuda_stream))
+        ws.data_ptr(), size, _stream(dev))
+    if status:
+        ctx.check(status)
     return tokens, accepted
 
 
