@@ -67,13 +67,12 @@ struct Verdict {
   int done;   // the row's p lies on one token, which has been written
 };
 // The workspace: statistics of the rows' slices; per sequence and chunk the
-// sum of exponentials, the sum of weights and the last token with weight; per
-// sequence the verdict and a count of finished chunks.
+// sum of exponentials and of weights; per sequence the verdict and a count of
+// finished chunks.
 struct Space {
   Stat* stats;
   double* z;
   double* w;
-  int* last;
   Verdict* verdict;
   unsigned* done;
   int slices, slice, chunks, chunk;
@@ -227,29 +226,36 @@ __global__ void __launch_bounds__(kThreads)
 
 // ------------------------------------------------------------ 64 bits
 //
-// e^((l - m) / t): 2^(k / 64) from a table and the rest, at most 1 / 128
-// octave, by the Taylor series to the 4th power (error 4e-14).
+// e^((l - m) / t): 2^(k / 256) from a table and the rest, at most 1 / 512
+// octave, by the Taylor series to the 3rd power (error 1.4e-13).
+constexpr int kTable = 256;
+static_assert(kTable == kThreads, "a thread fills an entry");
 struct Exp64 {
-  const double* table;  // 2^(i / 64), i < 64, in shared memory
-  double k64, mk;       // 64 log2(e) / t, and m times that
+  const double* table;  // 2^(i / 256), in shared memory
+  double k, mk;         // 256 log2(e) / t, and m times that
   __device__ __forceinline__ Exp64(const double* table_, float m, float t) : table(table_) {
-    k64 = 64.0 * 1.4426950408889634 / (double)t;
-    mk = (double)m * k64;
+    k = kTable * 1.4426950408889634 / (double)t;
+    mk = (double)m * k;
   }
-  __device__ __forceinline__ double operator()(float l) const {
-    constexpr double kMagic = 6755399441055744.0;  // 1.5 * 2^52
-    constexpr double a = 0.010830424696249145;     // ln(2) / 64
-    const double t = fma((double)l, k64, -mk);
-    const double kf = t + kMagic;
-    const int k = __double2loint(kf);
-    const double r = t - (kf - kMagic);
-    double p = fma(r, a * a * a * a / 24.0, a * a * a / 6.0);
-    p = fma(r, p, a * a / 2.0);
+  // The value, where `some`; it is 0 otherwise (below 2^-1000, and at -inf).
+  __device__ __forceinline__ double operator()(float l, bool& some) const {
+    constexpr double kMagic = 6755399441055744.0;            // 1.5 * 2^52
+    constexpr double a = 0.6931471805599453 / kTable;
+    const double x = fma((double)l, k, -mk);
+    const double xf = x + kMagic;
+    const int i = __double2loint(xf);
+    const double r = x - (xf - kMagic);
+    double p = fma(r, a * a * a / 6.0, a * a / 2.0);
     p = fma(r, p, a);
     p = fma(r, p, 1.0);
-    p *= table[k & 63];
-    p = __hiloint2double(__double2hiint(p) + ((k >> 6) << 20), __double2loint(p));
-    return t > -64000.0 ? p : 0.0;  // 0 below 2^-1000, and for -inf
+    p *= table[i & (kTable - 1)];
+    some = x > -1000.0 * kTable;
+    return __hiloint2double(__double2hiint(p) + ((i & -kTable) << 12), __double2loint(p));
+  }
+  __device__ __forceinline__ double operator()(float l) const {
+    bool some;
+    const double p = (*this)(l, some);
+    return some ? p : 0.0;
   }
 };
 
@@ -338,14 +344,12 @@ __device__ __forceinline__ void over(const L& logit, const float* q, int j0, int
 // writes it, and what is known of the result.
 template <bool kBf16>
 __global__ void __launch_bounds__(kThreads) weigh_kernel(const VerifyArgs a, const Space ws) {
-  __shared__ double table[64], part[kWarps];
+  __shared__ double table[kTable], part[kWarps];
   __shared__ unsigned verdict[kWarps], close[kWarps];  // bits: rejected; too close to say
   __shared__ Row rows[256];
-  __shared__ int shared_last;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int b = blockIdx.x / ws.chunks, chunk = blockIdx.x - b * ws.chunks, V = a.V, n = a.n;
-  if (tid < 64) table[tid] = exp2((double)tid / 64.0);
-  if (tid == 0) shared_last = -1;
+  table[tid] = exp2((double)tid / kTable);
   rl::pdl_wait();
   rl::pdl_launch_dependents();
   const float t = a.temperature[b];
@@ -435,23 +439,17 @@ __global__ void __launch_bounds__(kThreads) weigh_kernel(const VerifyArgs a, con
   const Exp64 ex(table, rows[acc].m, t);
   const int drop = a.probs ? -1 : x, c0 = min(V, chunk * ws.chunk), c1 = min(V, c0 + ws.chunk);
   double sum = 0.0;
-  int last = -1;
-  over<false>(Logits<kBf16>(a, row0 + acc), nullptr, c0 + tid, c1, kThreads, [&](int j, float l, float) {
-    const double w = ex(l);
-    if (w > 0.0 && j != drop) {
-      sum += w;
-      last = j;
-    }
-  });
+  const Logits<kBf16> logit(a, row0 + acc);
+  auto add = [&](int, float l, float) {
+    bool some;
+    const double w = ex(l, some);
+    if (some) sum += w;
+  };
+  const int cut = min(max(drop, c0), c1);  // around the dropped token, if it is here
+  over<false>(logit, nullptr, c0 + tid, cut, kThreads, add);
+  over<false>(logit, nullptr, (cut == drop ? cut + 1 : cut) + tid, c1, kThreads, add);
   sum = block_sum(sum, part);
-  last = __reduce_max_sync(0xffffffffu, last);
-  if (lane == 0 && last >= 0) atomicMax(&shared_last, last);
-  __syncthreads();
-  if (tid == 0) {
-    const int64_t at = (int64_t)b * ws.chunks + chunk;
-    ws.z[at] = ws.w[at] = sum;
-    ws.last[at] = shared_last;
-  }
+  if (tid == 0) ws.z[(int64_t)b * ws.chunks + chunk] = ws.w[(int64_t)b * ws.chunks + chunk] = sum;
 }
 
 // CTA (sequence, chunk): what the draft's distribution leaves of the chunk's
@@ -459,13 +457,12 @@ __global__ void __launch_bounds__(kThreads) weigh_kernel(const VerifyArgs a, con
 // done (its only one otherwise) takes the token.
 template <bool kBf16>
 __global__ void __launch_bounds__(kThreads) pick_kernel(const VerifyArgs a, const Space ws) {
-  __shared__ double table[64], part[kWarps];
-  __shared__ int shared_last;
+  __shared__ double table[kTable], part[kWarps];
   __shared__ bool is_last;
+  __shared__ int found;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int b = blockIdx.x / ws.chunks, chunk = blockIdx.x - b * ws.chunks, V = a.V, n = a.n;
-  if (tid < 64) table[tid] = exp2((double)tid / 64.0);
-  if (tid == 0) shared_last = -1;
+  table[tid] = exp2((double)tid / kTable);
   rl::pdl_wait();
   rl::pdl_launch_dependents();
   __syncthreads();
@@ -486,21 +483,13 @@ __global__ void __launch_bounds__(kThreads) pick_kernel(const VerifyArgs a, cons
     z = sum_of(ws.z + first, ws.chunks);
     const int c0 = min(V, chunk * ws.chunk), c1 = min(V, c0 + ws.chunk);
     double sum = 0.0;
-    int last = -1;
-    over<true>(logit, q, c0 + tid, c1, kThreads, [&](int j, float l, float x) {
+    over<true>(logit, q, c0 + tid, c1, kThreads, [&](int, float l, float x) {
       const double w = weight(l, x);
-      if (w > 0.0) {
-        sum += w;
-        last = j;
-      }
+      if (w > 0.0) sum += w;
     });
     sum = block_sum(sum, part);
-    last = __reduce_max_sync(0xffffffffu, last);
-    if (lane == 0 && last >= 0) atomicMax(&shared_last, last);
-    __syncthreads();
     if (tid == 0) {
       ws.w[first + chunk] = sum;
-      ws.last[first + chunk] = shared_last;
       __threadfence();
       is_last = atomicAdd(&ws.done[b], 1u) == (unsigned)ws.chunks - 1;
     }
@@ -551,17 +540,16 @@ __global__ void __launch_bounds__(kThreads) pick_kernel(const VerifyArgs a, cons
   }
   if (at < 0) {
     // A number of 1 or more, or none (NaN), or one that rounds up to the
-    // total: the last token with weight.
+    // total: the last token with weight, which chunk `some` holds.
+    if (tid == 0) found = 0;
+    __syncthreads();
+    const int c0 = min(V, some * ws.chunk), c1 = min(V, c0 + ws.chunk);
     int last = 0;
-    if (taken_off || !residual)
-      last = __ldcg(ws.last + first + some);
-    else
-      for (int j = V - 1; j >= 0; --j)  // p itself: seldom, and short
-        if (ex(logit(j)) > 0.0) {
-          last = j;
-          break;
-        }
-    if (tid == 0) a.tokens[row] = last;
+    for (int j = c0 + tid; j < c1; j += kThreads)
+      if (j != drop && weight(logit(j), taken_off ? q[j] : 0.f) > 0.0) last = j;
+    atomicMax(&found, last);
+    __syncthreads();
+    if (tid == 0) a.tokens[row] = found;
     return;
   }
   // Within the chunk a warp takes an eighth.
@@ -639,7 +627,6 @@ Space space_of(int num_sms, int B, int n, int V, void* base, uint64_t* bytes) {
   s.stats = reinterpret_cast<Stat*>(take((uint64_t)rows * s.slices * sizeof(Stat)));
   s.z = reinterpret_cast<double*>(take(chunks * 8));
   s.w = reinterpret_cast<double*>(take(chunks * 8));
-  s.last = reinterpret_cast<int*>(take(chunks * 4));
   s.verdict = reinterpret_cast<Verdict*>(take((uint64_t)B * sizeof(Verdict)));
   s.done = reinterpret_cast<unsigned*>(take((uint64_t)B * 4));
   *bytes = at;
