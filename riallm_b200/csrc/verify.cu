@@ -38,6 +38,8 @@ namespace {
 
 constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kBatch = 8;  // loads of an array that a thread has in flight
+constexpr int kTable = 256;
+static_assert(kTable == kThreads, "a thread fills an entry");
 
 using rl::ex2;
 
@@ -66,16 +68,19 @@ struct Verdict {
   float m;    // the row's maximum
   int done;   // the row's p lies on one token, which has been written
 };
-// The workspace: statistics of the rows' slices; per sequence and chunk the
-// sum of exponentials and of weights; per sequence the verdict and a count of
-// finished chunks.
+// The workspace: statistics of the rows' slices; a table of powers and per
+// sequence 256 log2(e) / temperature (see Exp64); per sequence and part (an
+// eighth of a chunk, a warp's share) the sum of exponentials and of weights;
+// per sequence the verdict and a count of finished chunks.
 struct Space {
   Stat* stats;
+  double* table;
+  double* scale;
   double* z;
   double* w;
   Verdict* verdict;
   unsigned* done;
-  int slices, slice, chunks, chunk;
+  int slices, slice, chunks, part;
 };
 
 // Of a slice of a row: its maximum (NaN left out); the sum of
@@ -147,6 +152,7 @@ __global__ void __launch_bounds__(kThreads)
   const int begin = min(a.V, (int)(blockIdx.x - row * ws.slices) * slice), end = min(a.V, begin + slice);
   const float temp = a.temperature[row / (a.n + 1)], c = scale_of(temp);
   const bool greedy = !(temp > 0.f);
+  if (blockIdx.x == 0) ws.table[tid] = exp2((double)tid / kTable);
   const int64_t base = (int64_t)row * a.V;
   // Whole vectors of the slice: [v0, v1) as row indices, the rest one by one.
   const int skew = (int)((base + begin) & (N - 1));
@@ -220,7 +226,10 @@ __global__ void __launch_bounds__(kThreads)
       st.top = min(st.top, sh_top[w]);
     }
     ws.stats[blockIdx.x] = st;
-    if (row * ws.slices == (int)blockIdx.x && row % (a.n + 1) == 0) ws.done[row / (a.n + 1)] = 0;
+    if (row * ws.slices == (int)blockIdx.x && row % (a.n + 1) == 0) {
+      ws.done[row / (a.n + 1)] = 0;
+      ws.scale[row / (a.n + 1)] = kTable * 1.4426950408889634 / (double)temp;
+    }
   }
 }
 
@@ -228,15 +237,11 @@ __global__ void __launch_bounds__(kThreads)
 //
 // e^((l - m) / t): 2^(k / 256) from a table and the rest, at most 1 / 512
 // octave, by the Taylor series to the 3rd power (error 1.4e-13).
-constexpr int kTable = 256;
-static_assert(kTable == kThreads, "a thread fills an entry");
 struct Exp64 {
   const double* table;  // 2^(i / 256), in shared memory
   double k, mk;         // 256 log2(e) / t, and m times that
-  __device__ __forceinline__ Exp64(const double* table_, float m, float t) : table(table_) {
-    k = kTable * 1.4426950408889634 / (double)t;
-    mk = (double)m * k;
-  }
+  __device__ __forceinline__ Exp64(const double* table_, float m, double k_)
+      : table(table_), k(k_), mk((double)m * k_) {}
   // The value, where `some`; it is 0 otherwise (below 2^-1000, and at -inf).
   __device__ __forceinline__ double operator()(float l, bool& some) const {
     constexpr double kMagic = 6755399441055744.0;            // 1.5 * 2^52
@@ -262,6 +267,15 @@ struct Exp64 {
 __device__ __forceinline__ double warp_sum(double v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+__device__ __forceinline__ double warp_scan(double v) {  // inclusive
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const double u = __shfl_up_sync(0xffffffffu, v, o);
+    if ((int)(threadIdx.x & 31) >= o) v += u;
+  }
   return v;
 }
 
@@ -349,10 +363,11 @@ __global__ void __launch_bounds__(kThreads) weigh_kernel(const VerifyArgs a, con
   __shared__ Row rows[256];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int b = blockIdx.x / ws.chunks, chunk = blockIdx.x - b * ws.chunks, V = a.V, n = a.n;
-  table[tid] = exp2((double)tid / kTable);
   rl::pdl_wait();
   rl::pdl_launch_dependents();
+  table[tid] = ws.table[tid];
   const float t = a.temperature[b];
+  const double scale = ws.scale[b];
   const int64_t row0 = (int64_t)b * (n + 1);
   auto draft = [&](int i) {
     const int x = i < n ? a.drafts[(int64_t)b * n + i] : -1;
@@ -392,7 +407,7 @@ __global__ void __launch_bounds__(kThreads) weigh_kernel(const VerifyArgs a, con
       if (r.top >= 0) {
         no = !(lhs < (x == r.top ? 1.0 : 0.0));
       } else {
-        const double p = Exp64(table, r.m, t)(Logits<kBf16>(a, row0 + tid)(x));
+        const double p = Exp64(table, r.m, scale)(Logits<kBf16>(a, row0 + tid)(x));
         near = p > 0.0 && fabs(lhs * r.z - p) <= 1e-4 * p;
         no = !(lhs * r.z < p);
       }
@@ -411,7 +426,7 @@ __global__ void __launch_bounds__(kThreads) weigh_kernel(const VerifyArgs a, con
     if (close[acc >> 5] & bit) {
       // The whole CTA sums this row in 64 bits.
       const int x = draft(acc);
-      const Exp64 ex(table, rows[acc].m, t);
+      const Exp64 ex(table, rows[acc].m, scale);
       const Logits<kBf16> logit(a, row0 + acc);
       double z = 0.0;
       over<false>(logit, nullptr, tid, V, kThreads, [&](int, float l, float) { z += ex(l); });
@@ -434,10 +449,10 @@ __global__ void __launch_bounds__(kThreads) weigh_kernel(const VerifyArgs a, con
   }
   if (top >= 0) return;
 
-  // The chunk's sum of exponentials, of which a draft that was chosen outright
+  // The parts' sums of exponentials, of which a draft that was chosen outright
   // (q = 1 there) leaves all but its own.
-  const Exp64 ex(table, rows[acc].m, t);
-  const int drop = a.probs ? -1 : x, c0 = min(V, chunk * ws.chunk), c1 = min(V, c0 + ws.chunk);
+  const Exp64 ex(table, rows[acc].m, scale);
+  const int drop = a.probs ? -1 : x, p = chunk * kWarps + warp, j0 = min(V, p * ws.part), j1 = min(V, j0 + ws.part);
   double sum = 0.0;
   const Logits<kBf16> logit(a, row0 + acc);
   auto add = [&](int, float l, float) {
@@ -445,11 +460,11 @@ __global__ void __launch_bounds__(kThreads) weigh_kernel(const VerifyArgs a, con
     const double w = ex(l, some);
     if (some) sum += w;
   };
-  const int cut = min(max(drop, c0), c1);  // around the dropped token, if it is here
-  over<false>(logit, nullptr, c0 + tid, cut, kThreads, add);
-  over<false>(logit, nullptr, (cut == drop ? cut + 1 : cut) + tid, c1, kThreads, add);
-  sum = block_sum(sum, part);
-  if (tid == 0) ws.z[(int64_t)b * ws.chunks + chunk] = ws.w[(int64_t)b * ws.chunks + chunk] = sum;
+  const int cut = min(max(drop, j0), j1);  // around the dropped token, if it is here
+  over<false>(logit, nullptr, j0 + lane, cut, 32, add);
+  over<false>(logit, nullptr, (cut == drop ? cut + 1 : cut) + lane, j1, 32, add);
+  sum = warp_sum(sum);
+  if (lane == 0) ws.z[(int64_t)b * ws.chunks * kWarps + p] = sum;
 }
 
 // CTA (sequence, chunk): what the draft's distribution leaves of the chunk's
@@ -457,75 +472,71 @@ __global__ void __launch_bounds__(kThreads) weigh_kernel(const VerifyArgs a, con
 // done (its only one otherwise) takes the token.
 template <bool kBf16>
 __global__ void __launch_bounds__(kThreads) pick_kernel(const VerifyArgs a, const Space ws) {
-  __shared__ double table[kTable], part[kWarps];
+  __shared__ double table[kTable];
   __shared__ bool is_last;
   __shared__ int found;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int b = blockIdx.x / ws.chunks, chunk = blockIdx.x - b * ws.chunks, V = a.V, n = a.n;
-  table[tid] = exp2((double)tid / kTable);
   rl::pdl_wait();
   rl::pdl_launch_dependents();
-  __syncthreads();
   const Verdict v = ws.verdict[b];
+  const double scale = ws.scale[b];
+  table[tid] = ws.table[tid];
+  __syncthreads();
   if (v.done) return;
   const bool residual = v.draft >= 0 && a.probs;
-  const int64_t row = (int64_t)b * (n + 1) + v.acc, first = (int64_t)b * ws.chunks;
+  const int parts = ws.chunks * kWarps;
+  const int64_t row = (int64_t)b * (n + 1) + v.acc, first = (int64_t)b * parts;
   const float* q = residual ? a.probs + ((int64_t)b * n + v.acc) * V : nullptr;
   const Logits<kBf16> logit(a, row);
-  const Exp64 ex(table, v.m, a.temperature[b]);
-  double z = 0.0;
+  const Exp64 ex(table, v.m, scale);
+  double total = sum_of(ws.z + first, parts);
+  const double z = total;
+  const double* w = ws.z + first;
   bool taken_off = residual;  // weights are max(0, e - q z), or e
   auto weight = [&](float l, float x) {
     const double e = ex(l);
     return taken_off ? fma(-(double)x, z, e) : e;
   };
   if (residual) {
-    z = sum_of(ws.z + first, ws.chunks);
-    const int c0 = min(V, chunk * ws.chunk), c1 = min(V, c0 + ws.chunk);
+    const int p = chunk * kWarps + warp, j0 = min(V, p * ws.part), j1 = min(V, j0 + ws.part);
     double sum = 0.0;
-    over<true>(logit, q, c0 + tid, c1, kThreads, [&](int, float l, float x) {
-      const double w = weight(l, x);
-      if (w > 0.0) sum += w;
+    over<true>(logit, q, j0 + lane, j1, 32, [&](int, float l, float x) {
+      const double y = weight(l, x);
+      if (y > 0.0) sum += y;
     });
-    sum = block_sum(sum, part);
-    if (tid == 0) {
-      ws.w[first + chunk] = sum;
-      __threadfence();
-      is_last = atomicAdd(&ws.done[b], 1u) == (unsigned)ws.chunks - 1;
-    }
+    sum = warp_sum(sum);
+    if (lane == 0) ws.w[first + p] = sum;
+    __threadfence();
+    __syncthreads();
+    if (tid == 0) is_last = atomicAdd(&ws.done[b], 1u) == (unsigned)ws.chunks - 1;
     __syncthreads();
     if (!is_last) return;
     __threadfence();
+    const double left = sum_of(ws.w + first, parts);
+    if (left > 0.0) {
+      w = ws.w + first;
+      total = left;
+    } else {
+      taken_off = false;  // p == q: nothing is left over; p itself
+    }
   } else if (chunk != 0) {
     return;
   }
 
-  // The total; where nothing is left over (p == q), p itself.
-  const double* w = ws.w + first;
-  double total = sum_of(w, ws.chunks);
-  if (!(total > 0.0) && residual) {
-    taken_off = false;
-    w = ws.z + first;
-    total = z;
-  }
   const int drop = a.probs ? -1 : v.draft;
   if (!(total > 0.0)) {  // all of p on the draft that was chosen outright
     if (tid == 0) a.tokens[row] = max(drop, 0);
     return;
   }
   // The first token whose cumulative weight exceeds the target lies in the
-  // first chunk whose end does.
+  // first part whose end does.
   const double target = (double)a.sample_u[b] * total;
   int at = -1, some = -1;
   double start = 0.0;
-  for (int c = 0; c < ws.chunks && at < 0; c += 32) {
-    const double y = c + lane < ws.chunks ? __ldcg(w + c + lane) : 0.0;
-    double upto = y;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const double u = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += u;
-    }
+  for (int c = 0; c < parts && at < 0; c += 32) {
+    const double y = c + lane < parts ? __ldcg(w + c + lane) : 0.0;
+    const double upto = warp_scan(y);
     const unsigned with = __ballot_sync(0xffffffffu, y > 0.0);
     const unsigned beyond = __ballot_sync(0xffffffffu, start + upto > target) & with;
     if (with) some = c + 31 - __clz(with);
@@ -540,65 +551,52 @@ __global__ void __launch_bounds__(kThreads) pick_kernel(const VerifyArgs a, cons
   }
   if (at < 0) {
     // A number of 1 or more, or none (NaN), or one that rounds up to the
-    // total: the last token with weight, which chunk `some` holds.
+    // total: the last token with weight, which part `some` holds.
     if (tid == 0) found = 0;
     __syncthreads();
-    const int c0 = min(V, some * ws.chunk), c1 = min(V, c0 + ws.chunk);
+    const int j0 = min(V, some * ws.part), j1 = min(V, j0 + ws.part);
     int last = 0;
-    for (int j = c0 + tid; j < c1; j += kThreads)
+    for (int j = j0 + tid; j < j1; j += kThreads)
       if (j != drop && weight(logit(j), taken_off ? q[j] : 0.f) > 0.0) last = j;
     atomicMax(&found, last);
     __syncthreads();
     if (tid == 0) a.tokens[row] = found;
     return;
   }
-  // Within the chunk a warp takes an eighth.
-  const int c0 = min(V, at * ws.chunk), c1 = min(V, c0 + ws.chunk), per = (c1 - c0 + kWarps - 1) / kWarps;
-  const int j0 = min(c1, c0 + warp * per), j1 = min(c1, j0 + per);
-  double mine = 0.0;
-  auto add = [&](int j, float l, float x) {
-    const double y = weight(l, x);
-    if (y > 0.0 && j != drop) mine += y;
-  };
-  if (taken_off) over<true>(logit, q, j0 + lane, j1, 32, add);
-  else over<false>(logit, nullptr, j0 + lane, j1, 32, add);
-  block_sum(mine, part);  // leaves the warps' sums in part
-  int owner = -1, upto = -1;
-  double sum = start;
-  for (int i = 0; i < kWarps; ++i) {
-    if (part[i] > 0.0) {
-      upto = i;
-      if (owner < 0 && sum + part[i] > target) {
-        owner = i;
-        start = sum;
-      }
-    }
-    sum += part[i];
-  }
-  if (owner < 0) owner = upto;  // the parts' ends round below their sum
-  if (warp != owner) return;
+  if (warp != 0) return;
+  // Within the part 256 tokens at a time, then 32 of those.
+  constexpr int kStep = 8;
+  const int j0 = at * ws.part, j1 = min(V, j0 + ws.part);
   int hit = -1, last = 0;
-  float l = 0.f, x = 0.f;
-  auto fetch = [&](int j) {
-    if (j < j1) {
-      l = logit(j);
-      if (taken_off) x = q[j];
-    }
-  };
-  fetch(j0 + lane);
-  for (int j = j0; j < j1 && hit < 0; j += 32) {
-    double y = j + lane < j1 && j + lane != drop ? fmax(0.0, weight(l, x)) : 0.0;
-    fetch(j + 32 + lane);
-    const unsigned with = __ballot_sync(0xffffffffu, y > 0.0);
+  for (int j = j0; j < j1 && hit < 0; j += 32 * kStep) {
+    float l[kStep], x[kStep];
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const double u = __shfl_up_sync(0xffffffffu, y, o);
-      if (lane >= o) y += u;
+    for (int e = 0; e < kStep; ++e) {
+      const int i = j + e * 32 + lane;
+      l[e] = i < j1 && i != drop ? logit(i) : -INFINITY;
+      x[e] = i < j1 && taken_off ? q[i] : 0.f;
     }
-    const unsigned beyond = __ballot_sync(0xffffffffu, start + y > target) & with;
-    if (beyond) hit = j + __ffs(beyond) - 1;
-    if (with) last = j + 31 - __clz(with);
-    start += __shfl_sync(0xffffffffu, y, 31);
+    double y[kStep], sum = 0.0;
+#pragma unroll
+    for (int e = 0; e < kStep; ++e) {
+      y[e] = fmax(0.0, weight(l[e], x[e]));
+      sum += y[e];
+    }
+    sum = warp_sum(sum);
+    if (start + sum > target || j + 32 * kStep >= j1) {
+#pragma unroll
+      for (int e = 0; e < kStep; ++e) {
+        const double upto = warp_scan(y[e]);
+        const unsigned with = __ballot_sync(0xffffffffu, y[e] > 0.0);
+        const unsigned beyond = __ballot_sync(0xffffffffu, start + upto > target) & with;
+        if (hit < 0 && beyond) hit = j + e * 32 + __ffs(beyond) - 1;
+        if (with) last = j + e * 32 + 31 - __clz(with);
+        start += __shfl_sync(0xffffffffu, upto, 31);
+      }
+    } else {
+      if (sum > 0.0) last = j;  // replaced by a later one, or the sums differ in their last bits
+      start += sum;
+    }
   }
   if (lane == 0) a.tokens[row] = hit >= 0 ? hit : last;
 }
@@ -616,17 +614,19 @@ Space space_of(int num_sms, int B, int n, int V, void* base, uint64_t* bytes) {
   s.slices = pick(8ll * num_sms, rows, 65536);
   s.slice = (V + s.slices - 1) / s.slices;
   s.chunks = pick(4ll * num_sms, B, 8192);
-  s.chunk = (V + s.chunks - 1) / s.chunks;
+  s.part = (V + s.chunks * kWarps - 1) / (s.chunks * kWarps);
   uint64_t at = 0;
   auto take = [&](uint64_t size) {
     char* p = static_cast<char*>(base) + at;
     at += (size + 15) / 16 * 16;
     return p;
   };
-  const uint64_t chunks = (uint64_t)B * s.chunks;
+  const uint64_t parts = (uint64_t)B * s.chunks * kWarps;
   s.stats = reinterpret_cast<Stat*>(take((uint64_t)rows * s.slices * sizeof(Stat)));
-  s.z = reinterpret_cast<double*>(take(chunks * 8));
-  s.w = reinterpret_cast<double*>(take(chunks * 8));
+  s.table = reinterpret_cast<double*>(take(kTable * 8));
+  s.scale = reinterpret_cast<double*>(take((uint64_t)B * 8));
+  s.z = reinterpret_cast<double*>(take(parts * 8));
+  s.w = reinterpret_cast<double*>(take(parts * 8));
   s.verdict = reinterpret_cast<Verdict*>(take((uint64_t)B * sizeof(Verdict)));
   s.done = reinterpret_cast<unsigned*>(take((uint64_t)B * 4));
   *bytes = at;
