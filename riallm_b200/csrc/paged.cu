@@ -324,6 +324,22 @@ struct Cursor {
   }
 };
 
+// The workspace begins with a record for every share: the group that it is
+// the first to hold part of, when others hold the rest.
+struct alignas(16) Cut {
+  int x, kh;   // the group
+  int parts;   // shares that hold part of it, this one the first (0: none)
+  int second;  // whether this share's part is in its second slot
+};
+constexpr uint64_t cuts_bytes(int G) { return ((uint64_t)G * sizeof(Cut) + 255) / 256 * 256; }
+// The record of share c, which ends at block i1 of the cursor's group.
+template <typename Sh>
+__device__ __forceinline__ Cut cut_of(const UnitAt& at, const Cursor<Sh>& c, int i0, int i1, int share, bool second) {
+  Cut r{c.x, c.kh, 0, second ? 1 : 0};
+  if (i0 == 0 && i1 < c.t.bl.n) r.parts = share_of(at.W, at.G, c.at0 + c.t.bl.n - 1) - share + 1;
+  return r;
+}
+
 // A share leaves at most two partial results, in slots 2c and 2c + 1: of the
 // group it begins with, and of one that begins inside it. A slot holds the
 // maxima, the sums and the accumulators of a tile's rows, [D][R] (a thread
@@ -393,7 +409,7 @@ constexpr int kFewSmem = kFewStages<D> * (kFewWarps * 2 + 1) * 16 * D * 2;
 
 template <int D>
 __global__ void __launch_bounds__(kFewWarps * 32, 2)
-    few_rows_kernel(const AttnArgs a, int tiles, float* __restrict__ ws) {
+    few_rows_kernel(const AttnArgs a, int tiles, Cut* __restrict__ cuts, float* __restrict__ ws) {
   constexpr int S = kFewStages<D>, C = D / 8;
   extern __shared__ __align__(128) uint16_t smem[];
   __shared__ float sm_m[kFewWarps][16], sm_l[kFewWarps][16];
@@ -401,6 +417,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
   rl::pdl_launch_dependents();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const UnitAt at = find_unit<Few, kFewWarps * 32>(a, tiles, gridDim.x, blockIdx.x);
+  if (cuts && threadIdx.x == 0) cuts[blockIdx.x].parts = 0;
   if (at.u >= at.W) return;
   Cursor<Few> now;
   now.init(a, tiles, at, blockIdx.x);
@@ -652,6 +669,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
               make_uint2(rl::pack_bf16x2(y.x * inv, y.y * inv), rl::pack_bf16x2(y.z * inv, y.w * inv));
         } else {
           *reinterpret_cast<float4*>(slot + 32 + r * D + c) = y;
+          if (x == 0) cuts[blockIdx.x] = cut_of(at, now, now.i - (n - first), now.i + 1, blockIdx.x, first != 0);
           if (c == 0) {
             slot[r] = M;
             slot[16 + r] = L;
@@ -743,7 +761,8 @@ struct Segments {
 template <int D, bool kTwoTiles>
 __global__ void __launch_bounds__(kManyThreads, 1)
     many_rows_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap,
-                     const __grid_constant__ CUtensorMap vmap, int tiles, float* __restrict__ ws, int* status) {
+                     const __grid_constant__ CUtensorMap vmap, int tiles, Cut* __restrict__ cuts,
+                     float* __restrict__ ws, int* status) {
   using Sh = Many<kTwoTiles>;
   constexpr int S = kManyStages<D>, H = D / 64, kHalf = 128 * 128;  // a tile is H column halves of 128 x 128 B
   extern __shared__ uint8_t smem_raw[];
@@ -796,6 +815,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
     Segments<Sh> sg;
     const bool work = at.u < at.W && sg.init(a, tiles, at, blockIdx.x);
+    if (cuts && !work && warp == 8 && lane == 0) cuts[blockIdx.x].parts = 0;
     if (work && warp == 8) {
       // ------------------------------------------------ loads
       const int per_page = 1 << a.pg.lg, pages = 128 >> a.pg.lg;
@@ -950,6 +970,8 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       int n = 0, seg = 0;
       bool go = true;
       do {
+        // The last segment's is the one that stays.
+        if (cuts && warp == 10 && lane == 0) cuts[blockIdx.x] = cut_of(at, sg.c, sg.i0, sg.i1, blockIdx.x, seg > 0);
         for (int i = sg.i0; go && i < sg.i1; ++i, ++n) {
           const int ld = 2 * n + 1, st = ld % S, j0 = sg.c.t.bl.index(i) * 128;
           go = warp_wait(&bars.full[st], (ld / S) & 1, abort, status);
@@ -1247,32 +1269,25 @@ __global__ void __launch_bounds__(kManyThreads, 1)
 }
 
 // CTA (c, y) adds up rows kJoinRows y .. of the partial results of the group
-// that the boundary between the shares c and c + 1 cuts, if c is the first
-// that holds part of it.
+// that share c's record names.
 constexpr int kMaxShares = 320, kJoinThreads = 256;
 template <typename Sh>
 constexpr int kJoinRows = kByColumn<Sh> ? 32 : 16;
 template <typename Sh, int D>
 __global__ void __launch_bounds__(kJoinThreads)
-    join_kernel(const AttnArgs a, int tiles, int G, const float* __restrict__ ws) {
+    join_kernel(const AttnArgs a, int tiles, const Cut* __restrict__ cuts, const float* __restrict__ ws) {
   constexpr int kSlot = kSlotFloats<Sh, D>, kRows = kJoinRows<Sh>;
   __shared__ float weight[kRows][kMaxShares + 1];  // of the parts
   rl::pdl_wait();
   rl::pdl_launch_dependents();
-  const int c0 = blockIdx.x;
-  const UnitAt at = find_unit<Sh, kJoinThreads>(a, tiles, G, c0 + 1);
-  if (at.u >= at.W) return;
-  Cursor<Sh> cut;
-  cut.init(a, tiles, at, c0 + 1);
-  const int64_t last = cut.at0 + cut.t.bl.n - 1;
-  if (cut.i == 0 || share_of(at.W, at.G, cut.at0) != c0) return;  // not cut here, or cut before as well
-  const int row0 = blockIdx.y * kRows, rows = min(kRows, cut.t.rows - row0);
+  const int c0 = blockIdx.x, row0 = blockIdx.y * kRows;
+  const Cut cut = cuts[c0];
+  const int parts = cut.parts;
+  if (parts == 0) return;
+  const Tile t = tile_of<Sh>(a, tiles, cut.x);
+  const int rows = min(kRows, t.rows - row0);
   if (rows <= 0) return;
-  const int parts = share_of(at.W, at.G, last) - c0 + 1;
-  // The first part is in its CTA's second slot where that share begins with
-  // another group.
-  const float* first =
-      ws + (2 * (int64_t)c0 + (share_begin(at.W, at.G, c0) < cut.at0 - Sh::kCost ? 1 : 0)) * kSlot;
+  const float* first = ws + (2 * (int64_t)c0 + cut.second) * kSlot;
   const float* rest = ws + 2 * (int64_t)c0 * kSlot;
   constexpr int kPer = kJoinThreads / kRows;  // neighbouring threads of a row
   {
@@ -1324,7 +1339,7 @@ __global__ void __launch_bounds__(kJoinThreads)
       y.z = fmaf(w, z.z, y.z);
       y.w = fmaf(w, z.w, y.w);
     }
-    *reinterpret_cast<uint2*>(a.out + head_of(a, cut.t, cut.kh, row0 + r) * D + c) =
+    *reinterpret_cast<uint2*>(a.out + head_of(a, t, cut.kh, row0 + r) * D + c) =
         make_uint2(rl::pack_bf16x2(y.x, y.y), rl::pack_bf16x2(y.z, y.w));
   }
 }
@@ -1348,31 +1363,41 @@ Plan make_plan(int num_sms, int B, int T, int nh, int nkv, int d, int64_t cap) {
   const int64_t most = (int64_t)B * nkv * p.tiles * blocks;
   p.G = (int)std::min<int64_t>(std::min((p.kind == Plan::kFew ? 2 : 1) * num_sms, kMaxShares), most);
   p.join = blocks > 1 && p.G > 1;
-  p.ws_bytes = p.join ? (uint64_t)2 * p.G * p.R * (d + 2) * sizeof(float) : 0;
+  p.ws_bytes = p.join ? cuts_bytes(p.G) + (uint64_t)2 * p.G * p.R * (d + 2) * sizeof(float) : 0;
   return p;
 }
 
+// The workspace of a call: records, then partial results (NULL where no group
+// can be cut).
+struct Space {
+  Cut* cuts;
+  float* slots;
+};
+
 template <typename Sh, int D>
-int32_t launch_join(riallm_ctx* ctx, const AttnArgs& a, const Plan& p, const float* ws, cudaStream_t st) {
+int32_t launch_join(riallm_ctx* ctx, const AttnArgs& a, const Plan& p, const Space& ws, cudaStream_t st) {
   if (!p.join) return RIALLM_OK;
+  // The last share is nobody's first of several.
+  const int rows = std::min<int64_t>(Sh::R, (int64_t)a.T * a.rep);
   return rl::launched(ctx, "paged_attention",
-                      rl::launch_pdl(join_kernel<Sh, D>, dim3(p.G - 1, Sh::R / kJoinRows<Sh>), dim3(kJoinThreads), 0, st, a, p.tiles,
-                                     p.G, ws));
+                      rl::launch_pdl(join_kernel<Sh, D>, dim3(p.G - 1, (rows + kJoinRows<Sh> - 1) / kJoinRows<Sh>),
+                                     dim3(kJoinThreads), 0, st, a, p.tiles, static_cast<const Cut*>(ws.cuts),
+                                     static_cast<const float*>(ws.slots)));
 }
 
 template <int D>
-int32_t launch_few(riallm_ctx* ctx, const AttnArgs& a, const Plan& p, float* ws, cudaStream_t st) {
+int32_t launch_few(riallm_ctx* ctx, const AttnArgs& a, const Plan& p, const Space& ws, cudaStream_t st) {
   const char* what = "paged_attention";
   if (int s = rl::allow_smem(ctx, what, few_rows_kernel<D>, kFewSmem<D>, D / 64 - 1)) return s;
   if (int s = rl::launched(ctx, what,
                            rl::launch_pdl(few_rows_kernel<D>, dim3(p.G), dim3(kFewWarps * 32), kFewSmem<D>, st, a,
-                                          p.tiles, ws)))
+                                          p.tiles, ws.cuts, ws.slots)))
     return s;
   return launch_join<Few, D>(ctx, a, p, ws, st);
 }
 
 template <int D, bool kTwoTiles>
-int32_t launch_many(riallm_ctx* ctx, const AttnArgs& a, const Plan& p, float* ws, cudaStream_t st) {
+int32_t launch_many(riallm_ctx* ctx, const AttnArgs& a, const Plan& p, const Space& ws, cudaStream_t st) {
   const char* what = "paged_attention";
   const auto kernel = many_rows_kernel<D, kTwoTiles>;
   if (int s = rl::allow_smem(ctx, what, kernel, kManySmem<D>, 2 + (D / 64 - 1) * 2 + kTwoTiles)) return s;
@@ -1385,13 +1410,13 @@ int32_t launch_many(riallm_ctx* ctx, const AttnArgs& a, const Plan& p, float* ws
   }
   if (int s = rl::launched(ctx, what,
                            rl::launch_pdl(kernel, dim3(p.G), dim3(kManyThreads), kManySmem<D>, st, a, map[0], map[1],
-                                          p.tiles, ws, ctx->d_status)))
+                                          p.tiles, ws.cuts, ws.slots, ctx->d_status)))
     return s;
   return launch_join<Many<kTwoTiles>, D>(ctx, a, p, ws, st);
 }
 
 template <int D>
-int32_t launch_attention(riallm_ctx* ctx, const AttnArgs& a, const Plan& p, float* ws, cudaStream_t st) {
+int32_t launch_attention(riallm_ctx* ctx, const AttnArgs& a, const Plan& p, const Space& ws, cudaStream_t st) {
   return p.kind == Plan::kFew       ? launch_few<D>(ctx, a, p, ws, st)
          : p.kind == Plan::kOneTile ? launch_many<D, false>(ctx, a, p, ws, st)
                                     : launch_many<D, true>(ctx, a, p, ws, st);
@@ -1502,7 +1527,10 @@ int32_t riallm_cuda_paged_attention(riallm_ctx* ctx, const void* q, const void* 
     a.window = window, a.sinks = sinks;
     a.scale_log2 = (float)(1.4426950408889634 / sqrt((double)d));
     a.out = static_cast<uint16_t*>(out);
-    float* ws = static_cast<float*>(workspace);
+    Space ws{nullptr, nullptr};
+    if (p.join)
+      ws = Space{static_cast<Cut*>(workspace),
+                 reinterpret_cast<float*>(static_cast<char*>(workspace) + cuts_bytes(p.G))};
     cudaStream_t st = (cudaStream_t)stream;
     return d == 128 ? launch_attention<128>(ctx, a, p, ws, st) : launch_attention<64>(ctx, a, p, ws, st);
   });
