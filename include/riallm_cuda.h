@@ -435,7 +435,7 @@ int32_t riallm_cuda_linear_bf16(riallm_ctx* ctx, const void* x, const void* w, v
  * page that the sequence does not hold: its positions are neither written
  * nor read. One page may stand in several sequences' tables (a shared
  * prefix) as long as no call appends to it. page_size is 16, 32, 64 or 128;
- * d is 64 or 128; nh / nkv at most 16. No riallm counterpart: its KVCACHE
+ * d is 64 or 128; nh / nkv at most 128. No riallm counterpart: its KVCACHE
  * (src/model.rs:15-38) is one contiguous tensor per layer. These functions
  * leave the calling thread's current device as it was. */
 
@@ -473,7 +473,10 @@ uint64_t riallm_cuda_paged_attention_workspace(const riallm_ctx* ctx, int32_t B,
  * does not see, infinities and NaN among it, does not change that row.
  * The workspace is the caller's (256-byte aligned), needs no initial values,
  * and is free again when the call's work is done on `stream`; calls that may
- * overlap need one each. Nothing else is shared between calls. */
+ * overlap need one each. Nothing else is shared between calls. The kernel
+ * for prompts waits for its own loads and products with a bound (1 s); past
+ * it the call's output is undefined and riallm_cuda_stream_synchronize
+ * returns RIALLM_ERR_TIMEOUT. */
 int32_t riallm_cuda_paged_attention(riallm_ctx* ctx, const void* q, const void* k_pages, const void* v_pages,
                                     const int32_t* pos, const int32_t* page_table, int64_t table_stride,
                                     int32_t max_pages, int32_t B, int32_t T, int32_t nh, int32_t nkv, int32_t d,

@@ -17,7 +17,6 @@
 namespace {
 
 __device__ __forceinline__ float bf2f(uint16_t b) { return __uint_as_float((uint32_t)b << 16); }
-__device__ __forceinline__ uint16_t f2bf(float f) { return __bfloat16_as_ushort(__float2bfloat16_rn(f)); }
 
 // The page table and the geometry of the pools.
 struct Pages {
@@ -206,8 +205,8 @@ struct Tile {
   Blocks bl;
 };
 // Token of row r of a tile, counted from the tile's first: (head0 + r) / rep.
-// rep is at most 16 and r below 256, so rounding 1 / rep up adds less than
-// 2^-20 to the quotient.
+// rep is at most 128 and r below 256, so rounding 1 / rep up adds less than
+// 2^-16 to the quotient.
 __device__ __forceinline__ int token_of(const AttnArgs& a, const Tile& t, int r) {
   return a.rep == 1 ? r : (int)__umulhi((uint32_t)(t.head0 + r), a.rep_inv);
 }
@@ -1430,7 +1429,7 @@ int check_pages(riallm_ctx* ctx, const char* what, int32_t B, int32_t T, int32_t
   auto bad = [&](const char* msg) { return rl::refuse(ctx, RIALLM_ERR_CONFIG, what, msg); };
   if (B < 0 || T < 0 || nh <= 0 || nkv <= 0 || nh % nkv != 0)
     return bad("bad dimensions (heads must be a multiple of kv heads)");
-  if (nh / nkv > 16) return bad("more than 16 heads per kv head");
+  if (nh / nkv > 128) return bad("more than 128 heads per kv head");
   if (d != 64 && d != 128) return bad("head_dim must be 64 or 128");
   if (page_size != 16 && page_size != 32 && page_size != 64 && page_size != 128)
     return bad("page_size must be 16, 32, 64 or 128");
@@ -1507,6 +1506,8 @@ int32_t riallm_cuda_paged_attention(riallm_ctx* ctx, const void* q, const void* 
   if (int s = check_pages(ctx, what, B, T, nh, nkv, d, num_pages, page_size, max_pages, table_stride)) return s;
   if (window < 0 || sinks < 0)
     return rl::refuse(ctx, RIALLM_ERR_CONFIG, what, "window and sinks must not be negative");
+  if ((int64_t)B * T * (nh / nkv) > INT32_MAX / 2)
+    return rl::refuse(ctx, RIALLM_ERR_CONFIG, what, "too many rows");
   if (ctx && (int64_t)B * T == 0) return RIALLM_OK;
   if (!ctx || !q || !k_pages || !v_pages || !pos || !page_table || !out)
     return rl::refuse(ctx, RIALLM_ERR_INVALID, what, "NULL argument");

@@ -155,7 +155,7 @@ __global__ void __launch_bounds__(kThreads)
   if (blockIdx.x == 0) ws.table[tid] = exp2((double)tid / kTable);
   const int64_t base = (int64_t)row * a.V;
   // Whole vectors of the slice: [v0, v1) as row indices, the rest one by one.
-  const int skew = (int)((base + begin) & (N - 1));
+  const int skew = (int)((reinterpret_cast<uintptr_t>(a.logits) / (kBf16 ? 2 : 4) + base + begin) & (N - 1));
   const int v0 = min(end, begin + (skew ? N - skew : 0)), v1 = v0 + (end - v0) / N * N;
   const uint4* vec = reinterpret_cast<const uint4*>(static_cast<const char*>(a.logits) + (base + v0) * (kBf16 ? 2 : 4));
   const int nv = (v1 - v0) / N;
@@ -239,14 +239,13 @@ __global__ void __launch_bounds__(kThreads)
 // octave, by the Taylor series to the 3rd power (error 1.4e-13).
 struct Exp64 {
   const double* table;  // 2^(i / 256), in shared memory
-  double k, mk;         // 256 log2(e) / t, and m times that
-  __device__ __forceinline__ Exp64(const double* table_, float m, double k_)
-      : table(table_), k(k_), mk((double)m * k_) {}
+  double k, m;          // 256 log2(e) / t
+  __device__ __forceinline__ Exp64(const double* table_, float m_, double k_) : table(table_), k(k_), m((double)m_) {}
   // The value, where `some`; it is 0 otherwise (below 2^-1000, and at -inf).
   __device__ __forceinline__ double operator()(float l, bool& some) const {
     constexpr double kMagic = 6755399441055744.0;            // 1.5 * 2^52
     constexpr double a = 0.6931471805599453 / kTable;
-    const double x = fma((double)l, k, -mk);
+    const double x = ((double)l - m) * k;  // in this order: 0 at the maximum, whatever the temperature
     const double xf = x + kMagic;
     const int i = __double2loint(xf);
     const double r = x - (xf - kMagic);
@@ -668,8 +667,8 @@ int32_t riallm_cuda_verify_draft(riallm_ctx* ctx, const void* logits, int32_t lo
   if (ctx && B == 0) return RIALLM_OK;
   if (!ctx || !logits || !temperature || !sample_u || !tokens || !accepted || (n > 0 && (!draft_tokens || !accept_u)))
     return rl::refuse(ctx, RIALLM_ERR_INVALID, what, "NULL argument");
-  if (reinterpret_cast<uintptr_t>(logits) & 15)
-    return rl::refuse(ctx, RIALLM_ERR_INVALID, what, "logits must be 16-byte aligned");
+  if (reinterpret_cast<uintptr_t>(logits) & (logits_dtype == RIALLM_DTYPE_BF16 ? 1 : 3))
+    return rl::refuse(ctx, RIALLM_ERR_INVALID, what, "logits must be aligned to their type");
   uint64_t bytes;
   const Space ws = space_of(ctx->num_sms, B, n, V, workspace, &bytes);
   if (!workspace || workspace_bytes < bytes || (reinterpret_cast<uintptr_t>(workspace) & 15))

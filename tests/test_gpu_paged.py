@@ -123,6 +123,10 @@ SHAPES = [
     (2, 65, 16, 2, 64, 64, [65, 300]),
     (1, 257, 8, 1, 128, 128, [400]),
     (1, 40, 48, 8, 128, 16, [555]),
+    (2, 1, 32, 1, 128, 16, [90, 300]),
+    (1, 1, 128, 1, 64, 32, [700]),
+    (2, 3, 64, 1, 64, 16, [40, 130]),
+    (1, 5, 33, 1, 128, 64, [200]),
 ]
 
 
@@ -253,7 +257,7 @@ def test_attention_out_and_refusals(rb):
     check(out, reference(s))
     for bad in (dict(q=s["q"].float()), dict(k=s["k"].transpose(1, 2)), dict(v=s["v"][:2]),
                 dict(pos=s["pos"].long()), dict(table=s["table"].long()), dict(table=s["table"].cpu()),
-                dict(q=s["q"][:, :100]), dict(q=s["q"][:, ::2]), dict(q=torch.cat([s["q"]] * 17, 1)),
+                dict(q=s["q"][:, :100]), dict(q=s["q"][:, ::2]), dict(q=torch.cat([s["q"]] * 65, 1)),
                 dict(table=torch.cat([s["table"]] * 2))):
         with pytest.raises(rb.ConfigError):
             attend(rb, dict(s, **bad))

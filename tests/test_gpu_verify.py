@@ -97,6 +97,27 @@ def test_all_accepted_and_all_rejected(rb):
     assert (check(rb, a)[1] == 0).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_any_place_and_extreme_temperatures(rb, dtype):
+    """Logits that begin at any element, and temperatures from the smallest
+    number to infinity (all weights alike) and NaN (greedy)."""
+    B, n, V = 7, 2, 1003
+    for shift in range(4):
+        a = inputs(B, n, V, seed=shift, dtype=dtype)
+        a[4] = torch.tensor([1e-45, 1e-10, 1e-2, 1e6, 3e38, INF, NAN])
+        a[0][:, :, 5] = -INF
+        # An infinite temperature as the number it tends to: finite logits alike.
+        flat = [x.clone() for x in a]
+        flat[0][5][torch.isfinite(flat[0][5])] = 0.0
+        flat[4][5] = 1.0
+        want = reference(*flat)
+        d = [x.cuda() for x in a]
+        room = torch.empty(d[0].numel() + 8, dtype=dtype, device="cuda")
+        place = room[shift:shift + d[0].numel()].view(B, n + 1, V).copy_(d[0])
+        got = rb.verify_draft(place, d[1], d[2], d[3], temperature=d[4], draft_probs=d[5])
+        assert torch.equal(got[0].cpu(), want[0]) and torch.equal(got[1].cpu(), want[1])
+
+
 def test_draft_ends_early(rb):
     a = inputs(6, 4, 500)
     a[2].zero_()

@@ -86,7 +86,7 @@ def _attend(L, B=1, T=1, nh=8, nkv=2, d=128, num_pages=4, ps=16, max_pages=2, st
 
 
 @pytest.mark.parametrize("call", [_append, _attend])
-@pytest.mark.parametrize("bad", [dict(B=-1), dict(T=-1), dict(nh=0), dict(nh=7), dict(nh=34, nkv=2), dict(d=96),
+@pytest.mark.parametrize("bad", [dict(B=-1), dict(T=-1), dict(nh=0), dict(nh=7), dict(nh=258, nkv=2), dict(d=96),
                                  dict(d=0), dict(ps=8), dict(ps=48), dict(ps=256), dict(num_pages=0),
                                  dict(max_pages=0), dict(stride=1), dict(num_pages=2**26, nkv=2, nh=2),
                                  dict(max_pages=2**28, stride=2**28), dict(B=2**20, T=2**20),
