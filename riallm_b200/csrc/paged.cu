@@ -1267,80 +1267,99 @@ __global__ void __launch_bounds__(kManyThreads, 1)
   if (warp == 9) rl::tmem_dealloc(tm, 512);
 }
 
-// CTA (c, y) adds up rows kJoinRows y .. of the partial results of the group
-// that share c's record names.
+// CTA (c, y, z) adds up kRows rows from kRows y on, 4 * kCols columns from
+// there times z on, of the partial results of the group that share c's record
+// names. A thread takes 4 columns of a row; where a group has many parts and
+// few rows, several threads share its parts.
 constexpr int kMaxShares = 320, kJoinThreads = 256;
-template <typename Sh>
-constexpr int kJoinRows = kByColumn<Sh> ? 32 : 16;
+template <typename Sh, int D>
+struct Join {
+  static constexpr bool kMany = kByColumn<Sh>;
+  static constexpr int kRows = kMany ? 32 : 2;
+  static constexpr int kCols = kMany ? 8 : D / 4;
+  static constexpr int kShared = kJoinThreads / (kRows * kCols);
+  static constexpr int kZ = D / (4 * kCols);
+  static constexpr int kPer = kMany ? kJoinThreads / kRows : 32;  // threads that work out a row's weights
+};
 template <typename Sh, int D>
 __global__ void __launch_bounds__(kJoinThreads)
     join_kernel(const AttnArgs a, int tiles, const Cut* __restrict__ cuts, const float* __restrict__ ws) {
-  constexpr int kSlot = kSlotFloats<Sh, D>, kRows = kJoinRows<Sh>;
-  __shared__ float weight[kRows][kMaxShares + 1];  // of the parts
+  using J = Join<Sh, D>;
+  constexpr int kSlot = kSlotFloats<Sh, D>;
+  __shared__ float weight[J::kRows][kMaxShares / (J::kMany ? 2 : 1) + 1];  // of the parts
+  __shared__ float4 red[J::kShared > 1 ? kJoinThreads : 1];
   rl::pdl_wait();
   rl::pdl_launch_dependents();
-  const int c0 = blockIdx.x, row0 = blockIdx.y * kRows;
+  const int c0 = blockIdx.x, row0 = blockIdx.y * J::kRows, tid = threadIdx.x;
   const Cut cut = cuts[c0];
   const int parts = cut.parts;
   if (parts == 0) return;
   const Tile t = tile_of<Sh>(a, tiles, cut.x);
-  const int rows = min(kRows, t.rows - row0);
+  const int rows = min(J::kRows, t.rows - row0);
   if (rows <= 0) return;
   const float* first = ws + (2 * (int64_t)c0 + cut.second) * kSlot;
   const float* rest = ws + 2 * (int64_t)c0 * kSlot;
-  constexpr int kPer = kJoinThreads / kRows;  // neighbouring threads of a row
   {
-    const int r = threadIdx.x / kPer, i0 = threadIdx.x % kPer;
+    const int r = tid / J::kPer, i0 = tid % J::kPer;
     const bool have = r < rows;
     float M = -INFINITY;
     if (have)
-      for (int i = i0; i < parts; i += kPer) {
+      for (int i = i0; i < parts; i += J::kPer) {
         const float x = __ldcg((i ? rest + (int64_t)i * 2 * kSlot : first) + row0 + r);
         weight[r][i] = x;
         M = fmaxf(M, x);
       }
 #pragma unroll
-    for (int o = kPer / 2; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    for (int o = J::kPer / 2; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
     float den = 0.f;
     if (have)
-      for (int i = i0; i < parts; i += kPer) {
+      for (int i = i0; i < parts; i += J::kPer) {
         const float f = M == -INFINITY ? 0.f : ex2(weight[r][i] - M);
         weight[r][i] = f;
         den = fmaf(f, __ldcg((i ? rest + (int64_t)i * 2 * kSlot : first) + Sh::R + row0 + r), den);
       }
 #pragma unroll
-    for (int o = kPer / 2; o > 0; o >>= 1) den += __shfl_xor_sync(0xffffffffu, den, o);
+    for (int o = J::kPer / 2; o > 0; o >>= 1) den += __shfl_xor_sync(0xffffffffu, den, o);
     const float inv = den == 0.f ? 0.f : __fdiv_rn(1.f, den);
     if (have)
-      for (int i = i0; i < parts; i += kPer) weight[r][i] *= inv;
+      for (int i = i0; i < parts; i += J::kPer) weight[r][i] *= inv;
   }
   __syncthreads();
-  // Four columns of a row a thread; neighbours hold neighbouring rows where
-  // the parts are stored by column.
-  for (int x = threadIdx.x; x < kRows * (D / 4); x += kJoinThreads) {
-    const int r = kByColumn<Sh> ? x % kRows : x / (D / 4), c = (kByColumn<Sh> ? x / kRows : x % (D / 4)) * 4;
-    if (r >= rows) continue;
-    auto load = [&](const float* slot) {
-      const float* p = slot + 2 * Sh::R;
-      if (!kByColumn<Sh>) return __ldcg(reinterpret_cast<const float4*>(p + (row0 + r) * D + c));
-      p += c * Sh::R + row0 + r;
-      return make_float4(__ldcg(p), __ldcg(p + Sh::R), __ldcg(p + 2 * Sh::R), __ldcg(p + 3 * Sh::R));
-    };
-    float4 y = load(first);
-    const float w0 = weight[r][0];
-    y.x *= w0, y.y *= w0, y.z *= w0, y.w *= w0;
+  // Neighbours hold neighbouring rows where the parts are stored by column.
+  const int r = J::kMany ? tid % J::kRows : tid / J::kCols % J::kRows;
+  const int c = (blockIdx.z * J::kCols + (J::kMany ? tid / J::kRows : tid % J::kCols)) * 4;
+  const int turn = J::kMany ? 0 : tid / (J::kRows * J::kCols);
+  float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (r < rows) {
 #pragma unroll 8
-    for (int i = 1; i < parts; ++i) {
+    for (int i = turn; i < parts; i += J::kShared) {
+      const float* p = (i ? rest + (int64_t)i * 2 * kSlot : first) + 2 * Sh::R;
+      float4 z;
+      if (J::kMany) {
+        p += c * Sh::R + row0 + r;
+        z = make_float4(__ldcg(p), __ldcg(p + Sh::R), __ldcg(p + 2 * Sh::R), __ldcg(p + 3 * Sh::R));
+      } else {
+        z = __ldcg(reinterpret_cast<const float4*>(p + (row0 + r) * D + c));
+      }
       const float w = weight[r][i];
-      const float4 z = load(rest + (int64_t)i * 2 * kSlot);
       y.x = fmaf(w, z.x, y.x);
       y.y = fmaf(w, z.y, y.y);
       y.z = fmaf(w, z.z, y.z);
       y.w = fmaf(w, z.w, y.w);
     }
+  }
+  if (J::kShared > 1) {
+    red[tid] = y;
+    __syncthreads();
+    if (turn) return;
+    for (int i = 1; i < J::kShared; ++i) {
+      const float4 z = red[i * J::kRows * J::kCols + tid];
+      y.x += z.x, y.y += z.y, y.z += z.z, y.w += z.w;
+    }
+  }
+  if (r < rows)
     *reinterpret_cast<uint2*>(a.out + head_of(a, t, cut.kh, row0 + r) * D + c) =
         make_uint2(rl::pack_bf16x2(y.x, y.y), rl::pack_bf16x2(y.z, y.w));
-  }
 }
 
 // The kernel for a call, its row tiles and CTAs, and whether a group can be
@@ -1360,7 +1379,7 @@ Plan make_plan(int num_sms, int B, int T, int nh, int nkv, int d, int64_t cap) {
   p.tiles = (int)((rows + p.R - 1) / p.R);
   const int64_t blocks = (cap + block - 1) / block;
   const int64_t most = (int64_t)B * nkv * p.tiles * blocks;
-  p.G = (int)std::min<int64_t>(std::min((p.kind == Plan::kFew ? 2 : 1) * num_sms, kMaxShares), most);
+  p.G = (int)std::min<int64_t>(p.kind == Plan::kFew ? std::min(2 * num_sms, kMaxShares) : std::min(num_sms, kMaxShares / 2), most);
   p.join = blocks > 1 && p.G > 1;
   p.ws_bytes = p.join ? cuts_bytes(p.G) + (uint64_t)2 * p.G * p.R * (d + 2) * sizeof(float) : 0;
   return p;
@@ -1379,7 +1398,8 @@ int32_t launch_join(riallm_ctx* ctx, const AttnArgs& a, const Plan& p, const Spa
   // The last share is nobody's first of several.
   const int rows = std::min<int64_t>(Sh::R, (int64_t)a.T * a.rep);
   return rl::launched(ctx, "paged_attention",
-                      rl::launch_pdl(join_kernel<Sh, D>, dim3(p.G - 1, (rows + kJoinRows<Sh> - 1) / kJoinRows<Sh>),
+                      rl::launch_pdl(join_kernel<Sh, D>,
+                                     dim3(p.G - 1, (rows + Join<Sh, D>::kRows - 1) / Join<Sh, D>::kRows, Join<Sh, D>::kZ),
                                      dim3(kJoinThreads), 0, st, a, p.tiles, static_cast<const Cut*>(ws.cuts),
                                      static_cast<const float*>(ws.slots)));
 }
