@@ -453,11 +453,19 @@ int64_t riallm_paged_row(const int32_t* page_table, int64_t table_stride, int32_
  * 100000). A position outside [0, max_pages * page_size), or in a page that
  * the sequence does not hold, writes nothing to the pools. Two rows that are
  * given the same place of a page leave either's values there. */
-int32_t riallm_cuda_rope_paged_append(riallm_ctx* ctx, const void* qkv, const int32_t* pos,
-                                      const int32_t* page_table, int64_t table_stride, int32_t max_pages,
-                                      int32_t B, int32_t T, int32_t nh, int32_t nkv, int32_t d,
-                                      const float* inv_freq, void* q_out, void* k_pages, void* v_pages,
-                                      int32_t num_pages, int32_t page_size, void* stream);
+typedef struct riallm_rope_paged_append_args {
+  const void* qkv;
+  const int32_t* pos;
+  const int32_t* page_table;
+  const float* inv_freq; /* float32 [d / 2] */
+  void* q_out;
+  void* k_pages;
+  void* v_pages;
+  int64_t table_stride;
+  int32_t max_pages, num_pages, page_size;
+  int32_t B, T, nh, nkv, d;
+} riallm_rope_paged_append_args;
+int32_t riallm_cuda_rope_paged_append(riallm_ctx* ctx, const riallm_rope_paged_append_args* args, void* stream);
 
 /* Bytes of workspace that riallm_cuda_paged_attention needs for a call of
  * this shape on the context's device (0: none). */
@@ -477,11 +485,21 @@ uint64_t riallm_cuda_paged_attention_workspace(const riallm_ctx* ctx, int32_t B,
  * for prompts waits for its own loads and products with a bound (1 s); past
  * it the call's output is undefined and riallm_cuda_stream_synchronize
  * returns RIALLM_ERR_TIMEOUT. */
-int32_t riallm_cuda_paged_attention(riallm_ctx* ctx, const void* q, const void* k_pages, const void* v_pages,
-                                    const int32_t* pos, const int32_t* page_table, int64_t table_stride,
-                                    int32_t max_pages, int32_t B, int32_t T, int32_t nh, int32_t nkv, int32_t d,
-                                    int32_t num_pages, int32_t page_size, int32_t window, int32_t sinks, void* out,
-                                    void* workspace, uint64_t workspace_bytes, void* stream);
+typedef struct riallm_paged_attention_args {
+  const void* q;
+  const void* k_pages;
+  const void* v_pages;
+  const int32_t* pos;
+  const int32_t* page_table;
+  void* out;
+  int64_t table_stride;
+  int32_t max_pages, num_pages, page_size;
+  int32_t B, T, nh, nkv, d;
+  int32_t window; /* 0: none */
+  int32_t sinks;
+} riallm_paged_attention_args;
+int32_t riallm_cuda_paged_attention(riallm_ctx* ctx, const riallm_paged_attention_args* args, void* workspace,
+                                    uint64_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------ drafted tokens
  * Bytes of workspace that riallm_cuda_verify_draft needs (0: none). */
@@ -507,11 +525,20 @@ uint64_t riallm_cuda_verify_draft_workspace(const riallm_ctx* ctx, int32_t B, in
  * comparisons are 64-bit, and results do not depend on the order in which
  * blocks run. n <= 255; with n == 0 (one sampled token per sequence)
  * draft_tokens and accept_u may be NULL. Workspace as above. */
-int32_t riallm_cuda_verify_draft(riallm_ctx* ctx, const void* logits, int32_t logits_dtype,
-                                 const int32_t* draft_tokens, const float* draft_probs, const float* temperature,
-                                 const float* accept_u, const float* sample_u, int32_t B, int32_t n, int32_t V,
-                                 int32_t* tokens, int32_t* accepted, void* workspace, uint64_t workspace_bytes,
-                                 void* stream);
+typedef struct riallm_verify_draft_args {
+  const void* logits;
+  const int32_t* draft_tokens;
+  const float* draft_probs;
+  const float* temperature;
+  const float* accept_u;
+  const float* sample_u;
+  int32_t* tokens;
+  int32_t* accepted;
+  int32_t logits_dtype; /* riallm_dtype */
+  int32_t B, n, V;
+} riallm_verify_draft_args;
+int32_t riallm_cuda_verify_draft(riallm_ctx* ctx, const riallm_verify_draft_args* args, void* workspace,
+                                 uint64_t workspace_bytes, void* stream);
 
 int32_t riallm_cuda_profile_enable(riallm_ctx* ctx, int32_t enable);
 int32_t riallm_cuda_profile_read(riallm_ctx* ctx, float* ms_per_phase,

@@ -88,6 +88,9 @@ class CMoeWeights(ctypes.Structure):
 # Every symbol include/riallm_cuda.h declares: name -> (restype, argtypes).
 _i32, _u32, _u64, _vp = ctypes.c_int32, ctypes.c_uint32, ctypes.c_uint64, ctypes.c_void_p
 _i64 = ctypes.c_int64
+# An argument structure of the header as packed bytes (struct, native layout):
+# a fifth of the cost of as many ctypes arguments.
+_args = ctypes.c_char_p
 _pp = ctypes.POINTER(ctypes.c_void_p)
 SIGNATURES = {
     "riallm_cuda_abi_version": (_i32, []),
@@ -150,14 +153,11 @@ SIGNATURES = {
     "riallm_cuda_attention": (_i32, [_vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _vp, _vp]),
     "riallm_cuda_linear_bf16": (_i32, [_vp, _vp, _vp, _vp, _i32, _i32, _i32, _vp]),
     "riallm_paged_row": (_i64, [_vp, _i64, _i32, _i32, _i32, _i32, _i32, _i32, _i64]),
-    "riallm_cuda_rope_paged_append": (_i32, [_vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _i32, _i32, _vp, _vp,
-                                             _vp, _vp, _i32, _i32, _vp]),
+    "riallm_cuda_rope_paged_append": (_i32, [_vp, _args, _vp]),
     "riallm_cuda_paged_attention_workspace": (_u64, [_vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32]),
-    "riallm_cuda_paged_attention": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _i32, _i32,
-                                           _i32, _i32, _i32, _i32, _vp, _vp, _u64, _vp]),
+    "riallm_cuda_paged_attention": (_i32, [_vp, _args, _vp, _u64, _vp]),
     "riallm_cuda_verify_draft_workspace": (_u64, [_vp, _i32, _i32, _i32]),
-    "riallm_cuda_verify_draft": (_i32, [_vp, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _vp, _vp, _vp,
-                                        _u64, _vp]),
+    "riallm_cuda_verify_draft": (_i32, [_vp, _args, _vp, _u64, _vp]),
 }
 
 PHASES = ("route", "gather", "gate_up", "down", "shared", "combine", "dispatch", "return")

@@ -1444,8 +1444,9 @@ int32_t launch_attention(riallm_ctx* ctx, const AttnArgs& a, const Plan& p, cons
 bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 // What both entry points share: the checks of the cache's geometry.
-int check_pages(riallm_ctx* ctx, const char* what, int32_t B, int32_t T, int32_t nh, int32_t nkv, int32_t d,
-                int32_t num_pages, int32_t page_size, int32_t max_pages, int64_t table_stride) {
+template <typename Args>
+int check_pages(riallm_ctx* ctx, const char* what, const Args& x) {
+  const int32_t B = x.B, T = x.T, nh = x.nh, nkv = x.nkv, d = x.d, page_size = x.page_size;
   auto bad = [&](const char* msg) { return rl::refuse(ctx, RIALLM_ERR_CONFIG, what, msg); };
   if (B < 0 || T < 0 || nh <= 0 || nkv <= 0 || nh % nkv != 0)
     return bad("bad dimensions (heads must be a multiple of kv heads)");
@@ -1453,8 +1454,8 @@ int check_pages(riallm_ctx* ctx, const char* what, int32_t B, int32_t T, int32_t
   if (d != 64 && d != 128) return bad("head_dim must be 64 or 128");
   if (page_size != 16 && page_size != 32 && page_size != 64 && page_size != 128)
     return bad("page_size must be 16, 32, 64 or 128");
-  if (num_pages <= 0 || max_pages <= 0 || table_stride < max_pages) return bad("bad page table");
-  if ((int64_t)num_pages * nkv * page_size > INT32_MAX || (int64_t)max_pages * page_size > INT32_MAX)
+  if (x.num_pages <= 0 || x.max_pages <= 0 || x.table_stride < x.max_pages) return bad("bad page table");
+  if ((int64_t)x.num_pages * nkv * page_size > INT32_MAX || (int64_t)x.max_pages * page_size > INT32_MAX)
     return bad("more than 2^31 - 1 cache rows");
   if ((int64_t)B * T > INT32_MAX / 4 || (int64_t)nh + 2 * nkv > 65535) return bad("too many rows or heads");
   return RIALLM_OK;
@@ -1467,6 +1468,71 @@ Pages make_pages(const int32_t* table, int64_t stride, int32_t max_pages, int32_
   return Pages{table, stride, max_pages, num_pages, nkv, lg};
 }
 
+int32_t append(riallm_ctx* ctx, const riallm_rope_paged_append_args& x, cudaStream_t stream) {
+  const char* what = "rope_paged_append";
+  if (int s = check_pages(ctx, what, x)) return s;
+  if (ctx && (int64_t)x.B * x.T == 0) return RIALLM_OK;
+  if (!ctx || !x.qkv || !x.pos || !x.page_table || !x.inv_freq || !x.q_out || !x.k_pages || !x.v_pages)
+    return rl::refuse(ctx, RIALLM_ERR_INVALID, what, "NULL argument");
+  if (!al16(x.qkv) || !al16(x.q_out) || !al16(x.k_pages) || !al16(x.v_pages))
+    return rl::refuse(ctx, RIALLM_ERR_INVALID, what, "buffers must be 16-byte aligned");
+  return rl::guarded(ctx, [&]() -> int32_t {
+    const Pages pg = make_pages(x.page_table, x.table_stride, x.max_pages, x.num_pages, x.nkv, x.page_size);
+    // Heads per CTA: all of a row's units where they fit, fewer where the
+    // rows alone would leave SMs idle; then as many rows as still fit.
+    const int rows = x.B * x.T, heads = x.nh + 2 * x.nkv, per_head = x.d / 16, fit = kAppendThreads * kAppendUnits;
+    int hg = std::min(heads, fit / per_head);
+    const int64_t want = 2ll * ctx->num_sms;
+    if ((int64_t)rows * ((heads + hg - 1) / hg) < want)
+      hg = (int)std::max<int64_t>(std::min(heads, kAppendThreads / per_head / 4), (int64_t)heads * rows / want);
+    hg = std::min(hg, fit / per_head);
+    int per_cta = std::min(kAppendRows, fit / (hg * per_head));
+    per_cta = (int)std::max<int64_t>(1, std::min<int64_t>(per_cta, rows * (int64_t)((heads + hg - 1) / hg) / want));
+    const auto kernel = x.d == 128 ? rope_paged_append_kernel<128> : rope_paged_append_kernel<64>;
+    return rl::launched(ctx, what,
+                        rl::launch_pdl(kernel, dim3((rows + per_cta - 1) / per_cta, (heads + hg - 1) / hg),
+                                       dim3(kAppendThreads), 0, stream, static_cast<const uint16_t*>(x.qkv), x.pos, pg,
+                                       rows, x.T, x.nh, per_cta, hg, x.inv_freq, static_cast<uint16_t*>(x.q_out),
+                                       static_cast<uint16_t*>(x.k_pages), static_cast<uint16_t*>(x.v_pages)));
+  });
+}
+
+int32_t attend(riallm_ctx* ctx, const riallm_paged_attention_args& x, void* workspace, uint64_t workspace_bytes,
+               cudaStream_t stream) {
+  const char* what = "paged_attention";
+  if (int s = check_pages(ctx, what, x)) return s;
+  if (x.window < 0 || x.sinks < 0)
+    return rl::refuse(ctx, RIALLM_ERR_CONFIG, what, "window and sinks must not be negative");
+  if ((int64_t)x.B * x.T * (x.nh / x.nkv) > INT32_MAX / 2)
+    return rl::refuse(ctx, RIALLM_ERR_CONFIG, what, "too many rows");
+  if (ctx && (int64_t)x.B * x.T == 0) return RIALLM_OK;
+  if (!ctx || !x.q || !x.k_pages || !x.v_pages || !x.pos || !x.page_table || !x.out)
+    return rl::refuse(ctx, RIALLM_ERR_INVALID, what, "NULL argument");
+  if (!al16(x.q) || !al16(x.out) || !al16(x.k_pages) || !al16(x.v_pages))
+    return rl::refuse(ctx, RIALLM_ERR_INVALID, what, "buffers must be 16-byte aligned");
+  const Plan p = make_plan(ctx->num_sms, x.B, x.T, x.nh, x.nkv, x.d, (int64_t)x.max_pages * x.page_size);
+  if (p.ws_bytes && (!workspace || workspace_bytes < p.ws_bytes || (reinterpret_cast<uintptr_t>(workspace) & 255)))
+    return rl::refuse(ctx, RIALLM_ERR_MEMORY, what, "workspace missing, too small or not 256-byte aligned");
+  return rl::guarded(ctx, [&]() -> int32_t {
+    AttnArgs a;
+    a.q = static_cast<const uint16_t*>(x.q);
+    a.k = static_cast<const uint16_t*>(x.k_pages);
+    a.v = static_cast<const uint16_t*>(x.v_pages);
+    a.pos = x.pos;
+    a.pg = make_pages(x.page_table, x.table_stride, x.max_pages, x.num_pages, x.nkv, x.page_size);
+    a.B = x.B, a.T = x.T, a.nh = x.nh, a.rep = x.nh / x.nkv;
+    a.rep_inv = (uint32_t)(((1ull << 32) + a.rep - 1) / a.rep);
+    a.window = x.window, a.sinks = x.sinks;
+    a.scale_log2 = (float)(1.4426950408889634 / sqrt((double)x.d));
+    a.out = static_cast<uint16_t*>(x.out);
+    Space ws{nullptr, nullptr};
+    if (p.join)
+      ws = Space{static_cast<Cut*>(workspace),
+                 reinterpret_cast<float*>(static_cast<char*>(workspace) + cuts_bytes(p.G))};
+    return x.d == 128 ? launch_attention<128>(ctx, a, p, ws, stream) : launch_attention<64>(ctx, a, p, ws, stream);
+  });
+}
+
 }  // namespace
 
 extern "C" {
@@ -1477,38 +1543,9 @@ int64_t riallm_paged_row(const int32_t* page_table, int64_t table_stride, int32_
   return make_pages(page_table, table_stride, max_pages, num_pages, nkv, page_size).row(b, kv_head, position);
 }
 
-int32_t riallm_cuda_rope_paged_append(riallm_ctx* ctx, const void* qkv, const int32_t* pos,
-                                      const int32_t* page_table, int64_t table_stride, int32_t max_pages, int32_t B,
-                                      int32_t T, int32_t nh, int32_t nkv, int32_t d, const float* inv_freq,
-                                      void* q_out, void* k_pages, void* v_pages, int32_t num_pages,
-                                      int32_t page_size, void* stream) {
-  const char* what = "rope_paged_append";
-  if (int s = check_pages(ctx, what, B, T, nh, nkv, d, num_pages, page_size, max_pages, table_stride)) return s;
-  if (ctx && (int64_t)B * T == 0) return RIALLM_OK;
-  if (!ctx || !qkv || !pos || !page_table || !inv_freq || !q_out || !k_pages || !v_pages)
-    return rl::refuse(ctx, RIALLM_ERR_INVALID, what, "NULL argument");
-  if (!al16(qkv) || !al16(q_out) || !al16(k_pages) || !al16(v_pages) || !al16(inv_freq))
-    return rl::refuse(ctx, RIALLM_ERR_INVALID, what, "buffers must be 16-byte aligned");
-  return rl::guarded(ctx, [&]() -> int32_t {
-    const Pages pg = make_pages(page_table, table_stride, max_pages, num_pages, nkv, page_size);
-    // Heads per CTA: all of a row's units where they fit, fewer where the
-    // rows alone would leave SMs idle; then as many rows as still fit.
-    const int rows = B * T, heads = nh + 2 * nkv, per_head = d / 16, fit = kAppendThreads * kAppendUnits;
-    int hg = std::min(heads, fit / per_head);
-    const int64_t want = 2ll * ctx->num_sms;
-    if ((int64_t)rows * ((heads + hg - 1) / hg) < want)
-      hg = (int)std::max<int64_t>(std::min(heads, kAppendThreads / per_head / 4), (int64_t)heads * rows / want);
-    hg = std::min(hg, fit / per_head);
-    int per_cta = std::min(kAppendRows, fit / (hg * per_head));
-    per_cta = (int)std::max<int64_t>(1, std::min<int64_t>(per_cta, rows * (int64_t)((heads + hg - 1) / hg) / want));
-    const auto kernel = d == 128 ? rope_paged_append_kernel<128> : rope_paged_append_kernel<64>;
-    return rl::launched(ctx, what,
-                        rl::launch_pdl(kernel, dim3((rows + per_cta - 1) / per_cta, (heads + hg - 1) / hg),
-                                       dim3(kAppendThreads), 0, (cudaStream_t)stream,
-                                       static_cast<const uint16_t*>(qkv), pos, pg, rows, T, nh, per_cta, hg, inv_freq,
-                                       static_cast<uint16_t*>(q_out), static_cast<uint16_t*>(k_pages),
-                                       static_cast<uint16_t*>(v_pages)));
-  });
+int32_t riallm_cuda_rope_paged_append(riallm_ctx* ctx, const riallm_rope_paged_append_args* args, void* stream) {
+  if (!args) return rl::refuse(ctx, RIALLM_ERR_INVALID, "rope_paged_append", "NULL argument");
+  return append(ctx, *args, (cudaStream_t)stream);
 }
 
 uint64_t riallm_cuda_paged_attention_workspace(const riallm_ctx* ctx, int32_t B, int32_t T, int32_t nh, int32_t nkv,
@@ -1517,44 +1554,10 @@ uint64_t riallm_cuda_paged_attention_workspace(const riallm_ctx* ctx, int32_t B,
   return make_plan(ctx->num_sms, B, T, nh, nkv, d, (int64_t)max_pages * page_size).ws_bytes;
 }
 
-int32_t riallm_cuda_paged_attention(riallm_ctx* ctx, const void* q, const void* k_pages, const void* v_pages,
-                                    const int32_t* pos, const int32_t* page_table, int64_t table_stride,
-                                    int32_t max_pages, int32_t B, int32_t T, int32_t nh, int32_t nkv, int32_t d,
-                                    int32_t num_pages, int32_t page_size, int32_t window, int32_t sinks, void* out,
-                                    void* workspace, uint64_t workspace_bytes, void* stream) {
-  const char* what = "paged_attention";
-  if (int s = check_pages(ctx, what, B, T, nh, nkv, d, num_pages, page_size, max_pages, table_stride)) return s;
-  if (window < 0 || sinks < 0)
-    return rl::refuse(ctx, RIALLM_ERR_CONFIG, what, "window and sinks must not be negative");
-  if ((int64_t)B * T * (nh / nkv) > INT32_MAX / 2)
-    return rl::refuse(ctx, RIALLM_ERR_CONFIG, what, "too many rows");
-  if (ctx && (int64_t)B * T == 0) return RIALLM_OK;
-  if (!ctx || !q || !k_pages || !v_pages || !pos || !page_table || !out)
-    return rl::refuse(ctx, RIALLM_ERR_INVALID, what, "NULL argument");
-  if (!al16(q) || !al16(out) || !al16(k_pages) || !al16(v_pages))
-    return rl::refuse(ctx, RIALLM_ERR_INVALID, what, "buffers must be 16-byte aligned");
-  const Plan p = make_plan(ctx->num_sms, B, T, nh, nkv, d, (int64_t)max_pages * page_size);
-  if (p.ws_bytes && (!workspace || workspace_bytes < p.ws_bytes || (reinterpret_cast<uintptr_t>(workspace) & 255)))
-    return rl::refuse(ctx, RIALLM_ERR_MEMORY, what, "workspace missing, too small or not 256-byte aligned");
-  return rl::guarded(ctx, [&]() -> int32_t {
-    AttnArgs a;
-    a.q = static_cast<const uint16_t*>(q);
-    a.k = static_cast<const uint16_t*>(k_pages);
-    a.v = static_cast<const uint16_t*>(v_pages);
-    a.pos = pos;
-    a.pg = make_pages(page_table, table_stride, max_pages, num_pages, nkv, page_size);
-    a.B = B, a.T = T, a.nh = nh, a.rep = nh / nkv;
-    a.rep_inv = (uint32_t)(((1ull << 32) + a.rep - 1) / a.rep);
-    a.window = window, a.sinks = sinks;
-    a.scale_log2 = (float)(1.4426950408889634 / sqrt((double)d));
-    a.out = static_cast<uint16_t*>(out);
-    Space ws{nullptr, nullptr};
-    if (p.join)
-      ws = Space{static_cast<Cut*>(workspace),
-                 reinterpret_cast<float*>(static_cast<char*>(workspace) + cuts_bytes(p.G))};
-    cudaStream_t st = (cudaStream_t)stream;
-    return d == 128 ? launch_attention<128>(ctx, a, p, ws, st) : launch_attention<64>(ctx, a, p, ws, st);
-  });
+int32_t riallm_cuda_paged_attention(riallm_ctx* ctx, const riallm_paged_attention_args* args, void* workspace,
+                                    uint64_t workspace_bytes, void* stream) {
+  if (!args) return rl::refuse(ctx, RIALLM_ERR_INVALID, "paged_attention", "NULL argument");
+  return attend(ctx, *args, workspace, workspace_bytes, (cudaStream_t)stream);
 }
 
 }  // extern "C"

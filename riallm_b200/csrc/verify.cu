@@ -653,29 +653,31 @@ uint64_t riallm_cuda_verify_draft_workspace(const riallm_ctx* ctx, int32_t B, in
   return bytes;
 }
 
-int32_t riallm_cuda_verify_draft(riallm_ctx* ctx, const void* logits, int32_t logits_dtype, const int32_t* draft_tokens,
-                                 const float* draft_probs, const float* temperature, const float* accept_u,
-                                 const float* sample_u, int32_t B, int32_t n, int32_t V, int32_t* tokens,
-                                 int32_t* accepted, void* workspace, uint64_t workspace_bytes, void* stream) {
+int32_t riallm_cuda_verify_draft(riallm_ctx* ctx, const riallm_verify_draft_args* args, void* workspace,
+                                 uint64_t workspace_bytes, void* stream) {
   const char* what = "verify_draft";
+  if (!args) return rl::refuse(ctx, RIALLM_ERR_INVALID, what, "NULL argument");
+  const riallm_verify_draft_args& x = *args;
+  const int32_t B = x.B, n = x.n, V = x.V;
   if (B < 0 || n < 0 || n > 255 || V <= 0 || V > (1 << 30))
     return rl::refuse(ctx, RIALLM_ERR_CONFIG, what, "bad dimensions (at most 255 drafted tokens)");
-  if (logits_dtype != RIALLM_DTYPE_F32 && logits_dtype != RIALLM_DTYPE_BF16)
+  if (x.logits_dtype != RIALLM_DTYPE_F32 && x.logits_dtype != RIALLM_DTYPE_BF16)
     return rl::refuse(ctx, RIALLM_ERR_CONFIG, what, "logits must be float32 or bf16");
   if ((int64_t)B * (n + 1) * ((V + 1023) / 1024) > INT32_MAX)
     return rl::refuse(ctx, RIALLM_ERR_CONFIG, what, "too many logits");
   if (ctx && B == 0) return RIALLM_OK;
-  if (!ctx || !logits || !temperature || !sample_u || !tokens || !accepted || (n > 0 && (!draft_tokens || !accept_u)))
+  if (!ctx || !x.logits || !x.temperature || !x.sample_u || !x.tokens || !x.accepted ||
+      (n > 0 && (!x.draft_tokens || !x.accept_u)))
     return rl::refuse(ctx, RIALLM_ERR_INVALID, what, "NULL argument");
-  if (reinterpret_cast<uintptr_t>(logits) & (logits_dtype == RIALLM_DTYPE_BF16 ? 1 : 3))
+  if (reinterpret_cast<uintptr_t>(x.logits) & (x.logits_dtype == RIALLM_DTYPE_BF16 ? 1 : 3))
     return rl::refuse(ctx, RIALLM_ERR_INVALID, what, "logits must be aligned to their type");
   uint64_t bytes;
   const Space ws = space_of(ctx->num_sms, B, n, V, workspace, &bytes);
   if (!workspace || workspace_bytes < bytes || (reinterpret_cast<uintptr_t>(workspace) & 15))
     return rl::refuse(ctx, RIALLM_ERR_MEMORY, what, "workspace missing, too small or not 16-byte aligned");
   return rl::guarded(ctx, [&]() -> int32_t {
-    const VerifyArgs a{logits, logits_dtype == RIALLM_DTYPE_BF16, draft_tokens, draft_probs, temperature, accept_u,
-                       sample_u, n, V, tokens, accepted};
+    const VerifyArgs a{x.logits,   x.logits_dtype == RIALLM_DTYPE_BF16, x.draft_tokens, x.draft_probs, x.temperature,
+                       x.accept_u, x.sample_u, n, V, x.tokens, x.accepted};
     const cudaStream_t st = (cudaStream_t)stream;
     return a.bf16 ? launch_verify<true>(ctx, what, a, B, ws, st) : launch_verify<false>(ctx, what, a, B, ws, st);
   });

@@ -7,6 +7,7 @@ Layout and meaning of the page table: include/riallm_cuda.h.
 """
 from __future__ import annotations
 
+import struct
 from typing import Dict, List, Optional, Tuple
 
 import torch
@@ -14,6 +15,9 @@ import torch
 from . import ConfigError, Context, MemoryError_, lib
 
 PAGE_SIZES = (16, 32, 64, 128)
+
+# riallm_rope_paged_append_args and riallm_paged_attention_args.
+_APPEND, _ATTEND = struct.Struct("@7Pq8i"), struct.Struct("@6Pq10i")
 
 
 def _need(ok: bool, what: str) -> None:
@@ -86,10 +90,10 @@ def rope_paged_append(qkv: torch.Tensor, pos: torch.Tensor, page_table: torch.Te
         _need(q_out.dtype is torch.bfloat16 and q_out.shape == (rows, nh * d) and q_out.get_device() == dev
               and q_out.is_contiguous(), "rope_paged_append: q_out must be contiguous bf16 [B*T, heads*head_dim]")
     ctx = _context("rope_paged_append", ctx, dev)
-    status = lib().riallm_cuda_rope_paged_append(
-        ctx.ptr, qkv.data_ptr(), pos.data_ptr(), page_table.data_ptr(), _table_stride(page_table),
-        page_table.shape[1], B, T, nh, nkv, d, inv_freq.data_ptr(), q_out.data_ptr(), k_pages.data_ptr(),
-        v_pages.data_ptr(), num_pages, ps, _stream(dev))
+    args = _APPEND.pack(qkv.data_ptr(), pos.data_ptr(), page_table.data_ptr(), inv_freq.data_ptr(), q_out.data_ptr(),
+                        k_pages.data_ptr(), v_pages.data_ptr(), _table_stride(page_table), page_table.shape[1],
+                        num_pages, ps, B, T, nh, nkv, d)
+    status = lib().riallm_cuda_rope_paged_append(ctx.ptr, args, _stream(dev))
     if status:
         ctx.check(status)
     return q_out
@@ -127,10 +131,13 @@ def paged_attention(q: torch.Tensor, pos: torch.Tensor, page_table: torch.Tensor
     # From the caching allocator, in the order of the call's stream: two calls
     # never share one, whatever streams or graphs they are in.
     ws = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
-    status = L.riallm_cuda_paged_attention(
-        ctx.ptr, q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), pos.data_ptr(), page_table.data_ptr(),
-        _table_stride(page_table), max_pages, B, T, nh, nkv, d, num_pages, ps, window, sinks, out.data_ptr(),
-        ws.data_ptr() if size else None, size, _stream(dev))
+    try:
+        args = _ATTEND.pack(q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), pos.data_ptr(),
+                            page_table.data_ptr(), out.data_ptr(), _table_stride(page_table), max_pages, num_pages, ps,
+                            B, T, nh, nkv, d, window, sinks)
+    except struct.error:
+        raise ConfigError("paged_attention: window and sinks must be 32-bit integers") from None
+    status = L.riallm_cuda_paged_attention(ctx.ptr, args, ws.data_ptr() if size else None, size, _stream(dev))
     if status:
         ctx.check(status)
     return out

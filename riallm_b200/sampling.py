@@ -6,6 +6,7 @@ temperature and top_p are accepted and unused).
 """
 from __future__ import annotations
 
+import struct
 from typing import Dict, List, Optional, Sequence, Tuple, Union
 
 import torch
@@ -14,6 +15,7 @@ from . import ConfigError, Context, lib
 from .paged import _context, _stream
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1}
+_VERIFY = struct.Struct("@8P4i")  # riallm_verify_draft_args
 
 # Workspace bytes by call shape.
 _workspace: Dict[Tuple[int, ...], int] = {}
@@ -74,11 +76,11 @@ def verify_draft(logits: torch.Tensor, draft_tokens: Optional[torch.Tensor], acc
             _workspace.clear()
         size = _workspace[key] = L.riallm_cuda_verify_draft_workspace(ctx.ptr, B, n, V)
     ws = torch.empty(size, dtype=torch.uint8, device=device)
-    status = L.riallm_cuda_verify_draft(
-        ctx.ptr, logits.data_ptr(), dtype, draft_tokens.data_ptr() if n else None,
-        draft_probs.data_ptr() if draft_probs is not None and n else None, temperature.data_ptr(),
-        accept_u.data_ptr() if n else None, sample_u.data_ptr(), B, n, V, tokens.data_ptr(), accepted.data_ptr(),
-        ws.data_ptr(), size, _stream(dev))
+    args = _VERIFY.pack(logits.data_ptr(), draft_tokens.data_ptr() if n else 0,
+                        draft_probs.data_ptr() if draft_probs is not None and n else 0, temperature.data_ptr(),
+                        accept_u.data_ptr() if n else 0, sample_u.data_ptr(), tokens.data_ptr(), accepted.data_ptr(),
+                        dtype, B, n, V)
+    status = L.riallm_cuda_verify_draft(ctx.ptr, args, ws.data_ptr(), size, _stream(dev))
     if status:
         ctx.check(status)
     return tokens, accepted

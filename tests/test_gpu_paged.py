@@ -263,6 +263,9 @@ def test_attention_out_and_refusals(rb):
             attend(rb, dict(s, **bad))
     with pytest.raises(rb.ConfigError, match="negative"):
         attend(rb, s, window=-1)
+    for bad in (2**31, 1.5, None):
+        with pytest.raises(rb.ConfigError, match="32-bit"):
+            attend(rb, s, window=bad)
     with pytest.raises(rb.ConfigError, match="out must"):
         attend(rb, s, out=out.float())
     shifted = torch.empty(8 * 128 + 8, dtype=torch.bfloat16, device="cuda")[1:8 * 128 + 1].view(1, -1)

@@ -72,17 +72,36 @@ def test_page_lookup_bounds(rb):
     assert row(0, 0, -1) == -1 and row(0, 0, 2**40) == -1 and row(0, 0, -2**40) == -1
 
 
+def test_argument_structures_match_the_header(rb, tmp_path):
+    """The packed layouts have the C structures' sizes and last offsets."""
+    import subprocess
+    from conftest import ROOT
+    from riallm_b200.paged import _APPEND, _ATTEND
+    from riallm_b200.sampling import _VERIFY
+    src = tmp_path / "s.c"
+    src.write_text('#include "riallm_cuda.h"\n#include <stdio.h>\nint main(void){printf("%zu %zu %zu %zu %zu %zu",'
+                   "sizeof(riallm_rope_paged_append_args),offsetof(riallm_rope_paged_append_args,d),"
+                   "sizeof(riallm_paged_attention_args),offsetof(riallm_paged_attention_args,sinks),"
+                   "sizeof(riallm_verify_draft_args),offsetof(riallm_verify_draft_args,V));return 0;}")
+    subprocess.run(["gcc", "-I", ROOT + "/include", str(src), "-o", str(tmp_path / "s")], check=True)
+    got = list(map(int, subprocess.run([str(tmp_path / "s")], check=True, capture_output=True, text=True).stdout.split()))
+    want = [v for s in (_APPEND, _ATTEND, _VERIFY) for v in (s.size, s.size - 4)]
+    assert got == want
+
+
 CONFIG, INVALID = 3, 7
 
 
 def _append(L, B=1, T=1, nh=8, nkv=2, d=128, num_pages=4, ps=16, max_pages=2, stride=2):
-    return L.riallm_cuda_rope_paged_append(None, None, None, None, stride, max_pages, B, T, nh, nkv, d, None, None,
-                                           None, None, num_pages, ps, None)
+    from riallm_b200.paged import _APPEND
+    args = _APPEND.pack(0, 0, 0, 0, 0, 0, 0, stride, max_pages, num_pages, ps, B, T, nh, nkv, d)
+    return L.riallm_cuda_rope_paged_append(None, args, None)
 
 
 def _attend(L, B=1, T=1, nh=8, nkv=2, d=128, num_pages=4, ps=16, max_pages=2, stride=2, window=0, sinks=0):
-    return L.riallm_cuda_paged_attention(None, None, None, None, None, None, stride, max_pages, B, T, nh, nkv, d,
-                                         num_pages, ps, window, sinks, None, None, 0, None)
+    from riallm_b200.paged import _ATTEND
+    args = _ATTEND.pack(0, 0, 0, 0, 0, 0, stride, max_pages, num_pages, ps, B, T, nh, nkv, d, window, sinks)
+    return L.riallm_cuda_paged_attention(None, args, None, 0, None)
 
 
 @pytest.mark.parametrize("call", [_append, _attend])
@@ -98,12 +117,15 @@ def test_entry_points_refuse_bad_shapes(rb, call, bad):
 def test_entry_points_refuse_null(rb):
     L = rb.lib()
     assert _append(L) == INVALID and _attend(L) == INVALID
+    assert L.riallm_cuda_rope_paged_append(None, None, None) == INVALID
+    assert L.riallm_cuda_paged_attention(None, None, None, 0, None) == INVALID
+    assert L.riallm_cuda_verify_draft(None, None, None, 0, None) == INVALID
     assert _attend(L, window=-1) == CONFIG and _attend(L, sinks=-1) == CONFIG
 
 
 def _verify(L, dtype=0, B=1, n=2, V=10):
-    return L.riallm_cuda_verify_draft(None, None, dtype, None, None, None, None, None, B, n, V, None, None, None, 0,
-                                      None)
+    from riallm_b200.sampling import _VERIFY
+    return L.riallm_cuda_verify_draft(None, _VERIFY.pack(0, 0, 0, 0, 0, 0, 0, 0, dtype, B, n, V), None, 0, None)
 
 
 def test_verify_refusals(rb):
