@@ -230,9 +230,14 @@ __device__ __forceinline__ int64_t head_of(const AttnArgs& a, const Tile& t, int
   return ((int64_t)t.b * a.T + t.tok0 + tok) * a.nh + kh * a.rep + (t.head0 + r - tok * a.rep);
 }
 
+// x / y of numbers that are not negative; 32-bit where both allow it (a
+// 64-bit division is some 300 cycles, and a share begins with several).
+__device__ __forceinline__ int64_t quotient(int64_t x, int64_t y) {
+  return ((x | y) >> 32) == 0 ? (int64_t)((uint32_t)x / (uint32_t)y) : x / y;
+}
 // Share c of G: units [W c / G, W (c+1) / G). The share that unit u is in.
-__device__ __forceinline__ int64_t share_begin(int64_t W, int G, int c) { return W * c / G; }
-__device__ __forceinline__ int share_of(int64_t W, int G, int64_t u) { return (int)(((u + 1) * G - 1) / W); }
+__device__ __forceinline__ int64_t share_begin(int64_t W, int G, int c) { return quotient(W * c, G); }
+__device__ __forceinline__ int share_of(int64_t W, int G, int64_t u) { return (int)quotient((u + 1) * G - 1, W); }
 
 // Finds the tile that the first unit of share c (of the call's G shares, fewer
 // where there are fewer units) lies in: every thread of a block of N threads sums the
@@ -303,7 +308,7 @@ struct Cursor {
     x = at.x;
     t = tile_of<Sh>(a, tiles, x);
     const int size = t.bl.n + Sh::kCost;
-    kh = (int)((at.u - at.start) / size);
+    kh = (int)quotient(at.u - at.start, size);
     at0 = at.start + (int64_t)kh * size + Sh::kCost;
     i = (int)max((int64_t)0, at.u - at0);
     end = share_begin(at.W, at.G, c + 1);
@@ -701,8 +706,8 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
 // not see whole. Keys and values share a ring of kStages blocks in smem.
 constexpr int kManyThreads = 12 * 32;
 // Registers: the launch's 168 a thread, of which the third warpgroup (loads,
-// products) keeps 56 and the weights' two take 224 (2 * 224 + 56 = 3 * 168).
-constexpr int kWeightRegs = 224, kOtherRegs = 56;
+// products) keeps 72 and the weights' two take 216 (2 * 216 + 72 = 3 * 168).
+constexpr int kWeightRegs = 216, kOtherRegs = 72;
 constexpr int kMaxStages = 8;
 template <bool kTwoTiles>
 using Many = Shape<kTwoTiles ? 256 : 128, 128, 4>;
@@ -771,6 +776,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
   __shared__ uint32_t gone[8];    // block n % 8: its pages that are not held, or that nobody sees
   __shared__ int poison[16];      // segment n % 16: a value that some rows must not meet is not finite
   __shared__ float ml[2][128];    // slot 1's maxima and sums, !kTwoTiles
+  __shared__ Segments<Sh> at_seg[8];  // of each weights' warp: its registers are for weights
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   uint8_t* qs = smem;                          // 2 tiles
   uint8_t* ring = smem + 2 * kTileBytes<D>;
@@ -1014,8 +1020,15 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kWeightRegs));
-    Segments<Sh> sg;
-    if (at.u < at.W && sg.init(a, tiles, at, blockIdx.x)) {
+    Segments<Sh>& sg = at_seg[warp];
+    int work = 0;
+    if (lane == 0) {
+      Segments<Sh> first;
+      work = at.u < at.W && first.init(a, tiles, at, blockIdx.x);
+      sg = first;
+    }
+    work = __shfl_sync(0xffffffffu, work, 0);
+    if (work) {
       // ---------------------------------------------- weights
       const int slot = warp >> 2, wr = warp & 3;
       const uint32_t lane_off = (uint32_t)(wr * 32) << 16;
@@ -1053,7 +1066,8 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         const int whole_lo = w1 < w0 ? 0 : a.span(t.p0 + token_of(a, t, w1)).lo;
         float m = -INFINITY, l = 0.f;  // maximum (of scaled scores) that the weights are relative to, and their sum
         int done = 0;                  // blocks of this segment
-        for (int i = sg.i0 + (kTwoTiles ? 0 : slot); i < sg.i1; i += kTwoTiles ? 1 : 2) {
+        const int i0 = sg.i0, i1 = sg.i1;
+        for (int i = i0 + (kTwoTiles ? 0 : slot); i < i1; i += kTwoTiles ? 1 : 2) {
           const int j0 = t.bl.index(i) * 128;
           go = warp_wait(&bars.s_full[slot], sc & 1, abort, status);
           if (!go) break;
@@ -1063,7 +1077,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
           for (int y = 0; y < 4; ++y) rl::tmem_ld_32x32b_x32(ts + y * 32, x[y]);
           rl::tmem_wait_ld();
           // Pages that are not held are loaded as zeros; their scores go too.
-          const uint32_t bad = *(volatile uint32_t*)&gone[(n0 + i - sg.i0) & 7];
+          const uint32_t bad = *(volatile uint32_t*)&gone[(n0 + i - i0) & 7];
           if (bad || j0 + 127 > whole_hi || (j0 < whole_lo && j0 + 127 >= a.sinks)) {
 #pragma unroll
             for (int y = 0; y < 4; ++y) {
@@ -1258,7 +1272,14 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         rl::tc_fence_before();  // the next group's first product overwrites O
         n0 += nb;
         ++seg;
-      } while (sg.next(a, tiles));
+        __syncwarp();
+        if (lane == 0) {
+          Segments<Sh> after = sg;
+          work = after.next(a, tiles);
+          sg = after;
+        }
+        work = __shfl_sync(0xffffffffu, work, 0);
+      } while (work);
     }
   }
   rl::tc_fence_before();
