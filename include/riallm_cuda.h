@@ -435,7 +435,9 @@ int32_t riallm_cuda_linear_bf16(riallm_ctx* ctx, const void* x, const void* w, v
  * page that the sequence does not hold: its positions are neither written
  * nor read. One page may stand in several sequences' tables (a shared
  * prefix) as long as no call appends to it. page_size is 16, 32, 64 or 128;
- * d is 64 or 128; nh / nkv at most 128. No riallm counterpart: its KVCACHE
+ * d is 64 or 128; nh / nkv at most 128; a pool has at most 2^31 - 1 rows
+ * (num_pages * nkv * page_size), a sequence at most 2^31 - 257 positions
+ * (max_pages * page_size). No riallm counterpart: its KVCACHE
  * (src/model.rs:15-38) is one contiguous tensor per layer. These functions
  * leave the calling thread's current device as it was. */
 

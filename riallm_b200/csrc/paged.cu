@@ -240,9 +240,9 @@ __device__ __forceinline__ int64_t share_begin(int64_t W, int G, int c) { return
 __device__ __forceinline__ int share_of(int64_t W, int G, int64_t u) { return (int)quotient((u + 1) * G - 1, W); }
 
 // Finds the tile that the first unit of share c (of the call's G shares, fewer
-// where there are fewer units) lies in: every thread of a block of N threads sums the
-// units of its slab of tiles, and the thread whose slab holds the unit walks
-// it.
+// where there are fewer units) lies in: every thread of a block of N threads
+// sums the units of its slab of tiles, and the thread whose slab holds the
+// unit walks it.
 struct UnitAt {
   int64_t W;      // all units of the call
   int G;          // shares, none of them empty
@@ -1476,8 +1476,9 @@ int check_pages(riallm_ctx* ctx, const char* what, const Args& x) {
   if (page_size != 16 && page_size != 32 && page_size != 64 && page_size != 128)
     return bad("page_size must be 16, 32, 64 or 128");
   if (x.num_pages <= 0 || x.max_pages <= 0 || x.table_stride < x.max_pages) return bad("bad page table");
-  if ((int64_t)x.num_pages * nkv * page_size > INT32_MAX || (int64_t)x.max_pages * page_size > INT32_MAX)
-    return bad("more than 2^31 - 1 cache rows");
+  // The kernels count positions in 32 bits, to the end of the last position's block and a page past it.
+  if ((int64_t)x.num_pages * nkv * page_size > INT32_MAX || (int64_t)x.max_pages * page_size > INT32_MAX - 256)
+    return bad("more than 2^31 - 257 positions, or 2^31 - 1 cache rows");
   if ((int64_t)B * T > INT32_MAX / 4 || (int64_t)nh + 2 * nkv > 65535) return bad("too many rows or heads");
   return RIALLM_OK;
 }

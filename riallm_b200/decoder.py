@@ -311,7 +311,8 @@ class Decoder:
 
     def _forward(self, ids: torch.Tensor, experts_used: list = None, all_logits: bool = False) -> torch.Tensor:
         """ids [B, T] on the device -> last-position logits [B, V] float32
-        (with all_logits every position's, [B, T, V]). Appends T positions to every sequence (pos += T on the device).
+        (with all_logits every position's, [B, T, V]). Appends T positions to
+        every sequence (pos += T on the device).
         With experts_used (a list), the number of distinct experts each
         layer's MoE block routes to is appended to it (an extra router pass;
         eager use only)."""

@@ -114,6 +114,16 @@ def test_entry_points_refuse_bad_shapes(rb, call, bad):
     assert call(rb.lib(), **bad) == CONFIG
 
 
+@pytest.mark.parametrize("call", [_append, _attend])
+def test_positions_end_a_block_below_32_bits(rb, call):
+    """The last position's block of 128 keys, and the page after it, are
+    counted in int32; 2^31 - 257 positions leave room for both."""
+    for ps in (16, 128):
+        most = (2**31 - 257) // ps
+        assert call(rb.lib(), ps=ps, max_pages=most, stride=most) == INVALID  # past the checks of sizes: NULL
+        assert call(rb.lib(), ps=ps, max_pages=most + 1, stride=most + 1) == CONFIG
+
+
 def test_entry_points_refuse_null(rb):
     L = rb.lib()
     assert _append(L) == INVALID and _attend(L) == INVALID
