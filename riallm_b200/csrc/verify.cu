@@ -38,6 +38,8 @@ namespace {
 
 constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kBatch = 8;  // loads of an array that a thread has in flight
+constexpr int kStep = 4;   // tokens of a thread where the last part is searched
+constexpr int kChunk = kThreads * kStep * kWarps;  // largest chunk: its parts are searched in one go
 constexpr int kTable = 256;
 static_assert(kTable == kThreads, "a thread fills an entry");
 
@@ -137,6 +139,12 @@ struct Part {
   }
 };
 
+// 2^(i / 256) for the table of Exp64: the upper word is i << 12 below.
+__device__ __forceinline__ double table_entry(int i) {
+  const double p = exp2((double)i / kTable);
+  return __hiloint2double(__double2hiint(p) - (i << 12), __double2loint(p));
+}
+
 // A CTA per slice of a row, row by row. 16 bytes a load where the row's place
 // allows, four loads of a thread in flight and four at work.
 template <bool kBf16>
@@ -152,7 +160,7 @@ __global__ void __launch_bounds__(kThreads)
   const int begin = min(a.V, (int)(blockIdx.x - row * ws.slices) * slice), end = min(a.V, begin + slice);
   const float temp = a.temperature[row / (a.n + 1)], c = scale_of(temp);
   const bool greedy = !(temp > 0.f);
-  if (blockIdx.x == 0) ws.table[tid] = exp2((double)tid / kTable);
+  if (blockIdx.x == 0) ws.table[tid] = table_entry(tid);
   const int64_t base = (int64_t)row * a.V;
   // Whole vectors of the slice: [v0, v1) as row indices, the rest one by one.
   const int skew = (int)((reinterpret_cast<uintptr_t>(a.logits) / (kBf16 ? 2 : 4) + base + begin) & (N - 1));
@@ -235,26 +243,33 @@ __global__ void __launch_bounds__(kThreads)
 
 // ------------------------------------------------------------ 64 bits
 //
-// e^((l - m) / t): 2^(k / 256) from a table and the rest, at most 1 / 512
-// octave, by the Taylor series to the 3rd power (error 1.4e-13).
+// e^((l - m) / t): 2^(i / 256) from a table and the rest, at most 1 / 512
+// octave, by the Taylor series to the 3rd power (error 1.4e-13). The table's
+// powers lie in their upper words below their exponents by i << 12, so that
+// adding i << 12 gives 2^(i / 256) for every i.
 struct Exp64 {
-  const double* table;  // 2^(i / 256), in shared memory
+  const double* table;  // in shared memory
   double k, m;          // 256 log2(e) / t
-  __device__ __forceinline__ Exp64(const double* table_, float m_, double k_) : table(table_), k(k_), m((double)m_) {}
-  // The value, where `some`; it is 0 otherwise (below 2^-1000, and at -inf).
+  float least;          // logits below it count as 0: 1000 octaves and more down
+  __device__ __forceinline__ Exp64(const double* table_, float m_, double k_, float t)
+      : table(table_), k(k_), m((double)m_) {
+    const double x = m - 693.0 * (double)t;
+    least = fmaxf((float)x, -3.402823466e38f);
+    if ((double)least < x) least = nextafterf(least, m_);
+  }
+  // The value, where `some`; it is 0 otherwise.
   __device__ __forceinline__ double operator()(float l, bool& some) const {
-    constexpr double kMagic = 6755399441055744.0;            // 1.5 * 2^52
+    constexpr double kMagic = 6755399441055744.0;  // 1.5 * 2^52
     constexpr double a = 0.6931471805599453 / kTable;
-    const double x = ((double)l - m) * k;  // in this order: 0 at the maximum, whatever the temperature
-    const double xf = x + kMagic;
+    const double d = (double)l - m;  // 0 at the maximum, whatever the temperature
+    const double xf = fma(d, k, kMagic);
     const int i = __double2loint(xf);
-    const double r = x - (xf - kMagic);
+    const double r = fma(d, k, -(xf - kMagic));
     double p = fma(r, a * a * a / 6.0, a * a / 2.0);
-    p = fma(r, p, a);
-    p = fma(r, p, 1.0);
-    p *= table[i & (kTable - 1)];
-    some = x > -1000.0 * kTable;
-    return __hiloint2double(__double2hiint(p) + ((i & -kTable) << 12), __double2loint(p));
+    p = fma(r, p, a) * r;
+    const double e = table[i & (kTable - 1)], power = __hiloint2double(__double2hiint(e) + (i << 12), __double2loint(e));
+    some = l >= least;
+    return fma(power, p, power);
   }
   __device__ __forceinline__ double operator()(float l) const {
     bool some;
@@ -292,6 +307,7 @@ __device__ __forceinline__ Row row_of(const Stat* s, int slices, float t) {
   const float c = scale_of(t);
   Stat st{-INFINITY, 0.f, 0x7fffffff, 0};
   double z = 0.0;
+#pragma unroll 4
   for (int i = lane; i < slices; i += 32) {
     const uint4 u = __ldcg(reinterpret_cast<const uint4*>(s + i));
     const float m = __uint_as_float(u.x), mn = fmaxf(st.m, m), base = mn == -INFINITY ? 0.f : mn;
@@ -321,11 +337,11 @@ __device__ __forceinline__ double block_sum(double v, double* part) {  // of all
   for (int w = 0; w < kWarps; ++w) v += part[w];
   return v;
 }
-// Sum of v[0 .. n), the same in every warp.
-__device__ __forceinline__ double sum_of(const double* v, int n) {
+// Sum of v[0 .. n), the same in every thread and every CTA.
+__device__ __forceinline__ double sum_of(const double* v, int n, double* part) {
   double s = 0.0;
-  for (int i = threadIdx.x & 31; i < n; i += 32) s += __ldcg(v + i);
-  return warp_sum(s);
+  for (int i = threadIdx.x; i < n; i += kThreads) s += __ldcg(v + i);
+  return block_sum(s, part);
 }
 // One row of logits.
 template <bool kBf16>
@@ -336,35 +352,37 @@ struct Logits {
   __device__ __forceinline__ float operator()(int j) const { return load_logit(p, kBf16, j); }
 };
 // Calls use(j, logit j, draft probability j) for j = j0, j0 + step, ... below
-// j1, kBatch loads of each array at a time.
-template <bool kQ, typename L, typename F>
-__device__ __forceinline__ void over(const L& logit, const float* q, int j0, int j1, int step, F&& use) {
-  int j = j0;
-  for (; j + (kBatch - 1) * step < j1; j += kBatch * step) {
-    float l[kBatch], x[kBatch];
+// j1, kBatch loads of each array at a time (what is past j1: -inf and 0);
+// ready() once, when the first of them are on their way.
+template <bool kQ, typename L, typename R, typename F>
+__device__ __forceinline__ void over(const L& logit, const float* q, int j0, int j1, int step, R&& ready, F&& use) {
+  float l[kBatch], x[kBatch];
+  auto fetch = [&](int j) {
 #pragma unroll
     for (int e = 0; e < kBatch; ++e) {
-      l[e] = logit(j + e * step);
-      x[e] = kQ ? __ldg(q + j + e * step) : 0.f;
+      const bool in = e * step < j1 - j;
+      l[e] = in ? logit(j + e * step) : -INFINITY;
+      x[e] = kQ && in ? __ldg(q + j + e * step) : 0.f;
     }
+  };
+  fetch(j0);
+  ready();
+  for (int j = j0; j < j1; j += kBatch * step) {
+    if (j > j0) fetch(j);
 #pragma unroll
-    for (int e = 0; e < kBatch; ++e) use(j + e * step, l[e], x[e]);
+    for (int e = 0; e < kBatch; ++e) use(l[e], x[e]);
   }
-  for (; j < j1; j += step) use(j, logit(j), kQ ? __ldg(q + j) : 0.f);
 }
 
-// CTA (sequence, chunk). Every CTA of a sequence finds the verdict; the first
-// writes it, and what is known of the result.
+// What the CTA of sequence b finds, from the slices' statistics: how many of
+// its drafts hold, and where its next token comes from. `writes`: this CTA is
+// to write what is known of the result.
 template <bool kBf16>
-__global__ void __launch_bounds__(kThreads) weigh_kernel(const VerifyArgs a, const Space ws) {
-  __shared__ double table[kTable], part[kWarps];
+__device__ __forceinline__ Verdict judge(const VerifyArgs& a, const Space& ws, const double* table, int b, bool writes) {
+  __shared__ double part[kWarps];
   __shared__ unsigned verdict[kWarps], close[kWarps];  // bits: rejected; too close to say
   __shared__ Row rows[256];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int b = blockIdx.x / ws.chunks, chunk = blockIdx.x - b * ws.chunks, V = a.V, n = a.n;
-  rl::pdl_wait();
-  rl::pdl_launch_dependents();
-  table[tid] = ws.table[tid];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, V = a.V, n = a.n;
   const float t = a.temperature[b];
   const double scale = ws.scale[b];
   const int64_t row0 = (int64_t)b * (n + 1);
@@ -406,7 +424,7 @@ __global__ void __launch_bounds__(kThreads) weigh_kernel(const VerifyArgs a, con
       if (r.top >= 0) {
         no = !(lhs < (x == r.top ? 1.0 : 0.0));
       } else {
-        const double p = Exp64(table, r.m, scale)(Logits<kBf16>(a, row0 + tid)(x));
+        const double p = Exp64(table, r.m, scale, t)(Logits<kBf16>(a, row0 + tid)(x));
         near = p > 0.0 && fabs(lhs * r.z - p) <= 1e-4 * p;
         no = !(lhs * r.z < p);
       }
@@ -425,10 +443,10 @@ __global__ void __launch_bounds__(kThreads) weigh_kernel(const VerifyArgs a, con
     if (close[acc >> 5] & bit) {
       // The whole CTA sums this row in 64 bits.
       const int x = draft(acc);
-      const Exp64 ex(table, rows[acc].m, scale);
+      const Exp64 ex(table, rows[acc].m, scale, t);
       const Logits<kBf16> logit(a, row0 + acc);
       double z = 0.0;
-      over<false>(logit, nullptr, tid, V, kThreads, [&](int, float l, float) { z += ex(l); });
+      over<false>(logit, nullptr, tid, V, kThreads, [] {}, [&](float l, float) { z += ex(l); });
       z = block_sum(z, part);
       const double q = a.probs ? (double)a.probs[((int64_t)b * n + acc) * V + x] : 1.0;
       rejected = !((double)a.accept_u[(int64_t)b * n + acc] * q * z < ex(logit(x)));
@@ -436,32 +454,64 @@ __global__ void __launch_bounds__(kThreads) weigh_kernel(const VerifyArgs a, con
     if (rejected) break;
   }
   const int top = rows[acc].top, x = draft(acc);
-  if (chunk == 0) {
+  // All of p on one token: so is what a rejected draft leaves of it.
+  const Verdict v{acc, x, rows[acc].m, top >= 0};
+  if (writes) {
     for (int i = tid; i <= n; i += kThreads)
       if (i != acc || top >= 0)
         a.tokens[row0 + i] = i < acc ? a.drafts[(int64_t)b * n + i] : i == acc ? top : -1;
     if (tid == 0) {
       a.accepted[b] = acc;
-      // All of p on one token: so is what a rejected draft leaves of it.
-      ws.verdict[b] = Verdict{acc, x, rows[acc].m, top >= 0};
+      ws.verdict[b] = v;
     }
   }
-  if (top >= 0) return;
+  return v;
+}
 
-  // The parts' sums of exponentials, of which a draft that was chosen outright
-  // (q = 1 there) leaves all but its own.
-  const Exp64 ex(table, rows[acc].m, scale);
-  const int drop = a.probs ? -1 : x, p = chunk * kWarps + warp, j0 = min(V, p * ws.part), j1 = min(V, j0 + ws.part);
+// A CTA per sequence.
+template <bool kBf16>
+__global__ void __launch_bounds__(kThreads) judge_kernel(const VerifyArgs a, const Space ws) {
+  __shared__ double table[kTable];
+  rl::pdl_wait();
+  rl::pdl_launch_dependents();
+  table[threadIdx.x] = ws.table[threadIdx.x];
+  judge<kBf16>(a, ws, table, blockIdx.x, true);
+}
+
+// CTA (sequence, chunk): the sums of exponentials of the chunk's parts in the
+// row that the token comes from. kJudge: every CTA of a sequence finds that
+// row itself, and the first writes it down; otherwise it is known.
+template <bool kBf16, bool kJudge>
+__global__ void __launch_bounds__(kThreads) weigh_kernel(const VerifyArgs a, const Space ws) {
+  __shared__ double table[kTable];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int b = blockIdx.x / ws.chunks, chunk = blockIdx.x - b * ws.chunks, V = a.V, n = a.n;
+  rl::pdl_wait();
+  rl::pdl_launch_dependents();
+  const double entry = ws.table[tid];
+  if (kJudge) table[tid] = entry;
+  const Verdict v = kJudge ? judge<kBf16>(a, ws, table, b, chunk == 0) : ws.verdict[b];
+  if (v.done) return;
+
+  // A draft that was chosen outright (q = 1 there) leaves all but its own
+  // token.
+  const int drop = a.probs ? -1 : v.draft, p = chunk * kWarps + warp, j0 = min(V, p * ws.part), j1 = min(V, j0 + ws.part);
+  const Exp64 ex(table, v.m, ws.scale[b], a.temperature[b]);
   double sum = 0.0;
-  const Logits<kBf16> logit(a, row0 + acc);
-  auto add = [&](int, float l, float) {
+  const Logits<kBf16> logit(a, (int64_t)b * (n + 1) + v.acc);
+  auto add = [&](float l, float) {
     bool some;
     const double w = ex(l, some);
     if (some) sum += w;
   };
   const int cut = min(max(drop, j0), j1);  // around the dropped token, if it is here
-  over<false>(logit, nullptr, j0 + lane, cut, 32, add);
-  over<false>(logit, nullptr, (cut == drop ? cut + 1 : cut) + lane, j1, 32, add);
+  auto ready = [&] {
+    if (kJudge) return;
+    table[tid] = entry;
+    __syncthreads();
+  };
+  over<false>(logit, nullptr, (cut == drop ? cut + 1 : cut) + lane, j1, 32, ready, add);
+  over<false>(logit, nullptr, j0 + lane, cut, 32, [] {}, add);
   sum = warp_sum(sum);
   if (lane == 0) ws.z[(int64_t)b * ws.chunks * kWarps + p] = sum;
 }
@@ -471,36 +521,38 @@ __global__ void __launch_bounds__(kThreads) weigh_kernel(const VerifyArgs a, con
 // done (its only one otherwise) takes the token.
 template <bool kBf16>
 __global__ void __launch_bounds__(kThreads) pick_kernel(const VerifyArgs a, const Space ws) {
-  __shared__ double table[kTable];
+  __shared__ double table[kTable], part[kWarps];
   __shared__ bool is_last;
-  __shared__ int found;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int b = blockIdx.x / ws.chunks, chunk = blockIdx.x - b * ws.chunks, V = a.V, n = a.n;
   rl::pdl_wait();
   rl::pdl_launch_dependents();
   const Verdict v = ws.verdict[b];
-  const double scale = ws.scale[b];
-  table[tid] = ws.table[tid];
-  __syncthreads();
+  const double entry = ws.table[tid];
   if (v.done) return;
   const bool residual = v.draft >= 0 && a.probs;
+  if (!residual && chunk != 0) return;
   const int parts = ws.chunks * kWarps;
   const int64_t row = (int64_t)b * (n + 1) + v.acc, first = (int64_t)b * parts;
   const float* q = residual ? a.probs + ((int64_t)b * n + v.acc) * V : nullptr;
   const Logits<kBf16> logit(a, row);
-  const Exp64 ex(table, v.m, scale);
-  double total = sum_of(ws.z + first, parts);
-  const double z = total;
+  const Exp64 ex(table, v.m, ws.scale[b], a.temperature[b]);
+  double z;
+  auto ready = [&] {
+    table[tid] = entry;
+    z = sum_of(ws.z + first, parts, part);  // waits for the table, too
+  };
   const double* w = ws.z + first;
   bool taken_off = residual;  // weights are max(0, e - q z), or e
   auto weight = [&](float l, float x) {
     const double e = ex(l);
     return taken_off ? fma(-(double)x, z, e) : e;
   };
+  double total;
   if (residual) {
     const int p = chunk * kWarps + warp, j0 = min(V, p * ws.part), j1 = min(V, j0 + ws.part);
     double sum = 0.0;
-    over<true>(logit, q, j0 + lane, j1, 32, [&](int, float l, float x) {
+    over<true>(logit, q, j0 + lane, j1, 32, ready, [&](float l, float x) {
       const double y = weight(l, x);
       if (y > 0.0) sum += y;
     });
@@ -512,15 +564,17 @@ __global__ void __launch_bounds__(kThreads) pick_kernel(const VerifyArgs a, cons
     __syncthreads();
     if (!is_last) return;
     __threadfence();
-    const double left = sum_of(ws.w + first, parts);
+    const double left = sum_of(ws.w + first, parts, part);
     if (left > 0.0) {
       w = ws.w + first;
       total = left;
     } else {
+      total = z;
       taken_off = false;  // p == q: nothing is left over; p itself
     }
-  } else if (chunk != 0) {
-    return;
+  } else {
+    ready();
+    total = z;
   }
 
   const int drop = a.probs ? -1 : v.draft;
@@ -531,73 +585,67 @@ __global__ void __launch_bounds__(kThreads) pick_kernel(const VerifyArgs a, cons
   // The first token whose cumulative weight exceeds the target lies in the
   // first part whose end does.
   const double target = (double)a.sample_u[b] * total;
-  int at = -1, some = -1;
+  // Of a range of parts a lane takes a 32nd; the range becomes that lane's.
+  int at = 0, count = parts;
+  bool beyond = true;  // (false: no part's end does; it becomes the last with weight)
   double start = 0.0;
-  for (int c = 0; c < parts && at < 0; c += 32) {
-    const double y = c + lane < parts ? __ldcg(w + c + lane) : 0.0;
+  do {
+    const int each = (count + 31) / 32, i0 = lane * each, i1 = min(count, i0 + each);
+    double y = 0.0;
+#pragma unroll 4
+    for (int i = i0; i < i1; ++i) y += __ldcg(w + at + i);
     const double upto = warp_scan(y);
     const unsigned with = __ballot_sync(0xffffffffu, y > 0.0);
-    const unsigned beyond = __ballot_sync(0xffffffffu, start + upto > target) & with;
-    if (with) some = c + 31 - __clz(with);
-    if (beyond) {
-      const int i = __ffs(beyond) - 1;
-      at = c + i;
-      const double before = __shfl_sync(0xffffffffu, upto, max(i - 1, 0));
-      if (i > 0) start += before;
-    } else {
-      start += __shfl_sync(0xffffffffu, upto, 31);
-    }
-  }
-  if (at < 0) {
-    // A number of 1 or more, or none (NaN), or one that rounds up to the
-    // total: the last token with weight, which part `some` holds.
-    if (tid == 0) found = 0;
-    __syncthreads();
-    const int j0 = min(V, some * ws.part), j1 = min(V, j0 + ws.part);
-    int last = 0;
-    for (int j = j0 + tid; j < j1; j += kThreads)
-      if (j != drop && weight(logit(j), taken_off ? q[j] : 0.f) > 0.0) last = j;
-    atomicMax(&found, last);
-    __syncthreads();
-    if (tid == 0) a.tokens[row] = found;
-    return;
-  }
-  if (warp != 0) return;
-  // Within the part 256 tokens at a time, then 32 of those.
-  constexpr int kStep = 8;
-  const int j0 = at * ws.part, j1 = min(V, j0 + ws.part);
-  int hit = -1, last = 0;
-  for (int j = j0; j < j1 && hit < 0; j += 32 * kStep) {
+    const unsigned past = __ballot_sync(0xffffffffu, beyond && start + upto > target) & with;
+    beyond = past != 0;
+    const int i = beyond ? __ffs(past) - 1 : max(0, 31 - __clz(with));
+    const double before = __shfl_sync(0xffffffffu, upto, max(i - 1, 0));
+    if (i > 0) start += before;
+    at += i * each;
+    count = min(each, count - i * each);
+  } while (count > 1);
+  // Within the part, of at most 1024 tokens, 128 a warp. No token is beyond
+  // the target where the number is 1 or more, or none (NaN), or rounds up to
+  // the total: then the last with weight.
+  __shared__ double sums[kWarps];
+  const int j0 = at * ws.part + warp * kStep * 32 + lane, j1 = min(V, (at + 1) * ws.part);
+  double y[kStep], sum = 0.0;
+  {
     float l[kStep], x[kStep];
 #pragma unroll
     for (int e = 0; e < kStep; ++e) {
-      const int i = j + e * 32 + lane;
+      const int i = j0 + e * 32;
       l[e] = i < j1 && i != drop ? logit(i) : -INFINITY;
       x[e] = i < j1 && taken_off ? q[i] : 0.f;
     }
-    double y[kStep], sum = 0.0;
 #pragma unroll
     for (int e = 0; e < kStep; ++e) {
       y[e] = fmax(0.0, weight(l[e], x[e]));
       sum += y[e];
     }
-    sum = warp_sum(sum);
-    if (start + sum > target || j + 32 * kStep >= j1) {
-#pragma unroll
-      for (int e = 0; e < kStep; ++e) {
-        const double upto = warp_scan(y[e]);
-        const unsigned with = __ballot_sync(0xffffffffu, y[e] > 0.0);
-        const unsigned beyond = __ballot_sync(0xffffffffu, start + upto > target) & with;
-        if (hit < 0 && beyond) hit = j + e * 32 + __ffs(beyond) - 1;
-        if (with) last = j + e * 32 + 31 - __clz(with);
-        start += __shfl_sync(0xffffffffu, upto, 31);
-      }
-    } else {
-      if (sum > 0.0) last = j;  // replaced by a later one, or the sums differ in their last bits
-      start += sum;
-    }
   }
-  if (lane == 0) a.tokens[row] = hit >= 0 ? hit : last;
+  sum = warp_sum(sum);
+  if (lane == 0) sums[warp] = sum;
+  __syncthreads();
+  int in = -1, last = 0;  // the warp whose tokens reach the target, else the last with weight
+  for (int i = 0; i < kWarps && in < 0; ++i) {
+    if (sums[i] > 0.0) last = i;
+    if (beyond && sums[i] > 0.0 && start + sums[i] > target) in = i;
+    else start += sums[i];
+  }
+  if (warp != (in < 0 ? last : in)) return;
+  int hit = -1;
+  last = 0;
+#pragma unroll
+  for (int e = 0; e < kStep; ++e) {
+    const double upto = warp_scan(y[e]);
+    const unsigned with = __ballot_sync(0xffffffffu, y[e] > 0.0);
+    const unsigned beyond = __ballot_sync(0xffffffffu, start + upto > target) & with;
+    if (hit < 0 && in >= 0 && beyond) hit = e * 32 + __ffs(beyond) - 1;
+    if (with) last = e * 32 + 31 - __clz(with);
+    start += __shfl_sync(0xffffffffu, upto, 31);
+  }
+  if (lane == 0) a.tokens[row] = j0 + (hit >= 0 ? hit : last);
 }
 
 // Slices of a row (1024 to 65536 tokens) and chunks of the row that a token
@@ -612,7 +660,7 @@ Space space_of(int num_sms, int B, int n, int V, void* base, uint64_t* bytes) {
   };
   s.slices = pick(8ll * num_sms, rows, 65536);
   s.slice = (V + s.slices - 1) / s.slices;
-  s.chunks = pick(4ll * num_sms, B, 8192);
+  s.chunks = pick(4ll * num_sms, B, kChunk);
   s.part = (V + s.chunks * kWarps - 1) / (s.chunks * kWarps);
   uint64_t at = 0;
   auto take = [&](uint64_t size) {
@@ -637,7 +685,13 @@ int32_t launch_verify(riallm_ctx* ctx, const char* what, const VerifyArgs& a, in
   const unsigned rows = (unsigned)B * (a.n + 1);
   if (int r = rl::launched(ctx, what, rl::launch_pdl(stats_kernel<kBf16>, dim3(rows * ws.slices), dim3(kThreads), 0, st, a, ws)))
     return r;
-  if (int r = rl::launched(ctx, what, rl::launch_pdl(weigh_kernel<kBf16>, dim3(B * ws.chunks), dim3(kThreads), 0, st, a, ws)))
+  // A launch costs 2 us; every CTA's own verdict a third of a chunk's time.
+  const bool apart = B * ws.chunks > 5 * ctx->num_sms;
+  if (apart)
+    if (int r = rl::launched(ctx, what, rl::launch_pdl(judge_kernel<kBf16>, dim3(B), dim3(kThreads), 0, st, a, ws)))
+      return r;
+  const auto weigh = apart ? weigh_kernel<kBf16, false> : weigh_kernel<kBf16, true>;
+  if (int r = rl::launched(ctx, what, rl::launch_pdl(weigh, dim3(B * ws.chunks), dim3(kThreads), 0, st, a, ws)))
     return r;
   return rl::launched(ctx, what, rl::launch_pdl(pick_kernel<kBf16>, dim3(B * ws.chunks), dim3(kThreads), 0, st, a, ws));
 }

@@ -240,6 +240,55 @@ def test_streams_and_graph(rb):
     assert torch.equal(out[0].cpu(), reference(*a)[0])
 
 
+@pytest.mark.parametrize("B,V", [(1, 200003), (1, 70000), (2, 1023), (7, 128001), (64, 32768), (70, 128001)])
+def test_every_border_is_found(rb, B, V):
+    """Uniform logits: every weight is exactly 1, so that sample_u = (k + 1/2)
+    / V takes token k; its rounding moves the target by at most V * 2^-25 <
+    0.01. Numbers of 1 and more, or none, take the last token. The same for
+    what a rejected draft leaves: the second half of the vocabulary."""
+    g = torch.Generator().manual_seed(V)
+    k = torch.randint(0, V, (B,), generator=g)
+    k[0] = V - 1
+    u = ((k.double() + 0.5) / V).float()
+    if B > 4:
+        u[1], u[2], u[3], k[1:4] = 1.0, NAN, INF, V - 1
+    logits = torch.zeros(B, 1, V, device="cuda", dtype=torch.bfloat16)
+    t, _ = rb.verify_draft(logits, None, None, u.cuda(), 0.9)
+    assert t[:, 0].tolist() == k.tolist()
+
+    h = V // 2
+    q = torch.zeros(B, 1, V, device="cuda")
+    q[:, :, :h] = 1.0 / h  # above 1 / V: rejected with accept_u of 0.9, and nothing of it is left
+    k = h + torch.randint(0, V - h, (B,), generator=g)
+    k[0] = h
+    u = ((k.double() - h + 0.5) / (V - h)).float()
+    d = torch.randint(0, h, (B, 1), generator=g, dtype=torch.int32)
+    t, c = rb.verify_draft(torch.zeros(B, 2, V, device="cuda"), d.cuda(), torch.full((B, 1), 0.9, device="cuda"), u.cuda(),
+                           0.9, draft_probs=q)
+    assert t[:, 0].tolist() == k.tolist() and c.tolist() == [0] * B and t[:, 1].tolist() == [-1] * B
+
+
+def test_batch_as_its_sequences(rb):
+    """A batch whose verdicts are found in a launch of their own gives what
+    each sequence gives alone."""
+    B, n, V = 60, 2, 128001
+    g = torch.Generator(device="cuda").manual_seed(5)
+    logits = torch.randn(B, n + 1, V, device="cuda", generator=g) * 3
+    q = torch.softmax(logits[:, :n] + 0.7 * torch.randn(B, n, V, device="cuda", generator=g), -1)
+    d = torch.multinomial(q.view(B * n, V), 1, generator=g).view(B, n).int()
+    d[5, 1], d[6, 0] = -1, V
+    au, su = (torch.rand(*x, device="cuda", generator=g) for x in ((B, n), (B,)))
+    temp = torch.full((B,), 1.0, device="cuda")
+    temp[7] = 0.0
+    logits[8, 0, 77], logits[9, 1, 5] = NAN, INF
+    t, c = rb.verify_draft(logits, d, au, su, temp, q)
+    assert len(set(c.tolist())) == n + 1
+    for b in range(B):
+        s = slice(b, b + 1)
+        tb, cb = rb.verify_draft(logits[s], d[s], au[s], su[s], temp[s], q[s])
+        assert torch.equal(tb, t[s]) and torch.equal(cb, c[s]), b
+
+
 def test_refusals(rb):
     d = [x.cuda() if x is not None else None for x in inputs(2, 3, 50)]
     ok = dict(logits=d[0], draft_tokens=d[1], accept_u=d[2], sample_u=d[3], temperature=d[4], draft_probs=d[5])
