@@ -130,7 +130,7 @@ def paged_attention(q: torch.Tensor, pos: torch.Tensor, page_table: torch.Tensor
         size = _workspace[key] = L.riallm_cuda_paged_attention_workspace(ctx.ptr, B, T, nh, nkv, d, max_pages, ps)
     # From the caching allocator, in the order of the call's stream: two calls
     # never share one, whatever streams or graphs they are in.
-    ws = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
+    ws = q.new_empty((size + 1) // 2) if size else None
     try:
         args = _ATTEND.pack(q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), pos.data_ptr(),
                             page_table.data_ptr(), out.data_ptr(), _table_stride(page_table), max_pages, num_pages, ps,

@@ -51,22 +51,39 @@ def verify_draft(logits: torch.Tensor, draft_tokens: Optional[torch.Tensor], acc
     B, n1, V = logits.shape
     n, device, f32 = n1 - 1, logits.device, torch.float32
 
-    def check(t, dtype, shape, name):
-        if not (t.dtype is dtype and t.shape == shape and t.get_device() == dev and t.is_contiguous()):
-            raise ConfigError(f"verify_draft: {name} must be contiguous {dtype} {list(shape)} on the logits' device")
-
-    if n or draft_tokens is not None:
-        _need(draft_tokens is not None and accept_u is not None, "draft_tokens and accept_u are wanted")
-        check(draft_tokens, torch.int32, (B, n), "draft_tokens")
-        check(accept_u, f32, (B, n), "accept_u")
-    check(sample_u, f32, (B,), "sample_u")
-    if draft_probs is not None:
-        check(draft_probs, f32, (B, n, V), "draft_probs")
     if not isinstance(temperature, torch.Tensor):
         temperature = torch.full((B,), float(temperature), dtype=f32, device=device)
-    check(temperature, f32, (B,), "temperature")
-    tokens = torch.empty((B, n1), dtype=torch.int32, device=device)
-    accepted = torch.empty((B,), dtype=torch.int32, device=device)
+    rows, drafts = (B,), (B, n)
+    # A step of a small model is a few launches long: what holds costs little,
+    # and the message is worked out only for what does not.
+    if not (sample_u.dtype is f32 and sample_u.shape == rows and sample_u.get_device() == dev
+            and sample_u.is_contiguous()
+            and temperature.dtype is f32 and temperature.shape == rows and temperature.get_device() == dev
+            and temperature.is_contiguous()
+            and (draft_tokens is accept_u is None and n == 0 or draft_tokens is not None and accept_u is not None
+                 and draft_tokens.dtype is torch.int32 and draft_tokens.shape == drafts
+                 and draft_tokens.get_device() == dev and draft_tokens.is_contiguous()
+                 and accept_u.dtype is f32 and accept_u.shape == drafts and accept_u.get_device() == dev
+                 and accept_u.is_contiguous())
+            and (draft_probs is None or draft_probs.dtype is f32 and draft_probs.shape == (B, n, V)
+                 and draft_probs.get_device() == dev and draft_probs.is_contiguous())):
+        def check(t, dtype, shape, name):
+            if not (t.dtype is dtype and t.shape == shape and t.get_device() == dev and t.is_contiguous()):
+                raise ConfigError(f"verify_draft: {name} must be contiguous {dtype} {list(shape)} on the logits' "
+                                  "device")
+
+        if n or draft_tokens is not None:
+            _need(draft_tokens is not None and accept_u is not None, "draft_tokens and accept_u are wanted")
+            check(draft_tokens, torch.int32, drafts, "draft_tokens")
+            check(accept_u, f32, drafts, "accept_u")
+        check(sample_u, f32, rows, "sample_u")
+        check(temperature, f32, rows, "temperature")
+        if draft_probs is not None:
+            check(draft_probs, f32, (B, n, V), "draft_probs")
+    if n:
+        tokens, accepted = draft_tokens.new_empty((B, n1)), draft_tokens.new_empty(B)
+    else:
+        tokens, accepted = (torch.empty(x, dtype=torch.int32, device=device) for x in ((B, n1), B))
     ctx = _context("verify_draft", ctx, dev)
     L = lib()
     key = (dev, B, n, V)
@@ -75,7 +92,7 @@ def verify_draft(logits: torch.Tensor, draft_tokens: Optional[torch.Tensor], acc
         if len(_workspace) > 4096:
             _workspace.clear()
         size = _workspace[key] = L.riallm_cuda_verify_draft_workspace(ctx.ptr, B, n, V)
-    ws = torch.empty(size, dtype=torch.uint8, device=device)
+    ws = sample_u.new_empty((size + 3) // 4)  # per call, in its stream's order
     args = _VERIFY.pack(logits.data_ptr(), draft_tokens.data_ptr() if n else 0,
                         draft_probs.data_ptr() if draft_probs is not None and n else 0, temperature.data_ptr(),
                         accept_u.data_ptr() if n else 0, sample_u.data_ptr(), tokens.data_ptr(), accepted.data_ptr(),
