@@ -16,18 +16,25 @@
 // Temperature 0 (and a row whose softmax is undefined: a NaN, +inf, or -inf
 // throughout) puts all of p_i on the first maximum.
 //
-// Three launches:
+// Three or four launches:
 //   stats_kernel : every row's maximum and sum of exponentials in float32, a
-//                  slice of a row per CTA; bound by reading the logits once
-//                  and, nearly, by the exponentials;
-//   weigh_kernel : finds a sequence's first rejection (a comparison that
+//                  slice of a row per CTA; bound by the exponential unit and
+//                  by reading the logits once;
+//   judge        : finds a sequence's first rejection (a comparison that
 //                  float32 sums leave within 1e-4 of equality is made again
-//                  with 64-bit ones) and goes over the one row that the token
-//                  comes from, in 64 bits, a chunk of the vocabulary per CTA;
+//                  with 64-bit ones), in judge_kernel or, for small calls, in
+//                  every CTA of weigh_kernel;
+//   weigh_kernel : goes over the one row that the token comes from, in 64
+//                  bits, a chunk of the vocabulary per CTA; bound by its
+//                  instructions, 20 a token;
 //   pick_kernel  : the chunks' weights after the draft's distribution is taken
-//                  off; a sequence's last CTA finds the token.
-// (A cluster of CTAs per sequence in place of the last two takes 280 us for
-// 128 sequences of 128001 tokens: its fixed cost, 10 us, comes 8 times over.)
+//                  off; a sequence's last CTA finds the token. Bound by the
+//                  same.
+// 128 sequences of 4 drafts over 128001 tokens (bf16 logits and float32 draft
+// probabilities, 262 MB): 100 us, 2.6 TB/s, of which the four take about 35,
+// 7, 22 and 36 %; one sequence: 16 us with the host's part. A cluster of CTAs
+// per sequence in place of the last three takes 218 us (8 CTAs) or 352 (16):
+// its fixed cost, 10 us, comes 8 times over.
 #include <algorithm>
 #include <cmath>
 
@@ -685,7 +692,9 @@ int32_t launch_verify(riallm_ctx* ctx, const char* what, const VerifyArgs& a, in
   const unsigned rows = (unsigned)B * (a.n + 1);
   if (int r = rl::launched(ctx, what, rl::launch_pdl(stats_kernel<kBf16>, dim3(rows * ws.slices), dim3(kThreads), 0, st, a, ws)))
     return r;
-  // A launch costs 2 us; every CTA's own verdict a third of a chunk's time.
+  // A launch costs 2 us (128 sequences, 32000 tokens, 640 CTAs: 47 us without
+  // it, 51 with it); where CTAs come in more than one wave, 5 an SM, their own
+  // verdicts cost more (128001 tokens, 2048 CTAs: 115 and 109 us).
   const bool apart = B * ws.chunks > 5 * ctx->num_sms;
   if (apart)
     if (int r = rl::launched(ctx, what, rl::launch_pdl(judge_kernel<kBf16>, dim3(B), dim3(kThreads), 0, st, a, ws)))

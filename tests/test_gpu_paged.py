@@ -137,6 +137,52 @@ def test_attention(rb, shape, window, sinks):
     check(attend(rb, s, window, sinks), reference(s, window, sinks))
 
 
+# 17 to 64 rows per kv head: each number of row tiles, whole and not, many
+# sequences, few long ones.
+SOME_ROWS = [
+    (2, 17, 4, 4, 128, 16, [17, 130]),
+    (3, 5, 32, 8, 128, 64, [700, 5, 64]),
+    (2, 8, 8, 2, 64, 16, [8, 1000]),
+    (2, 11, 6, 2, 128, 32, [11, 333]),
+    (40, 6, 12, 2, 128, 32, [6 + (i * 53) % 300 for i in range(40)]),
+    (2, 4, 24, 2, 64, 128, [260, 7]),
+    (1, 7, 14, 2, 128, 16, [4001]),
+    (2, 9, 14, 2, 64, 64, [1500, 77]),
+    (3, 16, 8, 2, 128, 16, [16, 81, 500]),
+    (1, 1, 64, 1, 128, 16, [900]),
+    (2, 1, 39, 1, 64, 32, [33, 1200]),
+]
+
+
+@pytest.mark.parametrize("window,sinks", [(0, 0), (1, 0), (20, 4), (100, 70)])
+@pytest.mark.parametrize("shape", SOME_ROWS, ids=str)
+def test_attention_some_rows(rb, shape, window, sinks):
+    s = poison(make(*shape), window, sinks)
+    check(attend(rb, s, window, sinks), reference(s, window, sinks))
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("T", [5, 9, 13, 16])
+def test_some_rows_later_token(rb, T, d):
+    """A token that is not finite does not reach the rows before it, in
+    whichever row tile they lie; the pool itself is not changed."""
+    s = make(2, T, 8, 2, d, 32, [150 + T, 40 + T])
+    clean, k0, v0 = attend(rb, s), s["k"].clone(), s["v"].clone()
+    for b, start in ((0, 150), (1, 40)):
+        for off in (0, T // 2, T - 1):
+            at = start + off
+            page, slot = int(s["table"][b, at // 32]), at % 32
+            for name, value in (("v", NAN), ("v", float("inf")), ("k", NAN)):
+                s[name][page, :, slot] = value
+                held = s[name].clone()
+                out = attend(rb, s).float().view(2, T, -1)
+                assert torch.equal(torch.nan_to_num(s[name].float(), 7.0), torch.nan_to_num(held.float(), 7.0))
+                s["k"].copy_(k0), s["v"].copy_(v0)
+                want = clean.float().view(2, T, -1)
+                assert torch.equal(out[1 - b], want[1 - b]) and torch.equal(out[b, :off], want[b, :off])
+                assert not torch.isfinite(out[b, off:]).any()
+
+
 @pytest.mark.parametrize("B,T,lens,window", [(1, 1, [30001], 0), (2, 1, [9000, 20011], 4096), (1, 4, [12003], 0),
                                              (300, 1, [1 + (i * 37) % 400 for i in range(300)], 0),
                                              (1, 300, [5000], 1000)])
