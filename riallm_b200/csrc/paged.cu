@@ -404,7 +404,7 @@ __device__ __forceinline__ uint32_t odd16(uint32_t x) { return ((x & 0x7f807f80u
 // what even these instructions can do at the rate the bytes arrive, so
 // nothing is gained by a 128-row tcgen05 tile of which 4 to 16 rows are
 // used. 8 kv heads of 128: one sequence of 131071 keys (537 MB) takes 98 us,
-// 5.5 TB/s; 96 of up to 16000 (3.3 GB) 530 to 570 us, 5.7 to 6.2 TB/s; 32 of
+// 5.5 TB/s; 96 of up to 16384 (3.3 GB) 530 to 570 us, 5.7 to 6.2 TB/s; 32 of
 // up to 2000 (135 MB) 32.6 us, of which the start, the groups' ends and
 // join_kernel are about 10. Two CTAs an SM, as 8 warps hide what one warp's
 // chain of load, product, maximum and product leaves open.
@@ -710,10 +710,10 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
 // 10 and 11 look through the values of blocks that some row of the tile does
 // not see whole. Keys and values share a ring of kStages blocks in smem.
 //
-// 4096 tokens, 32 heads of 128: 172 to 177 us, 780 to 800 TFLOP/s. Two times
-// 2501 tokens, heads of 64, window 2048: 106 us, 400 TFLOP/s (exponentials
-// alone: 36). 16 sequences with 6 drafted tokens each over up to 4001 keys
-// (147 MB): 46.6 us, 3.2 TB/s. A slot's block is a chain of product, maximum,
+// 4096 tokens, 32 heads of 128: 172 us, 800 TFLOP/s. Two times
+// 2501 tokens, heads of 64, window 2048: 103 us, 410 TFLOP/s (exponentials
+// alone: 36). 16 sequences of 6 tokens, 5 of them drafts, over up to 4001 keys
+// (147 MB): 45.6 us, 3.2 TB/s. A slot's block is a chain of product, maximum,
 // exponentials and product, 2500 of its 3700 cycles the weights'; the other
 // slot's chain fills what one leaves. 17 to 64 rows on m16n8k16 instead,
 // keys split over warps, take 105 us where this takes 47.
@@ -1301,21 +1301,26 @@ __global__ void __launch_bounds__(kManyThreads, 1)
   if (warp == 9) rl::tmem_dealloc(tm, 512);
 }
 
-// CTA (c, y, z) adds up kRows rows from kRows y on, 4 * kCols columns from
-// there times z on, of the partial results of the group that share c's record
-// names. A thread takes 4 columns of a row; where a group has many parts and
-// few rows, several threads share its parts. Bound by latency: two launches
-// over 256 keys take 7.7 us where one without a cut takes 4; a CTA for all of
-// a row's columns and a thread for all parts cost 3 us more (131071 keys, 37
-// parts a group) to 5 (drafted tokens).
+// CTA (c, y, z) adds up kRows rows from kRows y on, 4 kCols kPieces columns
+// from there times z on, of the partial results of the group that share c's
+// record names. A thread takes 4 columns of a row, kPieces times; where a
+// group has many parts and few rows, several threads share its parts. Bound by
+// latency, so what a CTA does is as much as keeps all CTAs in one wave: 256
+// rows of 128 columns in 32 CTAs of one piece take 2 to 4 us more than in 8
+// of four (4096 tokens 175 and 172 us, 128 tokens 17.7 and 14.1), and a CTA
+// for all columns of 16 or 128 rows, with a thread for all parts, 3 us more
+// (131071 keys, 37 parts a group) to 5 (drafted tokens) than this.
 constexpr int kMaxShares = 320, kJoinThreads = 256;
+template <typename Sh, int D>
+constexpr int kJoinPieces = Sh::R == 256 ? D / 32 : 1;
 template <typename Sh, int D>
 struct Join {
   static constexpr bool kMany = kByColumn<Sh>;
   static constexpr int kRows = kMany ? 32 : 2;
   static constexpr int kCols = kMany ? 8 : D / 4;
   static constexpr int kShared = kJoinThreads / (kRows * kCols);
-  static constexpr int kZ = D / (4 * kCols);
+  static constexpr int kPieces = kJoinPieces<Sh, D>;  // of 4 columns, a thread
+  static constexpr int kZ = D / (4 * kCols * kPieces);
   static constexpr int kPer = kMany ? kJoinThreads / kRows : 32;  // threads that work out a row's weights
 };
 template <typename Sh, int D>
@@ -1339,21 +1344,27 @@ __global__ void __launch_bounds__(kJoinThreads)
   {
     const int r = tid / J::kPer, i0 = tid % J::kPer;
     const bool have = r < rows;
-    float M = -INFINITY;
+    auto part_of = [&](int i) { return (i ? rest + (int64_t)i * 2 * kSlot : first) + row0 + r; };
+    // A thread's first part, usually its only one, stays in registers.
+    const bool any = have && i0 < parts;
+    const float m0 = any ? __ldcg(part_of(i0)) : -INFINITY, l0 = any ? __ldcg(part_of(i0) + Sh::R) : 0.f;
+    float M = m0;
     if (have)
-      for (int i = i0; i < parts; i += J::kPer) {
-        const float x = __ldcg((i ? rest + (int64_t)i * 2 * kSlot : first) + row0 + r);
+      for (int i = i0 + J::kPer; i < parts; i += J::kPer) {
+        const float x = __ldcg(part_of(i));
         weight[r][i] = x;
         M = fmaxf(M, x);
       }
 #pragma unroll
     for (int o = J::kPer / 2; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-    float den = 0.f;
+    const float base = M == -INFINITY ? 0.f : M, f0 = ex2(m0 - base);
+    float den = f0 * l0;
+    if (any) weight[r][i0] = f0;
     if (have)
-      for (int i = i0; i < parts; i += J::kPer) {
-        const float f = M == -INFINITY ? 0.f : ex2(weight[r][i] - M);
+      for (int i = i0 + J::kPer; i < parts; i += J::kPer) {
+        const float f = ex2(weight[r][i] - base);
         weight[r][i] = f;
-        den = fmaf(f, __ldcg((i ? rest + (int64_t)i * 2 * kSlot : first) + Sh::R + row0 + r), den);
+        den = fmaf(f, __ldcg(part_of(i) + Sh::R), den);
       }
 #pragma unroll
     for (int o = J::kPer / 2; o > 0; o >>= 1) den += __shfl_xor_sync(0xffffffffu, den, o);
@@ -1364,39 +1375,50 @@ __global__ void __launch_bounds__(kJoinThreads)
   __syncthreads();
   // Neighbours hold neighbouring rows where the parts are stored by column.
   const int r = J::kMany ? tid % J::kRows : tid / J::kCols % J::kRows;
-  const int c = (blockIdx.z * J::kCols + (J::kMany ? tid / J::kRows : tid % J::kCols)) * 4;
+  const int col0 = (blockIdx.z * J::kCols * J::kPieces + (J::kMany ? tid / J::kRows : tid % J::kCols)) * 4;
   const int turn = J::kMany ? 0 : tid / (J::kRows * J::kCols);
-  float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+  float4 y[J::kPieces];
+#pragma unroll
+  for (int x = 0; x < J::kPieces; ++x) y[x] = make_float4(0.f, 0.f, 0.f, 0.f);
   if (r < rows) {
-#pragma unroll 8
+#pragma unroll 8 / J::kPieces
     for (int i = turn; i < parts; i += J::kShared) {
       const float* p = (i ? rest + (int64_t)i * 2 * kSlot : first) + 2 * Sh::R;
-      float4 z;
-      if (J::kMany) {
-        p += c * Sh::R + row0 + r;
-        z = make_float4(__ldcg(p), __ldcg(p + Sh::R), __ldcg(p + 2 * Sh::R), __ldcg(p + 3 * Sh::R));
-      } else {
-        z = __ldcg(reinterpret_cast<const float4*>(p + (row0 + r) * D + c));
+      float4 z[J::kPieces];
+#pragma unroll
+      for (int x = 0; x < J::kPieces; ++x) {
+        const int c = col0 + x * J::kCols * 4;
+        if (J::kMany) {
+          const float* e = p + c * Sh::R + row0 + r;
+          z[x] = make_float4(__ldcg(e), __ldcg(e + Sh::R), __ldcg(e + 2 * Sh::R), __ldcg(e + 3 * Sh::R));
+        } else {
+          z[x] = __ldcg(reinterpret_cast<const float4*>(p + (row0 + r) * D + c));
+        }
       }
       const float w = weight[r][i];
-      y.x = fmaf(w, z.x, y.x);
-      y.y = fmaf(w, z.y, y.y);
-      y.z = fmaf(w, z.z, y.z);
-      y.w = fmaf(w, z.w, y.w);
+#pragma unroll
+      for (int x = 0; x < J::kPieces; ++x) {
+        y[x].x = fmaf(w, z[x].x, y[x].x);
+        y[x].y = fmaf(w, z[x].y, y[x].y);
+        y[x].z = fmaf(w, z[x].z, y[x].z);
+        y[x].w = fmaf(w, z[x].w, y[x].w);
+      }
     }
   }
   if (J::kShared > 1) {
-    red[tid] = y;
+    red[tid] = y[0];
     __syncthreads();
     if (turn) return;
     for (int i = 1; i < J::kShared; ++i) {
       const float4 z = red[i * J::kRows * J::kCols + tid];
-      y.x += z.x, y.y += z.y, y.z += z.z, y.w += z.w;
+      y[0].x += z.x, y[0].y += z.y, y[0].z += z.z, y[0].w += z.w;
     }
   }
   if (r < rows)
-    *reinterpret_cast<uint2*>(a.out + head_of(a, t, cut.kh, row0 + r) * D + c) =
-        make_uint2(rl::pack_bf16x2(y.x, y.y), rl::pack_bf16x2(y.z, y.w));
+#pragma unroll
+    for (int x = 0; x < J::kPieces; ++x)
+      *reinterpret_cast<uint2*>(a.out + head_of(a, t, cut.kh, row0 + r) * D + col0 + x * J::kCols * 4) =
+          make_uint2(rl::pack_bf16x2(y[x].x, y[x].y), rl::pack_bf16x2(y[x].z, y[x].w));
 }
 
 // The kernel for a call, its row tiles and CTAs, and whether a group can be

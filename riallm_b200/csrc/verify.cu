@@ -30,7 +30,7 @@
 //   pick_kernel  : the chunks' weights after the draft's distribution is taken
 //                  off; a sequence's last CTA finds the token. Bound by the
 //                  same.
-// 128 sequences of 4 drafts over 128001 tokens (bf16 logits and float32 draft
+// 128 sequences of 5 drafts over 128001 tokens (bf16 logits and float32 draft
 // probabilities, 262 MB): 100 us, 2.6 TB/s, of which the four take about 35,
 // 7, 22 and 36 %; one sequence: 16 us with the host's part. A cluster of CTAs
 // per sequence in place of the last three takes 218 us (8 CTAs) or 352 (16):
