@@ -704,32 +704,34 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
 //   kTwoTiles  : 256 rows a tile, a slot each half, both against every block
 //                (a block's keys and values are read once for 256 rows);
 //   !kTwoTiles : up to 128 rows a tile, the slots take the blocks in turn
-//                and are added up at the group's end.
+//                and are added up at the group's end, half of the columns by
+//                each slot's warps; the next group's queries are loaded
+//                meanwhile.
 // Roles: warps 0-3 and 4-7 the two slots' weights (a thread a row), warp 8
 // loads blocks by TMA, page by page, warp 9 issues the products, warps
 // 10 and 11 look through the values of blocks that some row of the tile does
 // not see whole. Keys and values share a ring of kStages blocks in smem.
 //
-// 4096 tokens, 32 heads of 128: 172 us, 800 TFLOP/s. Two times
+// 4096 tokens, 32 heads of 128: 170 us, 810 TFLOP/s. Two times
 // 2501 tokens, heads of 64, window 2048: 103 us, 410 TFLOP/s (exponentials
 // alone: 36). 16 sequences of 6 tokens, 5 of them drafts, over up to 4001 keys
-// (147 MB): 45.6 us, 3.2 TB/s. A slot's block is a chain of product, maximum,
+// (147 MB): 43 us, 3.4 TB/s. A slot's block is a chain of product, maximum,
 // exponentials and product, 2500 of its 3700 cycles the weights'; the other
 // slot's chain fills what one leaves. 17 to 64 rows on m16n8k16 instead,
-// keys split over warps, take 105 us where this takes 47.
+// keys split over warps, take 105 us where this takes 43.
 constexpr int kManyThreads = 12 * 32;
 // Registers: the launch's 168 a thread, of which the third warpgroup (loads,
 // products) keeps 72 and the weights' two take 216 (2 * 216 + 72 = 3 * 168).
 constexpr int kWeightRegs = 216, kOtherRegs = 72;
 constexpr int kMaxStages = 8;
 template <bool kTwoTiles>
-using Many = Shape<kTwoTiles ? 256 : 128, 128, 4>;
+using Many = Shape<kTwoTiles ? 256 : 128, 128, kTwoTiles ? 4 : 3>;
 template <int D>
-constexpr int kManyStages = D == 128 ? 4 : 8;
+constexpr int kManyStages = D == 128 ? 4 : 8;  // even: keys and values keep to stages of their own
 template <int D>
 constexpr int kTileBytes = 128 * D * 2;
-// Two query tiles (with !kTwoTiles one, and room to add the slots up), the
-// ring, and slack to start at a multiple of 1024.
+// Two query tiles (with !kTwoTiles one group's and the next one's), the ring,
+// and slack to start at a multiple of 1024.
 template <int D>
 constexpr int kManySmem = (2 + kManyStages<D>) * kTileBytes<D> + 1024;
 
@@ -788,12 +790,10 @@ __global__ void __launch_bounds__(kManyThreads, 1)
   __shared__ int abort_flag;
   __shared__ uint32_t gone[8];    // block n % 8: its pages that are not held, or that nobody sees
   __shared__ int poison[16];      // segment n % 16: a value that some rows must not meet is not finite
-  __shared__ float ml[2][128];    // slot 1's maxima and sums, !kTwoTiles
-  __shared__ Segments<Sh> at_seg[8];  // of each weights' warp: its registers are for weights
+  __shared__ Segments<Sh> at_seg[8], at_next[8];  // of each weights' warp: its registers are for weights
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  uint8_t* qs = smem;                          // 2 tiles
+  uint8_t* qs = smem;  // 2 tiles
   uint8_t* ring = smem + 2 * kTileBytes<D>;
-  float* merge = reinterpret_cast<float*>(smem + kTileBytes<D>);  // [D / 2 columns][128 rows], !kTwoTiles
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   volatile int* abort = &abort_flag;
 
@@ -810,8 +810,8 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       rl::mbar_init(&bars.p_full[i][1], 4);
       rl::mbar_init(&bars.pv_done[i], 1);
     }
-    rl::mbar_init(&bars.merge_full, 128);
-    rl::mbar_init(&bars.merge_empty, 128);
+    rl::mbar_init(&bars.merge_full, 8);
+    rl::mbar_init(&bars.merge_empty, 8);
     rl::mbar_init(&bars.drain, 1);
     rl::fence_mbar_init();
     abort_flag = 0;
@@ -888,8 +888,9 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         const uint64_t q_desc = rl::sdesc_kmajor_sw128(rl::smem_u32(qs));
         const uint64_t k_desc = rl::sdesc_kmajor_sw128(rl::smem_u32(ring));
         const uint64_t v_desc = rl::sdesc_mnmajor_sw128(rl::smem_u32(ring), kHalf);
+        int n0 = 0, seg = 0;  // blocks before this segment, segments
         auto scores = [&](int slot, int st) {
-          const uint64_t qd = q_desc + (kTwoTiles ? slot * (kTileBytes<D> >> 4) : 0), kd = k_desc + st * (kTileBytes<D> >> 4);
+          const uint64_t qd = q_desc + (kTwoTiles ? slot : seg & 1) * (kTileBytes<D> >> 4), kd = k_desc + st * (kTileBytes<D> >> 4);
           if (leader) {
 #pragma unroll
             for (int x = 0; x < D / 16; ++x) {
@@ -922,7 +923,6 @@ __global__ void __launch_bounds__(kManyThreads, 1)
           if (leader) rl::tc_commit(&bars.empty[st]);
           __syncwarp();
         };
-        int n0 = 0, seg = 0;      // blocks before this segment, segments
         bool go = true;
         do {
           const int nb = sg.i1 - sg.i0;
@@ -1050,26 +1050,28 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       int seg = 0, n0 = 0;  // segments, blocks before this one
       uint32_t sc = 0;      // blocks of this slot so far: phases of s_full and pv_done
       bool go = true;
+      // A segment's query rows, 32 by this warp (16 with one tile), 16 bytes a
+      // lane.
+      auto load_q = [&](const Tile& t, int kh, int segment) {
+        constexpr int kRowsPerWarp = kTwoTiles ? 32 : 16, C = D / 8;
+        uint8_t* tile = qs + (kTwoTiles ? slot : segment & 1) * kTileBytes<D>;
+#pragma unroll
+        for (int x = 0; x < kRowsPerWarp * C / 32; ++x) {
+          const int rr = warp * kRowsPerWarp + (x * 32 + lane) / C, c = lane % C, lr = rr & 127;
+          const bool have = rr < t.rows;
+          cp_async_16z(tile + (c / 8) * kHalf + lr * 128 + (((c & 7) ^ (lr & 7)) * 16),
+                       a.q + head_of(a, t, kh, have ? rr : 0) * D + c * 8, have ? 16 : 0);
+        }
+        rl::cp_async_commit();
+      };
       do {
         const Tile& t = sg.c.t;
         const int nb = sg.i1 - sg.i0;
-        // The query rows, 32 by this warp (16 with one tile), 16 bytes a lane.
-        {
-          constexpr int kRowsPerWarp = kTwoTiles ? 32 : 16, C = D / 8;
-          uint8_t* tile = qs + (kTwoTiles ? slot * kTileBytes<D> : 0);
-#pragma unroll
-          for (int x = 0; x < kRowsPerWarp * C / 32; ++x) {
-            const int rr = warp * kRowsPerWarp + (x * 32 + lane) / C, c = lane % C, lr = rr & 127;
-            const bool have = rr < t.rows;
-            cp_async_16z(tile + (c / 8) * kHalf + lr * 128 + (((c & 7) ^ (lr & 7)) * 16),
-                         a.q + head_of(a, t, sg.c.kh, have ? rr : 0) * D + c * 8, have ? 16 : 0);
-          }
-          rl::cp_async_commit();
-          rl::cp_async_wait<0>();
-          rl::fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) rl::mbar_arrive(&bars.q_full);
-        }
+        if (kTwoTiles || seg == 0) load_q(t, sg.c.kh, seg);
+        rl::cp_async_wait<0>();
+        rl::fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) rl::mbar_arrive(&bars.q_full);
         const bool in = r < t.rows;
         const Span sp = in ? a.span(t.p0 + token_of(a, t, r)) : Span{0, -1};
         // Blocks that every row of this warp sees whole end at most at
@@ -1166,7 +1168,18 @@ __global__ void __launch_bounds__(kManyThreads, 1)
           ++done;
         }
         if (!go) break;
-        // The group ends, or this CTA's share of it.
+        // The group ends, or this CTA's share of it. The next one is found
+        // while the last products run; with one tile its queries go where
+        // those of the group before this one were.
+        int more = 0;
+        if (lane == 0) {
+          Segments<Sh> after = sg;
+          more = after.next(a, tiles);
+          at_next[warp] = after;
+        }
+        __syncwarp();
+        more = __shfl_sync(0xffffffffu, more, 0);
+        if (!kTwoTiles && more) load_q(at_next[warp].c.t, at_next[warp].c.kh, seg + 1);
         if (done) {
           go = warp_wait(&bars.pv_done[slot], (sc - 1) & 1, abort, status);
           if (!go) break;
@@ -1175,58 +1188,62 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         const bool whole = sg.i0 == 0 && sg.i1 == t.bl.n;
         bool odd = false;
         float* part = ws + (2 * (int64_t)blockIdx.x + (seg == 0 ? 0 : 1)) * kSlotFloats<Sh, D>;
-        float mine = 1.f, other = 0.f;  // factors of the slots' sums
+        float f0 = 1.f, f1 = 0.f;  // factors of the slots' sums
         if constexpr (!kTwoTiles) {
-          if (slot == 1) {
-            ml[0][r] = m;
-            ml[1][r] = l;
-          }
-        }
-#pragma unroll 1
-        for (int y = 0; go && y < D / 32; ++y) {
-          uint32_t v[32];
+          // Both slots' sums are where either's warps can read them: a warp
+          // adds up half of the columns of its rows. Maxima and sums go by
+          // way of the query tile: when a slot's last block is done, so are
+          // all products of scores.
+          float* ml = reinterpret_cast<float*>(qs + (seg & 1) * kTileBytes<D>);
           if (done) {
+            ml[slot * 256 + r] = m;
+            ml[slot * 256 + 128 + r] = l;
+          }
+          rl::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) rl::mbar_arrive(&bars.merge_full);
+          go = warp_wait(&bars.merge_full, seg & 1, abort, status);
+          if (!go) break;
+          rl::tc_fence_after();
+          const float m0 = ml[r], m1 = nb > 1 ? ml[256 + r] : -INFINITY;  // slot 1 has no block of one
+          m = fmaxf(m0, m1);
+          const float base = m == -INFINITY ? 0.f : m;
+          f0 = ex2(m0 - base);
+          f1 = ex2(m1 - base);
+          l = ml[128 + r] * f0;
+          if (nb > 1) l = fmaf(ml[384 + r], f1, l);
+        }
+        // Here every block of the segment has been multiplied, the other
+        // slot's too, so it has been looked through.
+        odd = *(volatile int*)&poison[seg & 15] != 0;
+        if (!whole && in && (kTwoTiles || slot == 0)) {
+          part[r] = m;
+          part[Sh::R + r] = l;
+        }
+        constexpr int kPieces = kTwoTiles ? D / 32 : D / 64;  // of 32 columns
+        const int y0 = kTwoTiles ? 0 : slot * kPieces;
+        const bool rows = w0 < t.rows;  // of this warp
+#pragma unroll 1
+        for (int y = y0; rows && y < y0 + kPieces; ++y) {
+          uint32_t v[32];
+          if constexpr (kTwoTiles) {
             rl::tmem_ld_32x32b_x32(to + y * 32, v);
             rl::tmem_wait_ld();
           } else {
+            rl::tmem_ld_32x32b_x32(tm + 256 + lane_off + y * 32, v);
+            rl::tmem_wait_ld();
 #pragma unroll
-            for (int e = 0; e < 32; ++e) v[e] = 0;
-          }
-          if constexpr (!kTwoTiles) {
-            // D / 2 columns at a time through shared memory, slot 1 to slot 0.
-            constexpr int kTurn = D / 64;  // 32-column pieces in a turn
-            const uint32_t turn = (seg * 2 + y / kTurn) & 1;
-            float* mc = merge + (y % kTurn) * 32 * 128 + r;
-            if (slot == 1) {
+            for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * f0);
+            if (nb > 1) {
 #pragma unroll
-              for (int e = 0; e < 32; ++e) mc[e * 128] = __uint_as_float(v[e]);
-              if (y % kTurn == kTurn - 1) {
-                rl::mbar_arrive(&bars.merge_full);
-                go = warp_wait(&bars.merge_empty, turn, abort, status);
+              for (int h = 0; h < 2; ++h) {
+                uint32_t u[16];
+                rl::tmem_ld_32x32b_x16(tm + 256 + lane_off + D + y * 32 + h * 16, u);
+                rl::tmem_wait_ld();
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                  v[h * 16 + e] = __float_as_uint(fmaf(__uint_as_float(u[e]), f1, __uint_as_float(v[h * 16 + e])));
               }
-              continue;
-            }
-            if (y % kTurn == 0) go = warp_wait(&bars.merge_full, turn, abort, status);
-            if (!go) break;
-            if (y == 0) {
-              const float m1 = ml[0][r], M = fmaxf(m, m1), base = M == -INFINITY ? 0.f : M;
-              mine = ex2(m - base);
-              other = ex2(m1 - base);
-              l = l * mine + ml[1][r] * other;
-              m = M;
-            }
-#pragma unroll
-            for (int e = 0; e < 32; ++e)
-              v[e] = __float_as_uint(fmaf(__uint_as_float(v[e]), mine, mc[e * 128] * other));
-            if (y % kTurn == kTurn - 1) rl::mbar_arrive(&bars.merge_empty);
-          }
-          if (y == 0) {
-            // Here every block of the segment has been multiplied, the other
-            // slot's too, so it has been looked through.
-            odd = *(volatile int*)&poison[seg & 15] != 0;
-            if (!whole && in) {
-              part[r] = m;
-              part[Sh::R + r] = l;
             }
           }
           if (!in) continue;
@@ -1269,7 +1286,6 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             for (int e = 0; e < 32; ++e) o[e * Sh::R] = __uint_as_float(v[e]);
           }
         }
-        if (!go) break;
         if (kTwoTiles && whole) {
           constexpr int C = D / 8;
           __syncwarp();
@@ -1283,15 +1299,18 @@ __global__ void __launch_bounds__(kManyThreads, 1)
           __syncwarp();
         }
         rl::tc_fence_before();  // the next group's first product overwrites O
+        if constexpr (!kTwoTiles) {
+          __syncwarp();
+          if (lane == 0) rl::mbar_arrive(&bars.merge_empty);
+          go = warp_wait(&bars.merge_empty, seg & 1, abort, status);
+          if (!go) break;
+        }
         n0 += nb;
         ++seg;
         __syncwarp();
-        if (lane == 0) {
-          Segments<Sh> after = sg;
-          work = after.next(a, tiles);
-          sg = after;
-        }
-        work = __shfl_sync(0xffffffffu, work, 0);
+        if (lane == 0) sg = at_next[warp];
+        __syncwarp();
+        work = more;
       } while (work);
     }
   }
