@@ -118,8 +118,10 @@ struct Part {
     for (int e = 1; e + 1 < N; e += 2) mx = rl::max3(mx, x[e], x[e + 1]);
     m = N > 1 ? rl::max3(m, mx, x[N - 1]) : fmaxf(m, mx);
     if ((m - base) * c > 60.f || !begun) {  // -inf and NaN leave base as it is
+      // Sums that have not begun are 0, or NaN, relative to whatever base: the
+      // power of a first maximum far below 0 is infinite, and 0 times it NaN.
+      const float b = m > -INFINITY ? m : 0.f, f = begun ? ex2((base - b) * c) : 1.f;
       begun = m > -INFINITY;
-      const float b = begun ? m : 0.f, f = ex2((base - b) * c);
       s0 *= f;
       s1 *= f;
       base = b;
