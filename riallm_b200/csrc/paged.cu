@@ -659,19 +659,21 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
         float M = sm_m[0][r];
 #pragma unroll
         for (int w = 1; w < kFewWarps; ++w) M = fmaxf(M, sm_m[w][r]);
+        // A row that sees nothing has sums of 0, one whose scores are all NaN
+        // the same maximum and sums of NaN, which stay.
+        const float base = M == -INFINITY ? 0.f : M;
         float L = 0.f;
         float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (M != -INFINITY)
 #pragma unroll
-          for (int w = 0; w < kFewWarps; ++w) {
-            const float f = ex2(sm_m[w][r] - M);
-            const float4 z = *reinterpret_cast<const float4*>(part + w * (S * 16 * D) + r * D + (c ^ ((r & 3) * 8)));
-            L = fmaf(sm_l[w][r], f, L);
-            y.x = fmaf(z.x, f, y.x);
-            y.y = fmaf(z.y, f, y.y);
-            y.z = fmaf(z.z, f, y.z);
-            y.w = fmaf(z.w, f, y.w);
-          }
+        for (int w = 0; w < kFewWarps; ++w) {
+          const float f = ex2(sm_m[w][r] - base);
+          const float4 z = *reinterpret_cast<const float4*>(part + w * (S * 16 * D) + r * D + (c ^ ((r & 3) * 8)));
+          L = fmaf(sm_l[w][r], f, L);
+          y.x = fmaf(z.x, f, y.x);
+          y.y = fmaf(z.y, f, y.y);
+          y.z = fmaf(z.z, f, y.z);
+          y.w = fmaf(z.w, f, y.w);
+        }
         if (whole) {
           const float inv = L == 0.f ? 0.f : __fdiv_rn(1.f, L);
           *reinterpret_cast<uint2*>(a.out + head_of(a, now.t, now.kh, r) * D + c) =
