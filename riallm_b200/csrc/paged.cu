@@ -387,6 +387,10 @@ __device__ __forceinline__ void cp_async_16z(void* dst, const void* src, int byt
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(rl::smem_u32(dst)), "l"(src), "r"(bytes)
                : "memory");
 }
+// The largest bf16 below a positive x, as the upper half of a float; 0 of 0.
+__device__ __forceinline__ uint32_t bf16_below(float x) {
+  return (uint32_t)max(__float_as_int(x) - 1, 0) & 0xffff0000u;
+}
 // Not 0 where either bf16 of x is infinite or NaN: an exponent of all ones
 // carries into the sign's place.
 __device__ __forceinline__ uint32_t odd16(uint32_t x) { return ((x & 0x7f807f80u) + 0x00800080u) & 0x80008000u; }
@@ -606,17 +610,20 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
         }
       }
       // The weights as bf16 and what that leaves, also as bf16: two products
-      // keep 16 bits of each weight (one alone costs as much accuracy again
+      // keep 15 bits of each weight (one alone costs as much accuracy again
       // as the rounding of the output), and the matrix pipe is idle anyway.
+      // The first is cut off below the weight, so that the second is above
+      // 0, too: with one of either sign, or 0, an infinite value that the
+      // row sees would come out as NaN.
       uint32_t ph[4], pr[4];
 #pragma unroll
       for (int y = 0; y < 2; ++y)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const float x0 = sc[y][2 * h], x1 = sc[y][2 * h + 1];
-          const uint32_t hi = rl::pack_bf16x2(x0, x1);
-          ph[2 * y + h] = hi;
-          pr[2 * y + h] = rl::pack_bf16x2(x0 - __uint_as_float(hi << 16), x1 - __uint_as_float(hi & 0xffff0000u));
+          const uint32_t h0 = bf16_below(x0), h1 = bf16_below(x1);
+          ph[2 * y + h] = __byte_perm(h0, h1, 0x7632);
+          pr[2 * y + h] = rl::pack_bf16x2(x0 - __uint_as_float(h0), x1 - __uint_as_float(h1));
         }
 #pragma unroll
       for (int x = 0; x < D / 16; ++x) {
