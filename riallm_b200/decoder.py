@@ -457,7 +457,12 @@ class Decoder:
         tokens are distributed as if sampled one by one, with random numbers
         from `generator` (a CUDA generator). Returns the new ids as generate
         does; draft_stats then tells the model steps taken and the drafts
-        proposed and accepted."""
+        proposed and accepted. Not for an expert-parallel decoder (ep), whose
+        ranks have to take steps of the same sizes together: here they depend
+        on what each rank's sequences propose and accept."""
+        if self.ep is not None:
+            raise ConfigError("generate_drafted does not run on an expert-parallel decoder: its ranks would take "
+                              "steps of different sizes")
         if drafts < 0 or drafts > 255:
             raise ConfigError("drafts must be in 0..255")
         if new_tokens <= 0:
