@@ -364,11 +364,12 @@ class Decoder:
 
     def _advance(self, B: int, T: int, idle: Sequence[int] = ()):
         """Room for T more positions of B sequences; `idle` ones get no pages
-        for them (what is written there is dropped)."""
+        for them (what is written there, or past the cache, is dropped)."""
         if B > self.max_batch:
             raise ConfigError(f"batch {B} > max_batch {self.max_batch}")
-        if self.length + T > self.max_seq:
-            raise ConfigError(f"sequence length {self.length + T} > max_seq {self.max_seq}")
+        held = max(n for b, n in enumerate(self._lengths[:B]) if b not in idle) if idle else self.length
+        if held + T > self.max_seq:
+            raise ConfigError(f"sequence length {held + T} > max_seq {self.max_seq}")
         if self.pages is not None:
             if self.window:
                 self.pages.release_before([n - self.window + 1 for n in self._lengths[:B]], self.sinks)
@@ -485,13 +486,14 @@ class Decoder:
             s.append(t)
         stats = {"steps": 1, "proposed": 0, "accepted": 0}
         while any(len(s) < d for s, d in zip(seqs, done)):
-            n = min(drafts, self.max_seq - self.length - 1)
+            idle = [b for b in range(B) if len(seqs[b]) >= done[b]]  # finished: they wait for the others
+            n = min(drafts, self.max_seq - max(self._lengths[b] for b in range(B) if b not in idle) - 1)
             want = [min(n, d - len(s) - 1) for s, d in zip(seqs, done)]
             guess = [list(propose(list(s), w))[:w] if w > 0 else [] for s, w in zip(seqs, want)]
             n = max(0, min(n, max(map(len, guess))))
             guess = [g + [-1] * (n - len(g)) for g in guess]
             before = self._lengths[:B]
-            self._advance(B, n + 1, [b for b in range(B) if len(seqs[b]) >= done[b]])
+            self._advance(B, n + 1, idle)
             draft = torch.tensor(guess, dtype=torch.int32, device=dev).view(B, n)
             last = torch.tensor([[s[-1]] for s in seqs], dtype=torch.long, device=dev)
             # A guess outside the vocabulary ends its sequence's drafts; the
@@ -501,8 +503,8 @@ class Decoder:
             out, accepted = verify_draft(logits, draft, uniform(B, n), uniform(B), temp, ctx=self.ctx)
             stats["steps"] += 1
             for b, (toks, a) in enumerate(zip(out.tolist(), accepted.tolist())):
-                if len(seqs[b]) >= done[b]:
-                    self._lengths[b] = before[b]  # finished: it waits for the others
+                if b in idle:
+                    self._lengths[b] = before[b]
                     continue
                 stats["proposed"] += sum(0 <= g < self.cfg.vocab for g in guess[b])
                 stats["accepted"] += a

@@ -68,3 +68,42 @@ def test_expert_parallel_is_refused(monkeypatch, rb):
     with pytest.raises(rb.ConfigError, match="expert-parallel"):
         m.generate_drafted(torch.tensor([1, 2, 3]), 5)
     assert log.calls == [] and m.length == 0
+
+
+@pytest.mark.parametrize("page_size", [0, 16])
+@pytest.mark.parametrize("prompt_len,new_tokens,max_seq", [(4, 13, 16), (5, 12, 16), (4, 12, 16), (4, 30, 64)])
+def test_a_finished_sequence_holds_nobody_up(monkeypatch, rb, prompt_len, new_tokens, max_seq, page_size):
+    """One sequence's drafts are all right and the others' are all wrong: the
+    first ends early, with the cache full where its length is max_seq, and the
+    others go on to the end, with drafts."""
+    def follow(t):
+        return (3 * t + 1) % 50
+
+    m, log = stub(monkeypatch, rb, 3, max_seq, follow, page_size=page_size)
+    prompt = torch.tensor([[1] * (prompt_len - 1) + [7], [2] * (prompt_len - 1) + [8], [3] * (prompt_len - 1) + [9]])
+    want = [plain(p, new_tokens, follow) for p in prompt.tolist()]
+
+    def propose(tokens, n):
+        if tokens[0] == 2:
+            return plain(tokens, n, follow)
+        return [(follow(tokens[-1]) + 1) % 50] * n
+
+    out = m.generate_drafted(prompt, new_tokens, drafts=4, propose=propose)
+    assert out.tolist() == want
+    steps = log.calls[1:]
+    # The two that are left take one token a step, each with as many drafts as
+    # the longest unfinished sequence has room for.
+    full = prompt_len + new_tokens - 1
+    assert len(steps) == new_tokens - 1
+    for i, (T, pos) in enumerate(steps):
+        longest = max(p for p in pos if p < full)
+        assert pos[0] == pos[2] == prompt_len + i and T == 1 + min(4, new_tokens - i - 2, max_seq - longest - 1)
+        assert longest + T <= max_seq
+    assert m._lengths == [full] * 3 and m.length == full and m.pos.tolist() == [full] * 3
+
+
+def test_room_is_asked_of_the_unfinished(monkeypatch, rb):
+    """More tokens than the cache holds are refused as before."""
+    m, _ = stub(monkeypatch, rb, 2, 16, lambda t: (t + 1) % 50)
+    with pytest.raises(rb.ConfigError, match="max_seq"):
+        m.generate_drafted(torch.tensor([[1, 2, 3, 4], [5, 6, 7, 8]]), 14)
