@@ -90,9 +90,12 @@ def rope_paged_append(qkv: torch.Tensor, pos: torch.Tensor, page_table: torch.Te
         _need(q_out.dtype is torch.bfloat16 and q_out.shape == (rows, nh * d) and q_out.get_device() == dev
               and q_out.is_contiguous(), "rope_paged_append: q_out must be contiguous bf16 [B*T, heads*head_dim]")
     ctx = _context("rope_paged_append", ctx, dev)
-    args = _APPEND.pack(qkv.data_ptr(), pos.data_ptr(), page_table.data_ptr(), inv_freq.data_ptr(), q_out.data_ptr(),
-                        k_pages.data_ptr(), v_pages.data_ptr(), _table_stride(page_table), page_table.shape[1],
-                        num_pages, ps, B, T, nh, nkv, d)
+    try:
+        args = _APPEND.pack(qkv.data_ptr(), pos.data_ptr(), page_table.data_ptr(), inv_freq.data_ptr(),
+                            q_out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), _table_stride(page_table),
+                            page_table.shape[1], num_pages, ps, B, T, nh, nkv, d)
+    except struct.error:
+        raise ConfigError("rope_paged_append: sizes must be 32-bit integers") from None
     status = lib().riallm_cuda_rope_paged_append(ctx.ptr, args, _stream(dev))
     if status:
         ctx.check(status)
@@ -136,7 +139,7 @@ def paged_attention(q: torch.Tensor, pos: torch.Tensor, page_table: torch.Tensor
                             page_table.data_ptr(), out.data_ptr(), _table_stride(page_table), max_pages, num_pages, ps,
                             B, T, nh, nkv, d, window, sinks)
     except struct.error:
-        raise ConfigError("paged_attention: window and sinks must be 32-bit integers") from None
+        raise ConfigError("paged_attention: sizes, window and sinks must be 32-bit integers") from None
     status = L.riallm_cuda_paged_attention(ctx.ptr, args, ws.data_ptr() if size else None, size, _stream(dev))
     if status:
         ctx.check(status)

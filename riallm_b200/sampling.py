@@ -93,10 +93,13 @@ def verify_draft(logits: torch.Tensor, draft_tokens: Optional[torch.Tensor], acc
             _workspace.clear()
         size = _workspace[key] = L.riallm_cuda_verify_draft_workspace(ctx.ptr, B, n, V)
     ws = sample_u.new_empty((size + 3) // 4)  # per call, in its stream's order
-    args = _VERIFY.pack(logits.data_ptr(), draft_tokens.data_ptr() if n else 0,
-                        draft_probs.data_ptr() if draft_probs is not None and n else 0, temperature.data_ptr(),
-                        accept_u.data_ptr() if n else 0, sample_u.data_ptr(), tokens.data_ptr(), accepted.data_ptr(),
-                        dtype, B, n, V)
+    try:
+        args = _VERIFY.pack(logits.data_ptr(), draft_tokens.data_ptr() if n else 0,
+                            draft_probs.data_ptr() if draft_probs is not None and n else 0, temperature.data_ptr(),
+                            accept_u.data_ptr() if n else 0, sample_u.data_ptr(), tokens.data_ptr(),
+                            accepted.data_ptr(), dtype, B, n, V)
+    except struct.error:
+        raise ConfigError("verify_draft: sizes must be 32-bit integers") from None
     status = L.riallm_cuda_verify_draft(ctx.ptr, args, ws.data_ptr(), size, _stream(dev))
     if status:
         ctx.check(status)
