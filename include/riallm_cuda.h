@@ -443,7 +443,8 @@ int32_t riallm_cuda_linear_bf16(riallm_ctx* ctx, const void* x, const void* w, v
 
 /* Host-only helper (no device work; page_table is host memory here): the
  * row of a pool, viewed as [num_pages * nkv * page_size, d], that holds
- * `position` of sequence b for kv_head; -1 where the sequence holds none. */
+ * `position` of sequence b for kv_head; -1 where the sequence holds none (or
+ * page_size is none of the above). */
 int64_t riallm_paged_row(const int32_t* page_table, int64_t table_stride, int32_t max_pages, int32_t num_pages,
                          int32_t nkv, int32_t page_size, int32_t b, int32_t kv_head, int64_t position);
 

@@ -1530,6 +1530,8 @@ int32_t launch_attention(riallm_ctx* ctx, const AttnArgs& a, const Plan& p, cons
 
 bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
+bool is_page_size(int32_t n) { return n == 16 || n == 32 || n == 64 || n == 128; }
+
 // What both entry points share: the checks of the cache's geometry.
 template <typename Args>
 int check_pages(riallm_ctx* ctx, const char* what, const Args& x) {
@@ -1539,8 +1541,7 @@ int check_pages(riallm_ctx* ctx, const char* what, const Args& x) {
     return bad("bad dimensions (heads must be a multiple of kv heads)");
   if (nh / nkv > 128) return bad("more than 128 heads per kv head");
   if (d != 64 && d != 128) return bad("head_dim must be 64 or 128");
-  if (page_size != 16 && page_size != 32 && page_size != 64 && page_size != 128)
-    return bad("page_size must be 16, 32, 64 or 128");
+  if (!is_page_size(page_size)) return bad("page_size must be 16, 32, 64 or 128");
   if (x.num_pages <= 0 || x.max_pages <= 0 || x.table_stride < x.max_pages) return bad("bad page table");
   // The kernels count positions in 32 bits, to the end of the last position's block and a page past it.
   if ((int64_t)x.num_pages * nkv * page_size > INT32_MAX || (int64_t)x.max_pages * page_size > INT32_MAX - 256)
@@ -1627,7 +1628,7 @@ extern "C" {
 
 int64_t riallm_paged_row(const int32_t* page_table, int64_t table_stride, int32_t max_pages, int32_t num_pages,
                          int32_t nkv, int32_t page_size, int32_t b, int32_t kv_head, int64_t position) {
-  if (!page_table) return -1;
+  if (!page_table || !is_page_size(page_size)) return -1;
   return make_pages(page_table, table_stride, max_pages, num_pages, nkv, page_size).row(b, kv_head, position);
 }
 
