@@ -409,14 +409,16 @@ __device__ __forceinline__ Verdict judge(const VerifyArgs& a, const Space& ws, c
       if (rows[i].top != kUndefined) continue;
       const float m = rows[i].m;
       const Logits<kBf16> logit(a, row0 + i);
-      int at = m == -INFINITY ? 0 : kUndefined;
+      int at = kUndefined;
       for (int j = tid; j < V && at == kUndefined; j += kThreads)
         if (logit(j) == m) at = j;
       __syncthreads();  // rows[i] has been read
-      if (tid == 0) rows[i].top = V - 1;
+      if (tid == 0) rows[i].top = V;
       __syncthreads();
       at = __reduce_min_sync(0xffffffffu, at);
       if (lane == 0) atomicMin(&rows[i].top, at);
+      __syncthreads();
+      if (tid == 0 && rows[i].top == V) rows[i].top = 0;  // nothing but NaN
       __syncthreads();
     }
   }
