@@ -99,9 +99,13 @@ struct Stat {
   float m, s;
   int top, pad;
 };
-// log2(e) / temperature, kept where 0 * c and inf * c are harmless.
+// log2(e) / temperature, kept where 0 * c and inf * c are harmless: from the
+// smallest number (of an infinite temperature) to the largest. That one is
+// not the quotient of temperatures below kTiny: what the statistics say of
+// their sums is not used.
+constexpr float kTiny = 4.5e-39f;  // above log2(e) / FLT_MAX
 __device__ __forceinline__ float scale_of(float t) {
-  return t > 0.f ? fminf(fmaxf(1.4426950408889634f / t, 1e-30f), 1e30f) : 1.f;
+  return t > 0.f ? fminf(fmaxf(1.4426950408889634f / t, 1.4e-45f), 3.402823466e38f) : 1.f;
 }
 
 // A thread's part of a slice. Its sum is relative to `base`, at most 60
@@ -436,7 +440,7 @@ __device__ __forceinline__ Verdict judge(const VerifyArgs& a, const Space& ws, c
         no = !(lhs < (x == r.top ? 1.0 : 0.0));
       } else {
         const double p = Exp64(table, r.m, scale, t)(Logits<kBf16>(a, row0 + tid)(x));
-        near = p > 0.0 && fabs(lhs * r.z - p) <= 1e-4 * p;
+        near = p > 0.0 && (fabs(lhs * r.z - p) <= 1e-4 * p || t < kTiny);
         no = !(lhs * r.z < p);
       }
     }
