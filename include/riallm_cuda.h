@@ -478,10 +478,14 @@ uint64_t riallm_cuda_paged_attention_workspace(const riallm_ctx* ctx, int32_t B,
 /* riallm_cuda_attention over pages: row b*T + t, at position
  * p = pos[b] + t, attends the held positions j <= p (and below max_pages *
  * page_size); with window > 0 only those with j > p - window or j < sinks.
- * Scores q.k / sqrt(d), softmax and the weighted sum of v in float32; q and
- * out are [B*T, nh*d] bf16, 16-byte aligned. A row that sees nothing
- * (p < 0, no page held) is zero. What the pools hold at positions that a row
- * does not see, infinities and NaN among it, does not change that row.
+ * Scores q.k / sqrt(d), the softmax's maximum and sum and the weighted sum of
+ * v are float32. What multiplies v is the weight to 15 bits (2^-15 of it)
+ * where a kv head has up to 16 rows a sequence (T * nh / nkv: single and few
+ * drafted tokens), the weight as bf16 (2^-8 of it) where it has more
+ * (prompts, many drafted tokens). q and out are [B*T, nh*d] bf16, 16-byte
+ * aligned. A row that sees nothing (p < 0, no page held) is zero. What the
+ * pools hold at positions that a row does not see, infinities and NaN among
+ * it, does not change that row; what a row does see of them, it shows.
  * The workspace is the caller's (256-byte aligned), needs no initial values,
  * and is free again when the call's work is done on `stream`; calls that may
  * overlap need one each. Nothing else is shared between calls. The kernel
@@ -525,8 +529,9 @@ uint64_t riallm_cuda_verify_draft_workspace(const riallm_ctx* ctx, int32_t B, in
  * the lowest token of the maximum (NaN left out).
  * tokens [B, n + 1] receives the accepted drafts, the sampled token, then
  * -1; accepted [B] the number of accepted drafts. p, its sums and the
- * comparisons are 64-bit, and results do not depend on the order in which
- * blocks run. n <= 255; with n == 0 (one sampled token per sequence)
+ * comparisons are 64-bit, its exponentials good to 2e-13 of themselves (a
+ * number that close to a border may fall on either side of it), and results
+ * do not depend on the order in which blocks run. n <= 255; with n == 0 (one sampled token per sequence)
  * draft_tokens and accept_u may be NULL. Workspace as above. */
 typedef struct riallm_verify_draft_args {
   const void* logits;

@@ -53,9 +53,12 @@ __device__ __forceinline__ void rope_angle(int64_t p, float f, float* s, float* 
 // pos[b] + t, and `hg` of its heads. A thread takes 8 dimensions of a head's
 // first half and the same 8 of its second (two 16-byte pieces): the pieces of
 // its first units are loaded before the angles are worked out, a row's d / 2
-// cosines and sines once for all of its heads. Bound by the bytes, qkv read
-// once and as much written: 8192 rows of 40 heads of 64 (84 MB) take 17.6 us,
-// 4.8 TB/s; 64 rows less than their launch.
+// cosines and sines once for all of its heads. qkv is read once and as much
+// written: 8192 rows of 40 heads of 64 (84 MB) take 17.6 us, 4.8 TB/s where
+// the HBM's 6.45 would take 13.0. Neither the HBM (30 % of its cycles; what is
+// written is in the L2 when the kernel ends) nor the issue slots (53 %) are
+// full: a CTA is one chain of load, angles, barrier and store, 42 % of the
+// warps' places taken. 64 rows take less than their launch.
 constexpr int kAppendRows = 4, kAppendThreads = 256, kAppendUnits = 4;  // units a thread
 template <int D>
 __global__ void __launch_bounds__(kAppendThreads)
@@ -407,10 +410,10 @@ __device__ __forceinline__ uint32_t odd16(uint32_t x) { return ((x & 0x7f807f80u
 // barrier with other warps until a group's end. The products are 1/40 of
 // what even these instructions can do at the rate the bytes arrive, so
 // nothing is gained by a 128-row tcgen05 tile of which 4 to 16 rows are
-// used. 8 kv heads of 128: one sequence of 131071 keys (537 MB) takes 98 us,
-// 5.5 TB/s; 96 of up to 16384 (3.3 GB) 530 to 570 us, 5.7 to 6.2 TB/s; 32 of
-// up to 2000 (135 MB) 32.6 us, of which the start, the groups' ends and
-// join_kernel are about 10. Two CTAs an SM, as 8 warps hide what one warp's
+// used. 8 kv heads of 128: one sequence of 131071 keys (537 MB) takes 99 us,
+// 5.4 TB/s; 96 of up to 16384 (3.3 GB) 564 to 570 us, 5.8 TB/s; 32 of up to
+// 2000 (135 MB) 32.3 us, of which the start, the groups' ends and join_kernel are
+// about 10. Two CTAs an SM, as 8 warps hide what one warp's
 // chain of load, product, maximum and product leaves open.
 constexpr int kFewWarps = 4;
 using Few = Shape<16, 64, 1>;
@@ -721,8 +724,14 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
 // 10 and 11 look through the values of blocks that some row of the tile does
 // not see whole. Keys and values share a ring of kStages blocks in smem.
 //
-// 4096 tokens, 32 heads of 128: 170 us, 810 TFLOP/s. Two times
-// 2501 tokens, heads of 64, window 2048: 103 us, 410 TFLOP/s (exponentials
+// The weights multiply the values as bf16, at most 2^-8 of a weight off and
+// 2^-9.5 in the mean: two products, as for few rows, would be half as much
+// tensor work again and, on the chain that bounds this, a subtraction and a
+// second conversion and store per weight. The result is 2.1e-3 from 64 bits,
+// where the output's own rounding is 1.6e-3.
+//
+// 4096 tokens, 32 heads of 128: 171 us, 800 TFLOP/s. Two times
+// 2501 tokens, heads of 64, window 2048: 104 us, 405 TFLOP/s (exponentials
 // alone: 36). 16 sequences of 6 tokens, 5 of them drafts, over up to 4001 keys
 // (147 MB): 43 us, 3.4 TB/s. A slot's block is a chain of product, maximum,
 // exponentials and product, 2500 of its 3700 cycles the weights'; the other
@@ -1130,7 +1139,9 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             m = mb;
           } else if (__any_sync(0xffffffffu, mb > m + 8.f)) {
             // Weights may exceed 1 (by up to 2^8) before the sums so far are
-            // brought down to a new maximum: that rarely happens then.
+            // brought down to a new maximum: that rarely happens then (the
+            // running maximum of Milakov and Gimelshein, 2018, and a
+            // threshold, which is published for attention on tensor memory).
             const float mn = mb > m + 8.f ? mb : m;
             const float f = m == mn ? 1.f : ex2(m - mn);
             m = mn;

@@ -26,13 +26,15 @@
 //                  every CTA of weigh_kernel;
 //   weigh_kernel : goes over the one row that the token comes from, in 64
 //                  bits, a chunk of the vocabulary per CTA; bound by its
-//                  instructions, 20 a token;
+//                  instructions, 30 a token at 67 % of the issue slots;
 //   pick_kernel  : the chunks' weights after the draft's distribution is taken
-//                  off; a sequence's last CTA finds the token. Bound by the
-//                  same.
+//                  off; a sequence's last CTA finds the token. 36 instructions
+//                  a token or more, 49 % of the slots: bound by the latency of
+//                  its start (a sum over all parts) and of 64-bit arithmetic
+//                  as well.
 // 128 sequences of 5 drafts over 128001 tokens (bf16 logits and float32 draft
 // probabilities, 262 MB): 100 us, 2.6 TB/s, of which the four take about 35,
-// 7, 22 and 36 %; one sequence: 16 us with the host's part. A cluster of CTAs
+// 7, 22 and 37 %; one sequence: 16 us with the host's part. A cluster of CTAs
 // per sequence in place of the last three takes 218 us (8 CTAs) or 352 (16):
 // its fixed cost, 10 us, comes 8 times over.
 #include <algorithm>
@@ -257,7 +259,8 @@ __global__ void __launch_bounds__(kThreads)
 // ------------------------------------------------------------ 64 bits
 //
 // e^((l - m) / t): 2^(i / 256) from a table and the rest, at most 1 / 512
-// octave, by the Taylor series to the 3rd power (error 1.4e-13). The table's
+// octave, by the Taylor series to the 3rd power (the 4th, 1.4e-13 of the value
+// at most, is the error). The table's
 // powers lie in their upper words below their exponents by i << 12, so that
 // adding i << 12 gives 2^(i / 256) for every i.
 struct Exp64 {
