@@ -531,8 +531,9 @@ uint64_t riallm_cuda_verify_draft_workspace(const riallm_ctx* ctx, int32_t B, in
  * -1; accepted [B] the number of accepted drafts. p, its sums and the
  * comparisons are 64-bit, its exponentials good to 2e-13 of themselves (a
  * number that close to a border may fall on either side of it), and results
- * do not depend on the order in which blocks run. n <= 255; with n == 0 (one sampled token per sequence)
- * draft_tokens and accept_u may be NULL. Workspace as above. */
+ * do not depend on the order in which blocks run. n <= 255; with n == 0 (one
+ * sampled token per sequence) draft_tokens and accept_u may be NULL.
+ * Workspace as above. */
 typedef struct riallm_verify_draft_args {
   const void* logits;
   const int32_t* draft_tokens;

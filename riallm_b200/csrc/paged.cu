@@ -412,9 +412,9 @@ __device__ __forceinline__ uint32_t odd16(uint32_t x) { return ((x & 0x7f807f80u
 // nothing is gained by a 128-row tcgen05 tile of which 4 to 16 rows are
 // used. 8 kv heads of 128: one sequence of 131071 keys (537 MB) takes 99 us,
 // 5.4 TB/s; 96 of up to 16384 (3.3 GB) 564 to 570 us, 5.8 TB/s; 32 of up to
-// 2000 (135 MB) 32.3 us, of which the start, the groups' ends and join_kernel are
-// about 10. Two CTAs an SM, as 8 warps hide what one warp's
-// chain of load, product, maximum and product leaves open.
+// 2000 (135 MB) 32.3 us, of which the start, the groups' ends and join_kernel
+// are about 10. Two CTAs an SM, as 8 warps hide what one warp's chain of load,
+// product, maximum and product leaves open.
 constexpr int kFewWarps = 4;
 using Few = Shape<16, 64, 1>;
 

@@ -260,9 +260,9 @@ __global__ void __launch_bounds__(kThreads)
 //
 // e^((l - m) / t): 2^(i / 256) from a table and the rest, at most 1 / 512
 // octave, by the Taylor series to the 3rd power (the 4th, 1.4e-13 of the value
-// at most, is the error). The table's
-// powers lie in their upper words below their exponents by i << 12, so that
-// adding i << 12 gives 2^(i / 256) for every i.
+// at most, is the error). The table's powers lie in their upper words below
+// their exponents by i << 12, so that adding i << 12 gives 2^(i / 256) for
+// every i.
 struct Exp64 {
   const double* table;  // in shared memory
   double k, m;          // 256 log2(e) / t
